@@ -11,16 +11,32 @@ HIPCC   ?= /opt/rocm/bin/hipcc
 ARCH    ?= gfx950
 CSRC    := nano_vllm_amd/csrc
 LIB     := nano_vllm_amd/libnvk_paged_attn.so
-HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -shared -Iinclude -I$(CSRC) \
-            -Wall -Wno-unused-function -fno-gpu-rdc
+# No packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this machine.
+# (A device feature: hipcc's host pass says that it does not know it, which is harmless.)
+HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Iinclude -I$(CSRC) -Wall -Wno-unused-function -fno-gpu-rdc \
+            -Xclang -target-feature -Xclang -packed-fp32-ops
+OBJ      := build/obj
+HIP_SRC  := nvk_paged_attn nvk_batch nvk_linear nvk_model nvk_shard nvk_rotary nvk_mx4 nvk_sparse
+CPP_SRC  := nvk_block_manager nvk_tokenizer nvk_model_group
+OBJS     := $(HIP_SRC:%=$(OBJ)/%.o) $(CPP_SRC:%=$(OBJ)/%.o)
+HEADERS  := $(wildcard $(CSRC)/*.h) include/nvk_paged_attn.h
 
 .PHONY: all lib cli oracle ref clean asm asan
 all: lib cli oracle ref
 
 lib: $(LIB)
 
-$(LIB): $(CSRC)/nvk_paged_attn.hip $(CSRC)/nvk_batch.hip $(CSRC)/nvk_linear.hip $(CSRC)/nvk_model.hip $(CSRC)/nvk_shard.hip $(CSRC)/nvk_kernels.hip.h $(CSRC)/nvk_addr.hip.h $(CSRC)/nvk_block_manager.cpp $(CSRC)/nvk_tokenizer.cpp $(CSRC)/nvk_model_group.cpp $(CSRC)/nvk_internal.h $(CSRC)/nvk_device_scope.h include/nvk_paged_attn.h
-	$(HIPCC) $(HIPFLAGS) -o $@ $(CSRC)/nvk_paged_attn.hip $(CSRC)/nvk_batch.hip $(CSRC)/nvk_linear.hip $(CSRC)/nvk_model.hip $(CSRC)/nvk_shard.hip $(CSRC)/nvk_block_manager.cpp $(CSRC)/nvk_tokenizer.cpp $(CSRC)/nvk_model_group.cpp -ldl -lpthread
+# one object per source (make -j builds them side by side; without -fgpu-rdc each carries its own device code)
+$(OBJ)/%.o: $(CSRC)/%.hip $(HEADERS) Makefile
+	@mkdir -p $(OBJ)
+	$(HIPCC) $(HIPFLAGS) -c -o $@ $<
+
+$(OBJ)/%.o: $(CSRC)/%.cpp $(HEADERS) Makefile
+	@mkdir -p $(OBJ)
+	$(HIPCC) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Iinclude -I$(CSRC) -Wall -c -o $@ $<
+
+$(LIB): $(OBJS)
+	$(HIPCC) --offload-arch=$(ARCH) -shared -fPIC -o $@ $(OBJS) -ldl -lpthread
 
 # the reference's command line over the library (tools/nvk_run.cpp): host-only C++ over the C ABI
 CLI := nano_vllm_amd/nvk_run
