@@ -170,14 +170,15 @@ def _stream():
 
 
 class _Slab:
-    """A device buffer of the library as torch sees it."""
+    """A device buffer of the library as torch sees it; a tensor made from it keeps it, and it keeps the buffer's owner."""
 
-    def __init__(self, ptr, shape, typestr="<f4"):
-        self.__cuda_array_interface__ = dict(shape=tuple(shape), typestr=typestr, data=(ptr, False), version=3, strides=None)
+    def __init__(self, owner, ptr, shape):
+        self.owner = owner
+        self.__cuda_array_interface__ = dict(shape=tuple(shape), typestr="<f4", data=(ptr, False), version=3, strides=None)
 
 
-def _view(ptr, shape):
-    return torch.as_tensor(_Slab(ptr, shape), device=DEV)
+def _view(owner, ptr, shape):
+    return torch.as_tensor(_Slab(owner, ptr, shape), device=DEV)
 
 
 def _quantise(x):
@@ -239,7 +240,7 @@ def _prepare_append(case, gen):
         s["q_out"] = torch.empty_like(s["q"])
         if case["cache"] == "fp32":
             s["pool"] = nv.PagedKVPool(1, blocks, bs, KV, hd)
-            s["slabs"] = tuple(_view(p, (blocks, bs, KV, hd)) for p in s["pool"].layer_ptrs(0))
+            s["slabs"] = tuple(_view(s["pool"], p, (blocks, bs, KV, hd)) for p in s["pool"].layer_ptrs(0))
         else:
             s["pool"] = nv.Mx4KVPool(1, blocks, bs, KV, hd)
             s["k_back"], s["v_back"] = torch.empty_like(s["k"]), torch.empty_like(s["v"])
@@ -308,7 +309,7 @@ def _prepare_sparse(case, gen):
 
         s["stream"] = _stream()
         s["pool"] = nv.PagedKVPool(1, blocks, bs, KV, hd)
-        k, v = (_view(p, shape) for p in s["pool"].layer_ptrs(0))
+        k, v = (_view(s["pool"], p, shape) for p in s["pool"].layer_ptrs(0))
         torch.add(mean, _randn(gen, *shape), alpha=0.7, out=k)
         v.copy_(_randn(gen, *shape))
         torch.cuda.synchronize()
@@ -321,7 +322,7 @@ def _prepare_sparse(case, gen):
             s["out"] = torch.empty_like(s["q"])
             s["chosen"] = torch.empty(len(ctx), KV, case["top"], device=DEV, dtype=torch.int32)
         else:
-            s["bounds"] = _view(s["index"].layer_ptr(0), (blocks, KV, 2, hd))
+            s["bounds"] = _view(s["index"], s["index"].layer_ptr(0), (blocks, KV, 2, hd))
         torch.cuda.synchronize()
     else:
         s["k"] = torch.add(mean, _randn(gen, *shape), alpha=0.7)
