@@ -391,6 +391,148 @@ long long nvk_host_cache_staged_bytes(int reset);
  * ref: the layer slicing in LlamaModel::attention, include/core/model.hpp:400-403. */
 int nvk_bind_pool(nvk_pool *pool, int layer);
 
+/* ------------------------------------------------ rotary tables and the fused append --
+ * RoPE in the forms that checkpoints beyond the reference's use.  The reference rotates adjacent pairs over the whole head,
+ * unscaled and without a norm (Ops::apply_rope, include/ops/positional.hpp:13-39): NVK_ROPE_INTERLEAVED, rotary_dim =
+ * head_dim, NVK_ROPE_SCALE_NONE.
+ *   layout      INTERLEAVED pairs channels (2i, 2i+1), HALF pairs (i, i + rotary_dim/2)
+ *   rotary_dim  the first rotary_dim channels turn (even, <= head_dim <= 256); the rest pass through
+ *   scaling     angle per position of pair i, f_i = theta^(-2i/rotary_dim) unscaled:
+ *     LINEAR    f_i / factor
+ *     NTK       the base becomes theta * factor^(rotary_dim / (rotary_dim - 2)); rotary_dim > 2
+ *     YARN      a pair that turns t = original_len * f_i / 2 pi times over original_len keeps the share
+ *               clamp((t - 1) / 31, 0, 1) of f_i, the rest is divided by factor; cos and sin are multiplied by
+ *               0.1 ln(factor) + 1
+ *     factor >= 1; original_len > 0 for YARN; both ignored otherwise
+ * The table is made on the host in 64 bits and does not change: it may be used from any stream of its device.
+ * nvk_rope_destroy waits for the device. */
+#define NVK_ROPE_INTERLEAVED 0
+#define NVK_ROPE_HALF 1
+#define NVK_ROPE_SCALE_NONE 0
+#define NVK_ROPE_SCALE_LINEAR 1
+#define NVK_ROPE_SCALE_NTK 2
+#define NVK_ROPE_SCALE_YARN 3
+typedef struct nvk_rope nvk_rope;
+int nvk_rope_create(int head_dim, int rotary_dim, int layout, double theta, int scaling, double factor, int original_len,
+                    int device, nvk_rope **out_rope);
+int nvk_rope_destroy(nvk_rope *rope);
+/* number of pairs (at most cap written to freq: angle per position of each); *factor (may be NULL) = the factor on cos, sin */
+int nvk_rope_frequencies(const nvk_rope *rope, double *freq, int cap, double *factor);
+
+/* RMS norm of each query and key head + rotation + append to the cache, one launch; `rows` token rows in all.
+ *   q [rows, n_heads, head_dim] -> q_out (the same shape; may be q itself, must not overlap it otherwise)
+ *   k_rows, v_rows [rows, n_kv_heads, head_dim]: keys normed and rotated, values as they are, into the slot of their token
+ *   q_weight, k_weight [head_dim]: y = x / sqrt(mean(x^2) + eps) * weight before the rotation; NULL = no norm
+ *   rope        NULL = no rotation
+ *   row_seqs    [rows] table row of each token row; NULL = row r belongs to sequence r
+ *   positions   [rows] position of each row's token; negative = a row of padding: nothing of it is read or written
+ *   block_tables [num_seqs, max_blocks]
+ * Either q and q_out or k_rows and v_rows may be NULL (append only; rotate only: then positions alone matter).
+ * All sums, angles and products are held in 64 bits and rounded once, to fp32 or to the cache's 4 bits.
+ * ptr_kind says where every array lives.  NVK_PTR_HOST: validates (positions inside their table, blocks inside the pool, no
+ * two rows in one slot), stages, runs, synchronises.  NVK_PTR_DEVICE: asynchronous on `stream` (NULL = the pool's), nothing
+ * is allocated; a row whose sequence or position has no place in the tables is left alone, one whose block lies outside the
+ * pool is rotated but not stored; two rows of one slot leave a mix of both there. */
+int nvk_pool_norm_rope_append(nvk_pool *pool, int layer, const nvk_rope *rope, int rows, int n_heads, const float *q,
+                              float *q_out, const float *k_rows, const float *v_rows, const float *q_weight,
+                              const float *k_weight, float eps, const int *row_seqs, const int *positions,
+                              const int *block_tables, int num_seqs, int max_blocks, int ptr_kind, void *stream);
+
+/* --------------------------------------------------------- the 4-bit paged KV cache --
+ * The reference's cache (include/core/model.hpp:94-97) in 17/32 byte a value instead of 4: each value is
+ * sign * {0, .5, 1, 1.5, 2, 3, 4, 6} * 2^e (e2m1), with one e (a byte) for each 32 channels of a row, the smallest with
+ * |values| <= 7 * 2^e; the last group is what is left of the row.  Values go to the nearest, ties to the even code.  A group
+ * that holds an infinity or a NaN is stored as NaN.  Block tables, positions and contexts are those of nvk_pool.
+ *   block_size  a multiple of 16;  head_dim  a multiple of 8, at most 256 (stored as 32, 64, 128 or 256 channels)
+ * Zero-initialised.  The layout inside a layer is the library's (nvk_mx4_pool_layer_ptr / _layer_bytes: for copies of whole
+ * layers between pools of one geometry).
+ * Streams and threads as for nvk_pool: one workspace per pool, so attention launches on a pool must be ordered with
+ * respect to each other.  Entry points that may have to grow the workspace (the attention calls) refuse to under stream
+ * capture; nvk_mx4_pool_reserve_workspace sizes it beforehand, and _workspace_generation counts its moves (a captured
+ * graph holds its address). */
+typedef struct nvk_mx4_pool nvk_mx4_pool;
+int nvk_mx4_pool_create(int n_layers, int num_blocks, int block_size, int n_kv_heads, int head_dim, int device,
+                        nvk_mx4_pool **out_pool);
+int nvk_mx4_pool_destroy(nvk_mx4_pool *pool); /* waits for the device */
+/* out6 = {n_layers, num_blocks, block_size, n_kv_heads, head_dim, device} */
+int       nvk_mx4_pool_geometry(const nvk_mx4_pool *pool, int *out6);
+long long nvk_mx4_pool_layer_bytes(const nvk_mx4_pool *pool);
+int       nvk_mx4_pool_layer_ptr(const nvk_mx4_pool *pool, int layer, void **base_dev);
+int       nvk_mx4_pool_stream(const nvk_mx4_pool *pool, void **stream);
+int       nvk_mx4_pool_synchronize(nvk_mx4_pool *pool);
+/* total_rows, max_rows: query rows in all and of one sequence (decode: num_seqs and 1) */
+int       nvk_mx4_pool_reserve_workspace(nvk_mx4_pool *pool, int num_seqs, int n_heads, int total_rows, int max_rows, int max_ctx);
+long long nvk_mx4_pool_workspace_generation(const nvk_mx4_pool *pool);
+/* nvk_pool_norm_rope_append into the 4-bit cache (rope, weights NULL: a plain append) */
+int nvk_mx4_pool_norm_rope_append(nvk_mx4_pool *pool, int layer, const nvk_rope *rope, int rows, int n_heads, const float *q,
+                                  float *q_out, const float *k_rows, const float *v_rows, const float *q_weight,
+                                  const float *k_weight, float eps, const int *row_seqs, const int *positions,
+                                  const int *block_tables, int num_seqs, int max_blocks, int ptr_kind, void *stream);
+/* What the cache holds for the given rows, as fp32: k_out, v_out [rows, n_kv_heads, head_dim].  Rows without a place (as
+ * above) are left as they were. */
+int nvk_mx4_pool_read_rows(nvk_mx4_pool *pool, int layer, int rows, const int *row_seqs, const int *positions,
+                           const int *block_tables, int num_seqs, int max_blocks, float *k_out, float *v_out, int ptr_kind,
+                           void *stream);
+
+/* Attention over the 4-bit cache: the arithmetic of nvk_decode / nvk_prefill (products exact, sums in fp32) over the
+ * values it holds.  A context of 0 tokens gives a zero row.  Codes of tokens that a row does not see never reach it, also
+ * where they are NaN.
+ *   decode   q, out [num_seqs, n_heads, head_dim]; sequence s attends to ctx_lens[s] tokens
+ *   prefill  q, out [total_rows, n_heads, head_dim]; sequence s has rows row_offsets[s] .. row_offsets[s+1] - 1 (an
+ *            ascending list of num_seqs + 1, starting at 0), the newest of its ctx_lens[s] tokens, and each sees the tokens up
+ *            to its own.  The chunk's keys and values must be in the cache.  A sequence without rows is skipped; rows
+ *            beyond the last offset are left as they were.
+ * Host-pointer forms: validate tables and lengths, stage, run, synchronise (prefill takes chunk_lens [num_seqs] instead of
+ * offsets).  Device-pointer forms: asynchronous on `stream` (NULL = the pool's); max_ctx >= every ctx_lens[s] and
+ * max_rows >= every chunk size the launch, lengths are read on the device; table entries are clamped to the pool. */
+int nvk_mx4_decode(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, const float *q, const int *block_tables,
+                   int max_blocks, const int *ctx_lens, float *out);
+int nvk_mx4_decode_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, const float *q_dev,
+                          const int *block_tables_dev, int max_blocks, const int *ctx_lens_dev, int max_ctx, float *out_dev,
+                          void *stream);
+int nvk_mx4_prefill(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, const float *q, const int *block_tables,
+                    int max_blocks, const int *chunk_lens, const int *ctx_lens, float *out);
+int nvk_mx4_prefill_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, int total_rows, const float *q_dev,
+                           const int *row_offsets_dev, int max_rows, const int *block_tables_dev, int max_blocks,
+                           const int *ctx_lens_dev, int max_ctx, float *out_dev, void *stream);
+
+/* ------------------------------------------------------- block-sparse decode --
+ * Decode attention that reads the blocks a cheap score selects, for long contexts; the cache is an nvk_pool (head_dim a
+ * multiple of 4, at most 256).  An index beside the pool keeps the least (lo) and the largest (hi) key element of each block,
+ * kv-head and channel: [layer][block][kv-head][lo | hi][head_dim] fp32, 1 / (2 block_size) of the pool, zero like a new pool.
+ * For a query head q, q . k <= sum_c max(q_c, 0) hi_c + min(q_c, 0) lo_c for every key k of a block; a block's score for a kv-head
+ * is the largest of these over the group's query heads (summed in 64 bits, rounded to fp32; a score that is no number
+ * counts as infinite).  For each (sequence, kv-head) a call reads
+ *   the first first_blocks and the last last_blocks (at least 1: the newest block) of the context, and
+ *   the best-scored others, equal scores lowest block first, up to top_blocks in all -- or every block, if there are no more.
+ * Over those the result is nvk_decode's.  A context of 0 tokens gives a zero row.
+ *
+ * nvk_block_index_update: behind an append (any entry point that writes keys), brings the blocks that hold the tokens
+ * [starts[s], ctx_lens[s]) of each sequence up to date, from all their tokens below ctx_lens[s].  The newest block is always
+ * read, so a block has to be up to date only once it is no longer among the last ones.  max_new >= every ctx_lens[s] -
+ * starts[s] sizes the launch.
+ * selected [num_seqs, n_kv_heads, top_blocks] (may be NULL): the logical blocks read, ascending, filled up with -1.
+ * Host-pointer forms (ptr_kind NVK_PTR_HOST, nvk_sparse_decode) validate, stage, run, synchronise; device-pointer forms are
+ * asynchronous on `stream` (NULL = the pool's), max_ctx >= every ctx_lens[s], q 16-byte aligned; table entries outside the pool are
+ * clamped for reading and skipped by an update.  Scores, lists and partial results live in one workspace of the index: decode
+ * calls on an index must be ordered with respect to each other; a call that would have to grow it under stream capture is refused
+ * (nvk_block_index_reserve_workspace).  The index must be destroyed before its pool; destroying waits for the device. */
+typedef struct nvk_block_index nvk_block_index;
+int       nvk_block_index_create(nvk_pool *pool, nvk_block_index **out_index);
+int       nvk_block_index_destroy(nvk_block_index *index);
+int       nvk_block_index_layer_ptr(const nvk_block_index *index, int layer, void **bounds_dev);
+int       nvk_block_index_reserve_workspace(nvk_block_index *index, int num_seqs, int n_heads, int max_ctx, int top_blocks);
+long long nvk_block_index_workspace_generation(const nvk_block_index *index);
+int       nvk_block_index_update(nvk_block_index *index, int layer, int num_seqs, const int *block_tables, int max_blocks,
+                                 const int *starts, const int *ctx_lens, int max_new, int ptr_kind, void *stream);
+int       nvk_sparse_decode(nvk_block_index *index, int layer, int num_seqs, int n_heads, const float *q, const int *block_tables,
+                            int max_blocks, const int *ctx_lens, int top_blocks, int first_blocks, int last_blocks, float *out,
+                            int *selected);
+int       nvk_sparse_decode_device(nvk_block_index *index, int layer, int num_seqs, int n_heads, const float *q_dev,
+                                   const int *block_tables_dev, int max_blocks, const int *ctx_lens_dev, int max_ctx,
+                                   int top_blocks, int first_blocks, int last_blocks, float *out_dev, int *selected_dev,
+                                   void *stream);
+
 /* ------------------------------------------------------- head-sharded decode --
  * The decode layer-call split over the G GPUs of one node by kv-head group.  The reference has one
  * process and no collective; heads are independent in it (q-head loop outermost, include/core/attention.hpp:102,

@@ -36,6 +36,13 @@ PREFILL_AUTO = 0
 PREFILL_ROWWISE = 1
 PREFILL_TILED = 2
 
+ROPE_INTERLEAVED = 0
+ROPE_HALF = 1
+ROPE_SCALE_NONE = 0
+ROPE_SCALE_LINEAR = 1
+ROPE_SCALE_NTK = 2
+ROPE_SCALE_YARN = 3
+
 HOST_CACHE_RESTAGE = 0
 HOST_CACHE_APPEND_ONLY = 1
 
@@ -190,6 +197,37 @@ SIGNATURES = {
     "nvk_batch_layer": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _vp, C.c_float, _vp]),
     "nvk_batch_end_step": (C.c_int, [_vp]),
     "nvk_batch_stats": (C.c_int, [_vp, C.POINTER(C.c_longlong)]),
+    "nvk_rope_create": (C.c_int, [C.c_int] * 3 + [C.c_double, C.c_int, C.c_double, C.c_int, C.c_int, C.POINTER(_vp)]),
+    "nvk_rope_destroy": (C.c_int, [_vp]),
+    "nvk_rope_frequencies": (C.c_int, [_vp, C.POINTER(C.c_double), C.c_int, C.POINTER(C.c_double)]),
+    "nvk_pool_norm_rope_append": (C.c_int, [_vp, C.c_int, _vp, C.c_int, C.c_int] + [_vp] * 6 + [C.c_float] + [_vp] * 3
+                                  + [C.c_int, C.c_int, C.c_int, _vp]),
+    "nvk_mx4_pool_create": (C.c_int, [C.c_int] * 6 + [C.POINTER(_vp)]),
+    "nvk_mx4_pool_destroy": (C.c_int, [_vp]),
+    "nvk_mx4_pool_geometry": (C.c_int, [_vp, _i]),
+    "nvk_mx4_pool_layer_bytes": (C.c_longlong, [_vp]),
+    "nvk_mx4_pool_layer_ptr": (C.c_int, [_vp, C.c_int, C.POINTER(_vp)]),
+    "nvk_mx4_pool_stream": (C.c_int, [_vp, C.POINTER(_vp)]),
+    "nvk_mx4_pool_synchronize": (C.c_int, [_vp]),
+    "nvk_mx4_pool_reserve_workspace": (C.c_int, [_vp] + [C.c_int] * 5),
+    "nvk_mx4_pool_workspace_generation": (C.c_longlong, [_vp]),
+    "nvk_mx4_pool_norm_rope_append": (C.c_int, [_vp, C.c_int, _vp, C.c_int, C.c_int] + [_vp] * 6 + [C.c_float] + [_vp] * 3
+                                      + [C.c_int, C.c_int, C.c_int, _vp]),
+    "nvk_mx4_pool_read_rows": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp]),
+    "nvk_mx4_decode": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, _vp]),
+    "nvk_mx4_decode_device": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, C.c_int, _vp, _vp]),
+    "nvk_mx4_prefill": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, _vp, _vp]),
+    "nvk_mx4_prefill_device": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int,
+                                         _vp, _vp]),
+    "nvk_block_index_create": (C.c_int, [_vp, C.POINTER(_vp)]),
+    "nvk_block_index_destroy": (C.c_int, [_vp]),
+    "nvk_block_index_layer_ptr": (C.c_int, [_vp, C.c_int, C.POINTER(_vp)]),
+    "nvk_block_index_reserve_workspace": (C.c_int, [_vp] + [C.c_int] * 4),
+    "nvk_block_index_workspace_generation": (C.c_longlong, [_vp]),
+    "nvk_block_index_update": (C.c_int, [_vp, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int, _vp]),
+    "nvk_sparse_decode": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp] + [C.c_int] * 3 + [_vp, _vp]),
+    "nvk_sparse_decode_device": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp] + [C.c_int] * 4
+                                 + [_vp, _vp, _vp]),
     "nvk_bm_create": (C.c_int, [C.c_int, C.c_int, C.POINTER(_vp)]),
     "nvk_bm_destroy": (None, [_vp]),
     "nvk_bm_allocate_block": (C.c_int, [_vp]),

@@ -1,0 +1,568 @@
+// nvk_rotary.hip -- from projected rows to the paged cache in one launch: RMS norm of each query and key head, rotary
+// positions, append (nvk_rope_*, nvk_pool_norm_rope_append, nvk_mx4_pool_norm_rope_append), and the way back from the 4-bit
+// cache (nvk_mx4_pool_read_rows).
+//
+// The mathematics, for one head row x of a token at position p:
+//     y = x / sqrt(mean(x^2) + eps) * w                       (only where a weight is given)
+//     (a, b) -> (a c - b s, a s + b c),  c = m cos(p f_i), s = m sin(p f_i), i = 0 .. rotary_dim / 2 - 1
+// Pair i is (y[2i], y[2i+1]) or (y[i], y[i + rotary_dim/2]); channels from rotary_dim on pass through.  The reference knows
+// the first pairing over the whole head, unscaled and without a norm (Ops::apply_rope, include/ops/positional.hpp:13-39).
+//
+// Everything between the loaded row and the stored value is computed in 64 bits and rounded once: a key that is stored in
+// 4 bits is then the nearest code of the exact value, whatever the order of the sums, and the angle of a far position keeps
+// its fraction (p f to 2^-53 relative; in fp32 a position of 100 000 would leave 2^-7 of a radian).  It costs little: the
+// kernel is bound by the rows it moves, and MI355X adds and multiplies fp64 at the unpacked fp32 rate.
+// gfx950 only; no CPU path.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "nvk_addr.hip.h"
+#include "nvk_hip_util.h"
+#include "nvk_mx4.hip.h"
+
+struct nvk_rope
+{
+    int                 head_dim = 0, rotary_dim = 0, layout = 0, device = 0;
+    double              factor   = 1.0; // m, on cos and sin
+    double             *freq_dev = nullptr;
+    std::vector<double> freq;
+};
+
+namespace nvk {
+
+constexpr int kRotaryMaxHead = 256; // channels of a head row
+constexpr int kRotaryBatch   = 512; // values a wave holds at a time: 8 per lane
+constexpr int kRotaryWaves   = 4;
+
+struct RotaryArgs
+{
+    const float  *q, *k, *v;   // [rows, heads, head_dim]; q or (k and v) may be null
+    float        *q_out;
+    const float  *q_weight, *k_weight; // [head_dim] or null
+    double        eps;
+    const double *freq; // [rotary_dim / 2] or null
+    double        factor;
+    int           rotary_dim, half_layout;
+    const int    *row_seqs, *positions, *tables;
+    int           num_seqs, max_blocks, n_heads;
+    float        *k_slab, *v_slab; // fp32 cache
+    Mx4Layer      mx;              // its geometry also for the fp32 cache; base and kk only for the 4-bit one
+};
+
+// channels of pair p of a head row: rotated pairs first, then what is left two by two
+__device__ __forceinline__ void pair_channels(const RotaryArgs &a, int p, int &ia, int &ib)
+{
+    const int half = a.rotary_dim >> 1;
+    if (p < half && a.half_layout)
+        ia = p, ib = p + half;
+    else
+        ia = 2 * p, ib = 2 * p + 1;
+}
+
+// One workgroup takes row blockIdx.x; its waves (and those of gridDim.y workgroups) share the row's heads in batches of
+// kRotaryBatch values.  W lanes hold one head row, PPL pairs each; U head rows are in flight in a lane.
+// For the 4-bit cache the batch then crosses LDS, after which a lane holds eight neighbouring channels: one dword of codes.
+template <int W, int PPL, bool MX4>
+__global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel(const RotaryArgs a)
+{
+    constexpr int U = PPL == 2 ? 2 : 4; // head rows per lane at a time
+    constexpr int R = 64 / W;           // head rows side by side in a wave
+    constexpr int HB = U * R;           // head rows per batch
+    __shared__ double2 s_cs[kRotaryMaxHead / 2];
+    __shared__ double  s_row[MX4 ? kRotaryWaves : 1][MX4 ? kRotaryBatch : 1];
+
+    const int row = blockIdx.x;
+    const int pos = a.positions[row];
+    const int seq = a.row_seqs ? a.row_seqs[row] : row;
+    const int bs = a.mx.block_size;
+    // rows of padding, and rows that have no place in their table, are left alone (uniform over the workgroup)
+    if (pos < 0 || (a.k && (seq < 0 || seq >= a.num_seqs || pos / bs >= a.max_blocks)))
+        return;
+    const int  hd = a.mx.head_dim, pairs = hd >> 1, kv = a.mx.n_kv_heads;
+    const int  turned = a.freq ? a.rotary_dim >> 1 : 0;
+    if (turned) {
+        for (int p = threadIdx.x; p < turned; p += blockDim.x) {
+            double s, c;
+            sincos((double)pos * a.freq[p], &s, &c);
+            s_cs[p] = make_double2(a.factor * c, a.factor * s);
+        }
+        __syncthreads();
+    }
+    const int  block = a.k ? a.tables[(int64_t)seq * a.max_blocks + pos / bs] : 0;
+    const int  offset = pos % bs;
+    const bool keep = a.k && block >= 0 && block < a.mx.num_blocks;
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int sub = lane / W, lw = lane % W; // which of the wave's head rows, and the lane's place in it
+    const int kb = a.k ? (kv + HB - 1) / HB : 0, qb = a.q ? (a.n_heads + HB - 1) / HB : 0;
+    const int batches = 2 * kb + qb; // keys, values, queries
+
+    for (int t = blockIdx.y * kRotaryWaves + wave; t < batches; t += gridDim.y * kRotaryWaves) {
+        const int    kind = t < kb ? 0 : t < 2 * kb ? 1 : 2; // key, value, query
+        const int    head0 = (t - (kind == 0 ? 0 : kind == 1 ? kb : 2 * kb)) * HB;
+        const int    heads = kind == 2 ? a.n_heads : kv;
+        const float *src = (kind == 0 ? a.k : kind == 1 ? a.v : a.q) + (int64_t)row * heads * hd;
+        const float *weight = kind == 0 ? a.k_weight : kind == 1 ? nullptr : a.q_weight;
+        const int    turn = kind == 1 ? 0 : turned;
+        if (kind < 2 && !keep)
+            continue;
+
+        float2 x[U][PPL];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < PPL; j++) {
+                const int head = head0 + u * R + sub, p = lw + j * W;
+                int       ia, ib;
+                pair_channels(a, p, ia, ib);
+                x[u][j] = make_float2(0.f, 0.f);
+                if (head < heads && p < pairs)
+                    x[u][j] = make_float2(src[head * hd + ia], src[head * hd + ib]);
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int head = head0 + u * R + sub;
+            double    scale = 1.0;
+            if (weight) {
+                double ss = 0.0;
+#pragma unroll
+                for (int j = 0; j < PPL; j++)
+                    ss = fma((double)x[u][j].x, (double)x[u][j].x, fma((double)x[u][j].y, (double)x[u][j].y, ss));
+#pragma unroll
+                for (int o = W / 2; o > 0; o >>= 1)
+                    ss += __shfl_xor(ss, o);
+                scale = 1.0 / sqrt(ss / hd + a.eps);
+            }
+#pragma unroll
+            for (int j = 0; j < PPL; j++) {
+                const int p = lw + j * W;
+                int       ia, ib;
+                pair_channels(a, p, ia, ib);
+                const bool there = head < heads && p < pairs;
+                double     ya = x[u][j].x, yb = x[u][j].y;
+                if (weight && there)
+                    ya = ya * scale * (double)weight[ia], yb = yb * scale * (double)weight[ib];
+                if (p < turn) {
+                    const double2 cs = s_cs[p];
+                    const double  na = ya * cs.x - yb * cs.y;
+                    yb               = ya * cs.y + yb * cs.x;
+                    ya               = na;
+                }
+                if (!there)
+                    continue;
+                if (MX4 && kind < 2) {
+                    s_row[wave][(u * R + sub) * hd + ia] = ya;
+                    s_row[wave][(u * R + sub) * hd + ib] = yb;
+                }
+                else {
+                    float *dst;
+                    if (kind == 2)
+                        dst = a.q_out + ((int64_t)row * heads + head) * hd;
+                    else
+                        dst = (kind == 0 ? a.k_slab : a.v_slab)
+                              + row_float_index(block, offset, head, bs, kv, hd);
+                    dst[ia] = (float)ya, dst[ib] = (float)yb;
+                }
+            }
+        }
+        if constexpr (MX4) {
+            if (kind < 2) { // (the wave's own part of LDS: written and read by the same wave, in order)
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                const int  octets = hd >> 3; // dwords of codes per head row
+                const int  mine = lane / octets, c0 = (lane % octets) * 8, head = head0 + mine;
+                const bool there = mine < HB && head < heads;
+                double     y[8], amax = 0.0;
+                bool       finite = true;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    y[i] = there ? s_row[wave][mine * hd + c0 + i] : 0.0;
+                    amax = fmax(amax, fabs(y[i]));
+                    finite = finite && fabs(y[i]) < INFINITY;
+                }
+                // the group of 32 channels is four lanes, or what is left of the row (rows of 48 or 56 channels are 6 or 7
+                // lanes: partners go by the place in the row, and each lane asks all of them)
+                const int    group = c0 / 32;
+                const double amax_own = amax;
+                const int    bad_own = finite ? 0 : 1;
+                int          bad = bad_own;
+#pragma unroll
+                for (int o = 1; o <= 3; o++) {
+                    const int pc = (((c0 >> 3) & 3) ^ o) + 4 * group;
+                    const int from = pc < octets ? mine * octets + pc : lane;
+                    amax = fmax(amax, __shfl(amax_own, from));
+                    bad |= __shfl(bad_own, from);
+                }
+                if (there) {
+                    const unsigned sb = bad ? 255u : (unsigned)mx4_scale_byte(amax);
+                    const double   inv = __longlong_as_double((long long)(1023 - ((int)sb - 127)) << 52);
+                    unsigned       word = 0;
+                    if (!bad)
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            word |= mx4_code(y[i] * inv) << (4 * i);
+                    const int      kk = a.mx.kk, tok = offset % kMx4Tile;
+                    unsigned char *tile = a.mx.tile(block, offset, head);
+                    if (kind == 0)
+                        *reinterpret_cast<unsigned *>(tile + tok * 16 * kk + c0 / 2) = word;
+                    else if (kk >= 4)
+                        *reinterpret_cast<unsigned *>(tile + mx4_v_at(kk) + mx4_v_byte(tok, c0, kk)) = word;
+                    else
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            tile[mx4_v_at(kk) + mx4_v_byte(tok, c0 + 2 * i, kk)] = (unsigned char)(word >> (8 * i));
+                    if (c0 % 32 == 0)
+                        tile[(kind == 0 ? mx4_ks_at(kk) : mx4_vs_at(kk)) + group * kMx4Tile + tok] = (unsigned char)sb;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+    }
+}
+
+// ---- the values of cached rows: one thread per 8 channels of (row, kv-head) -----------------------------------------
+__global__ void __launch_bounds__(256)
+    nvk_mx4_read_rows_kernel(const Mx4Layer mx, const int *__restrict__ row_seqs, const int *__restrict__ positions,
+                             const int *__restrict__ tables, int num_seqs, int max_blocks, float *__restrict__ k_out,
+                             float *__restrict__ v_out)
+{
+    const int row = blockIdx.x;
+    const int pos = positions[row], seq = row_seqs ? row_seqs[row] : row, bs = mx.block_size;
+    if (pos < 0 || seq < 0 || seq >= num_seqs || pos / bs >= max_blocks)
+        return;
+    const int block = tables[(int64_t)seq * max_blocks + pos / bs], offset = pos % bs, tok = offset % kMx4Tile;
+    if (block < 0 || block >= mx.num_blocks)
+        return;
+    const int octets = mx.head_dim >> 3, kk = mx.kk;
+    for (int i = threadIdx.x; i < mx.n_kv_heads * octets; i += blockDim.x) {
+        const int            head = i / octets, c0 = (i % octets) * 8;
+        const unsigned char *tile = mx.tile(block, offset, head);
+        unsigned             kw = *reinterpret_cast<const unsigned *>(tile + tok * 16 * kk + c0 / 2), vw = 0;
+        if (kk >= 4)
+            vw = *reinterpret_cast<const unsigned *>(tile + mx4_v_at(kk) + mx4_v_byte(tok, c0, kk));
+        else
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                vw |= (unsigned)tile[mx4_v_at(kk) + mx4_v_byte(tok, c0 + 2 * j, kk)] << (8 * j);
+        const unsigned ks = tile[mx4_ks_at(kk) + (c0 / 32) * kMx4Tile + tok], vs = tile[mx4_vs_at(kk) + (c0 / 32) * kMx4Tile + tok];
+        const int64_t  at = ((int64_t)row * mx.n_kv_heads + head) * mx.head_dim + c0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            k_out[at + j] = mx4_value((kw >> (4 * j)) & 15u, ks);
+            v_out[at + j] = mx4_value((vw >> (4 * j)) & 15u, vs);
+        }
+    }
+}
+
+} // namespace nvk
+
+namespace {
+
+using nvk::RotaryArgs;
+
+constexpr int kCus = 256; // MI355X
+
+template <bool MX4> void launch_rotary(const RotaryArgs &a, int rows, hipStream_t st)
+{
+    const int hd = a.mx.head_dim, pairs = hd / 2;
+    const int w = pairs <= 16 ? 16 : pairs <= 32 ? 32 : 64;
+    const int hb = pairs > 64 ? 2 : 4 * (64 / w);
+    const int batches = (a.k ? 2 * ((a.mx.n_kv_heads + hb - 1) / hb) : 0) + (a.q ? (a.n_heads + hb - 1) / hb : 0);
+    // Few rows: a row's batches are spread over several workgroups (each computes the row's angles again, side by side), up
+    // to one batch per wave, until the launch has two workgroups for every CU.
+    const int most = (batches + nvk::kRotaryWaves - 1) / nvk::kRotaryWaves;
+    const int parts = std::max(1, std::min(most, (2 * kCus + rows - 1) / rows));
+    const dim3 grid((unsigned)rows, (unsigned)parts), block(64 * nvk::kRotaryWaves);
+    if (pairs > 64)
+        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<64, 2, MX4>), grid, block, 0, st, a);
+    else if (w == 64)
+        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<64, 1, MX4>), grid, block, 0, st, a);
+    else if (w == 32)
+        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<32, 1, MX4>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<16, 1, MX4>), grid, block, 0, st, a);
+}
+
+// Host-pointer calls: every row has a place of its own.  (Two rows in one slot: whichever comes last would stay, or a mix.)
+int check_rows(int rows, const int *row_seqs, const int *positions, const int *tables, int num_seqs, int max_blocks,
+               int block_size, int num_blocks, bool own_slots, const char *who)
+{
+    try {
+        std::vector<long long> slots;
+        for (int r = 0; r < rows; r++) {
+            const int pos = positions[r], seq = row_seqs ? row_seqs[r] : r;
+            if (pos < 0)
+                continue; // padding
+            if (seq < 0 || seq >= num_seqs || pos / block_size >= max_blocks)
+                return nvk::fail(NVK_ERR_INVALID_ARG, "%s: row %d: position %d of sequence %d outside its table", who, r, pos, seq);
+            const int pb = tables[(size_t)seq * max_blocks + pos / block_size];
+            if (pb < 0 || pb >= num_blocks)
+                return nvk::fail(NVK_ERR_BAD_BLOCK, "%s: block %d of sequence %d outside [0,%d)", who, pb, seq, num_blocks);
+            slots.push_back((long long)pb * block_size + pos % block_size);
+        }
+        if (own_slots) {
+            std::sort(slots.begin(), slots.end());
+            if (std::adjacent_find(slots.begin(), slots.end()) != slots.end())
+                return nvk::fail(NVK_ERR_INVALID_ARG, "%s: two rows share one slot of the cache", who);
+        }
+    }
+    catch (const std::bad_alloc &) {
+        return nvk::fail(NVK_ERR_OOM, "%s: host allocation failed", who);
+    }
+    return NVK_OK;
+}
+
+bool aligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+// The part that the two caches share: checks, staging of host arrays, launch.
+template <bool MX4>
+int norm_rope_append(RotaryArgs a, int device, hipStream_t own_stream, const nvk_rope *rope, int rows,
+                     int ptr_kind, void *stream, const char *who)
+{
+    const int hd = a.mx.head_dim, bs = a.mx.block_size, kv = a.mx.n_kv_heads;
+    if (ptr_kind != NVK_PTR_HOST && ptr_kind != NVK_PTR_DEVICE)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: ptr_kind %d", who, ptr_kind);
+    if (rows < 0 || a.num_seqs < 0 || (a.k && a.max_blocks <= 0) || a.n_heads <= 0 || !(a.eps >= 0.0))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: bad arguments (rows %d, num_seqs %d, max_blocks %d, n_heads %d)", who, rows,
+                         a.num_seqs, a.max_blocks, a.n_heads);
+    if (hd % 2 != 0 || hd > nvk::kRotaryMaxHead)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: head_dim %d (even, at most %d)", who, hd, nvk::kRotaryMaxHead);
+    if (a.k && (long long)a.max_blocks * bs > 0x7fffffffLL)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: a table of %d blocks of %d tokens passes 2^31 tokens", who, a.max_blocks, bs);
+    if (rope && (rope->head_dim != hd || rope->device != device))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: the rotary table is for head_dim %d on device %d, the pool has %d on %d", who,
+                         rope->head_dim, rope->device, hd, device);
+    if (rows == 0)
+        return NVK_OK;
+    if ((!a.q && !a.k) || (a.q != nullptr) != (a.q_out != nullptr) || (a.k != nullptr) != (a.v != nullptr))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: q and q_out, k_rows and v_rows come in pairs, at least one of them", who);
+    if (!a.positions || (a.k && !a.tables))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: positions or block_tables missing", who);
+    if (!aligned(a.q, 4) || !aligned(a.q_out, 4) || !aligned(a.k, 4) || !aligned(a.v, 4))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: rows are not aligned to their type", who);
+
+    NVK_SCOPE(device);
+    hipStream_t st = (ptr_kind == NVK_PTR_DEVICE && stream) ? (hipStream_t)stream : own_stream;
+    a.freq = rope ? rope->freq_dev : nullptr;
+    a.factor = rope ? rope->factor : 1.0;
+    a.rotary_dim = rope ? rope->rotary_dim : 0;
+    a.half_layout = rope ? (rope->layout == NVK_ROPE_HALF) : 0;
+    if (ptr_kind == NVK_PTR_DEVICE) {
+        launch_rotary<MX4>(a, rows, st);
+        NVK_HIP_TRY(hipGetLastError());
+        return NVK_OK;
+    }
+
+    if (a.k) {
+        const int rc = check_rows(rows, a.row_seqs, a.positions, a.tables, a.num_seqs, a.max_blocks, bs, a.mx.num_blocks, true, who);
+        if (rc != NVK_OK)
+            return rc;
+    }
+    float       *q_host = a.q_out;
+    const size_t qb = a.q ? (size_t)rows * a.n_heads * hd * sizeof(float) : 0, kb = a.k ? (size_t)rows * kv * hd * sizeof(float) : 0;
+    const size_t rb = (size_t)rows * sizeof(int), tb = a.tables ? (size_t)a.num_seqs * a.max_blocks * sizeof(int) : 0;
+    nvk::Staging s;
+    const int    iq = s.add(a.q, qb), ik = s.add(a.k, kb), iv = s.add(a.v, kb), ip = s.add(a.positions, rb),
+              is = s.add(a.row_seqs, a.row_seqs ? rb : 0), it = s.add(a.tables, tb),
+              iw = s.add(a.q_weight, a.q_weight ? hd * sizeof(float) : 0), ix = s.add(a.k_weight, a.k_weight ? hd * sizeof(float) : 0);
+    NVK_HIP_TRY(s.upload(st));
+    if (a.q)
+        a.q = s.at<float>(iq), a.q_out = s.at<float>(iq); // in place: a row is read whole before it is written
+    if (a.k)
+        a.k = s.at<float>(ik), a.v = s.at<float>(iv);
+    a.positions = s.at<int>(ip);
+    a.row_seqs  = a.row_seqs ? s.at<int>(is) : nullptr;
+    a.tables    = s.at<int>(it);
+    a.q_weight  = a.q_weight ? s.at<float>(iw) : nullptr;
+    a.k_weight  = a.k_weight ? s.at<float>(ix) : nullptr;
+    launch_rotary<MX4>(a, rows, st);
+    NVK_HIP_TRY(hipGetLastError());
+    // (rows of padding come back as they went)
+    if (q_host && a.q)
+        NVK_HIP_TRY(hipMemcpyAsync(q_host, a.q_out, qb, hipMemcpyDeviceToHost, st));
+    NVK_HIP_TRY(hipStreamSynchronize(st));
+    return NVK_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+int nvk_rope_create(int head_dim, int rotary_dim, int layout, double theta, int scaling, double factor, int original_len,
+                    int device, nvk_rope **out_rope)
+{
+    if (!out_rope)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_rope_create: out_rope is null");
+    *out_rope = nullptr;
+    if (head_dim <= 0 || head_dim > nvk::kRotaryMaxHead || head_dim % 2 != 0 || rotary_dim <= 0 || rotary_dim > head_dim
+        || rotary_dim % 2 != 0)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_rope_create: head_dim %d, rotary_dim %d (both even, at most %d)", head_dim,
+                         rotary_dim, nvk::kRotaryMaxHead);
+    if (layout != NVK_ROPE_INTERLEAVED && layout != NVK_ROPE_HALF)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_rope_create: layout %d", layout);
+    if (scaling < NVK_ROPE_SCALE_NONE || scaling > NVK_ROPE_SCALE_YARN)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_rope_create: scaling %d", scaling);
+    if (!(theta > 0.0) || !std::isfinite(theta))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_rope_create: theta %g", theta);
+    if (scaling != NVK_ROPE_SCALE_NONE && (!(factor >= 1.0) || !std::isfinite(factor)))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_rope_create: factor %g (1 or more)", factor);
+    if (scaling == NVK_ROPE_SCALE_NTK && rotary_dim <= 2)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_rope_create: a changed base needs more than one pair (rotary_dim %d)", rotary_dim);
+    if (scaling == NVK_ROPE_SCALE_YARN && original_len <= 0)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_rope_create: original_len %d", original_len);
+    if (device < 0 || device >= nvk::device_count_cached())
+        return nvk::fail(nvk::device_count_cached() ? NVK_ERR_INVALID_ARG : NVK_ERR_NO_DEVICE,
+                         "nvk_rope_create: device %d outside [0,%d)", device, nvk::device_count_cached());
+    nvk_rope *r = nullptr;
+    try {
+        r = new nvk_rope();
+        r->head_dim = head_dim, r->rotary_dim = rotary_dim, r->layout = layout, r->device = device;
+        const double base = scaling == NVK_ROPE_SCALE_NTK
+                                ? theta * std::pow(factor, (double)rotary_dim / (double)(rotary_dim - 2)) : theta;
+        for (int i = 0; i < rotary_dim; i += 2) {
+            double f = std::pow(base, -(double)i / rotary_dim);
+            if (scaling == NVK_ROPE_SCALE_LINEAR)
+                f /= factor;
+            else if (scaling == NVK_ROPE_SCALE_YARN) {
+                // turns a pair makes over the trained context: up to 1 slowed down, from 32 on kept, a ramp between
+                const double turns = original_len * f / (2.0 * M_PI);
+                const double kept  = std::min(1.0, std::max(0.0, (turns - 1.0) / 31.0));
+                f                  = (1.0 - kept) * f / factor + kept * f;
+            }
+            r->freq.push_back(f);
+        }
+        if (scaling == NVK_ROPE_SCALE_YARN)
+            r->factor = 0.1 * std::log(factor) + 1.0;
+    }
+    catch (const std::bad_alloc &) {
+        delete r;
+        return nvk::fail(NVK_ERR_OOM, "nvk_rope_create: host allocation failed");
+    }
+    nvk::DeviceScope scope(device);
+    hipError_t       e = scope.ok ? hipSuccess : hipErrorInvalidDevice;
+    if (e == hipSuccess)
+        e = hipMalloc((void **)&r->freq_dev, r->freq.size() * sizeof(double));
+    if (e == hipSuccess)
+        e = hipMemcpy(r->freq_dev, r->freq.data(), r->freq.size() * sizeof(double), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        const int rc = nvk::fail(e == hipErrorOutOfMemory ? NVK_ERR_OOM : NVK_ERR_HIP, "nvk_rope_create: %s", hipGetErrorString(e));
+        if (r->freq_dev)
+            (void)hipFree(r->freq_dev);
+        delete r;
+        return rc;
+    }
+    *out_rope = r;
+    return NVK_OK;
+}
+
+int nvk_rope_destroy(nvk_rope *rope)
+{
+    if (!rope)
+        return NVK_OK;
+    nvk::DeviceScope scope(rope->device); // (a release path: goes on whatever the switch returned)
+    (void)hipDeviceSynchronize();         // launches on any stream may still read the table
+    (void)hipFree(rope->freq_dev);
+    delete rope;
+    return NVK_OK;
+}
+
+int nvk_rope_frequencies(const nvk_rope *rope, double *freq, int cap, double *factor)
+{
+    if (!rope || cap < 0 || (cap > 0 && !freq))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_rope_frequencies: bad arguments");
+    for (int i = 0; i < std::min(cap, (int)rope->freq.size()); i++)
+        freq[i] = rope->freq[(size_t)i];
+    if (factor)
+        *factor = rope->factor;
+    return (int)rope->freq.size();
+}
+
+int nvk_pool_norm_rope_append(nvk_pool *pool, int layer, const nvk_rope *rope, int rows, int n_heads, const float *q,
+                              float *q_out, const float *k_rows, const float *v_rows, const float *q_weight,
+                              const float *k_weight, float eps, const int *row_seqs, const int *positions,
+                              const int *block_tables, int num_seqs, int max_blocks, int ptr_kind, void *stream)
+{
+    const char *who = "nvk_pool_norm_rope_append";
+    int         g[6];
+    int         rc = pool ? nvk_pool_geometry(pool, g) : nvk::fail(NVK_ERR_INVALID_ARG, "%s: null pool", who);
+    if (rc != NVK_OK)
+        return rc;
+    void *k = nullptr, *v = nullptr, *own = nullptr;
+    if ((rc = nvk_pool_layer_ptrs(pool, layer, &k, &v)) != NVK_OK || (rc = nvk_pool_stream(pool, &own)) != NVK_OK)
+        return rc;
+    RotaryArgs a{};
+    a.q = q, a.q_out = q_out, a.k = k_rows, a.v = v_rows, a.q_weight = q_weight, a.k_weight = k_weight, a.eps = eps;
+    a.row_seqs = row_seqs, a.positions = positions, a.tables = block_tables, a.num_seqs = num_seqs, a.max_blocks = max_blocks;
+    a.n_heads = n_heads, a.k_slab = (float *)k, a.v_slab = (float *)v;
+    a.mx.num_blocks = g[1], a.mx.block_size = g[2], a.mx.n_kv_heads = g[3], a.mx.head_dim = g[4];
+    return norm_rope_append<false>(a, g[5], (hipStream_t)own, rope, rows, ptr_kind, stream, who);
+}
+
+int nvk_mx4_pool_norm_rope_append(nvk_mx4_pool *pool, int layer, const nvk_rope *rope, int rows, int n_heads, const float *q,
+                                  float *q_out, const float *k_rows, const float *v_rows, const float *q_weight,
+                                  const float *k_weight, float eps, const int *row_seqs, const int *positions,
+                                  const int *block_tables, int num_seqs, int max_blocks, int ptr_kind, void *stream)
+{
+    const char *who = "nvk_mx4_pool_norm_rope_append";
+    if (!pool)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: null pool", who);
+    if (layer < 0 || layer >= pool->n_layers)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: layer %d outside [0,%d)", who, layer, pool->n_layers);
+    RotaryArgs a{};
+    a.q = q, a.q_out = q_out, a.k = k_rows, a.v = v_rows, a.q_weight = q_weight, a.k_weight = k_weight, a.eps = eps;
+    a.row_seqs = row_seqs, a.positions = positions, a.tables = block_tables, a.num_seqs = num_seqs, a.max_blocks = max_blocks;
+    a.n_heads = n_heads, a.mx = pool->layer(layer);
+    return norm_rope_append<true>(a, pool->device, pool->stream, rope, rows, ptr_kind, stream, who);
+}
+
+int nvk_mx4_pool_read_rows(nvk_mx4_pool *pool, int layer, int rows, const int *row_seqs, const int *positions,
+                           const int *block_tables, int num_seqs, int max_blocks, float *k_out, float *v_out, int ptr_kind,
+                           void *stream)
+{
+    const char *who = "nvk_mx4_pool_read_rows";
+    if (!pool)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: null pool", who);
+    if (layer < 0 || layer >= pool->n_layers)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: layer %d outside [0,%d)", who, layer, pool->n_layers);
+    if (ptr_kind != NVK_PTR_HOST && ptr_kind != NVK_PTR_DEVICE)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: ptr_kind %d", who, ptr_kind);
+    if (rows < 0 || num_seqs < 0 || max_blocks <= 0 || (long long)max_blocks * pool->block_size > 0x7fffffffLL
+        || (rows > 0 && (!positions || !block_tables || !k_out || !v_out)))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: bad arguments", who);
+    if (rows == 0)
+        return NVK_OK;
+    NVK_SCOPE(pool->device);
+    hipStream_t st = (ptr_kind == NVK_PTR_DEVICE && stream) ? (hipStream_t)stream : pool->stream;
+    const dim3  grid((unsigned)rows), block(256);
+    if (ptr_kind == NVK_PTR_DEVICE) {
+        hipLaunchKernelGGL(nvk::nvk_mx4_read_rows_kernel, grid, block, 0, st, pool->layer(layer), row_seqs, positions,
+                           block_tables, num_seqs, max_blocks, k_out, v_out);
+        NVK_HIP_TRY(hipGetLastError());
+        return NVK_OK;
+    }
+    const int rc = check_rows(rows, row_seqs, positions, block_tables, num_seqs, max_blocks, pool->block_size, pool->num_blocks,
+                              false, who);
+    if (rc != NVK_OK)
+        return rc;
+    const size_t kb = (size_t)rows * pool->n_kv_heads * pool->head_dim * sizeof(float), rb = (size_t)rows * sizeof(int);
+    nvk::Staging s;
+    const int    ik = s.add(k_out, kb), iv = s.add(v_out, kb), ip = s.add(positions, rb), is = s.add(row_seqs, row_seqs ? rb : 0),
+              it = s.add(block_tables, (size_t)num_seqs * max_blocks * sizeof(int));
+    NVK_HIP_TRY(s.upload(st));
+    hipLaunchKernelGGL(nvk::nvk_mx4_read_rows_kernel, grid, block, 0, st, pool->layer(layer),
+                       row_seqs ? s.at<int>(is) : (const int *)nullptr, s.at<int>(ip), s.at<int>(it), num_seqs, max_blocks,
+                       s.at<float>(ik), s.at<float>(iv));
+    NVK_HIP_TRY(hipGetLastError());
+    NVK_HIP_TRY(hipMemcpyAsync(k_out, s.at<float>(ik), kb, hipMemcpyDeviceToHost, st));
+    NVK_HIP_TRY(hipMemcpyAsync(v_out, s.at<float>(iv), kb, hipMemcpyDeviceToHost, st));
+    NVK_HIP_TRY(hipStreamSynchronize(st));
+    return NVK_OK;
+}
+
+} // extern "C"

@@ -1,0 +1,832 @@
+// nvk_sparse.hip -- decode attention over the cache blocks that a cheap score selects (nvk_block_index_*, nvk_sparse_decode*).
+//
+// The index keeps, for every block, kv-head and channel, the least and the largest key element: lo and hi.  For a query
+// head q, q . k <= sum_c max(q_c, 0) hi_c + min(q_c, 0) lo_c for every key k of the block; the largest of these bounds over the
+// group's query heads is the block's score for that kv-head.  A decode call reads the first blocks, the last blocks and the
+// best-scored others, and attends to their tokens alone (Attention::paged_attention, include/core/attention.hpp:82-159, over
+// a subset): with block_size 16 it moves 1/16 of the keys for the scores and top / blocks of keys and values.
+//
+// Four kernels: nvk_index_update_kernel behind an append, and for a decode call score, select and attend (and the join of
+// chunks).  gfx950 only; no CPU path.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "nvk_hip_util.h"
+
+struct nvk_block_index
+{
+    nvk_pool *pool = nullptr;
+    int       n_layers = 0, num_blocks = 0, block_size = 0, n_kv_heads = 0, head_dim = 0, device = 0;
+    size_t    layer_floats = 0; // num_blocks * n_kv_heads * 2 * head_dim
+    float    *base = nullptr;   // [layer][block][kv-head][lo | hi][head_dim]
+    float    *ws = nullptr;     // scores | chosen blocks | partial results
+    size_t    ws_floats = 0;
+    long long ws_generation = 0;
+};
+
+namespace nvk {
+
+constexpr int kSparseWaves = 4;
+
+struct SparseArgs
+{
+    const float *k, *v;    // the layer's slabs [block][offset][kv-head][head_dim]
+    float       *bounds;   // the layer's index
+    const float *q;        // [num_seqs, n_heads, head_dim]
+    float       *out;
+    const int   *tables, *ctx_lens, *starts; // starts: index update only
+    int          num_seqs, max_blocks, n_heads, group, n_kv_heads, head_dim, num_blocks, block_size;
+    int          top, first, last;
+    float       *scores; // [num_seqs, n_kv_heads, max_nb]
+    int         *chosen; // [num_seqs, n_kv_heads, top]
+    int          max_nb; // blocks of the longest context
+    int          blocks_per_wave;          // score
+    int          blocks_per_chunk, chunks; // attend
+    int          head_sets;                // attend: workgroups along the group's heads
+    float        scale_log2e;
+    float       *ws_o, *ws_ml;
+};
+
+__device__ __forceinline__ int context_of(const SparseArgs &a, int seq)
+{
+    const int64_t room = (int64_t)min(a.max_nb, a.max_blocks) * a.block_size;
+    return (int)min((int64_t)max(a.ctx_lens[seq], 0), room);
+}
+
+// ---- the index: lo and hi of each block that the tokens [starts[s], ctx_lens[s]) lie in, from all its tokens ------------
+// One workgroup per block; a thread takes four channels of the row (all kv-heads).  Bound by the keys it reads.
+__global__ void __launch_bounds__(256) nvk_index_update_kernel(const SparseArgs a, int slots)
+{
+    const int seq = (int)(blockIdx.x / (unsigned)slots), slot = (int)(blockIdx.x % (unsigned)slots);
+    const int bs = a.block_size;
+    const int end = (int)min((int64_t)a.ctx_lens[seq], (int64_t)a.max_blocks * bs), begin = max(a.starts[seq], 0);
+    const int b = begin / bs + slot;
+    if (end <= begin || (int64_t)b * bs >= end)
+        return;
+    const int pb = a.tables[(int64_t)seq * a.max_blocks + b];
+    if (pb < 0 || pb >= a.num_blocks)
+        return;
+    const int    held = min(bs, end - b * bs), row = a.n_kv_heads * a.head_dim;
+    const float *k = a.k + (int64_t)pb * bs * row;
+    float       *to = a.bounds + (int64_t)pb * 2 * row;
+    // a NaN stays: x < lo is false for it, and lo < x once lo is one
+    auto take = [](float &lo, float &hi, float x) {
+        lo = (x < lo || x != x) ? x : lo;
+        hi = (x > hi || x != x) ? x : hi;
+    };
+    for (int c = threadIdx.x * 4; c < row; c += 1024) {
+        float4 lo = make_float4(INFINITY, INFINITY, INFINITY, INFINITY), hi = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll 8
+        for (int t = 0; t < held; t++) {
+            const float4 x = *reinterpret_cast<const float4 *>(k + (int64_t)t * row + c);
+            take(lo.x, hi.x, x.x), take(lo.y, hi.y, x.y), take(lo.z, hi.z, x.z), take(lo.w, hi.w, x.w);
+        }
+        const int head = c / a.head_dim, at = c % a.head_dim;
+        *reinterpret_cast<float4 *>(to + (int64_t)head * 2 * a.head_dim + at)              = lo;
+        *reinterpret_cast<float4 *>(to + (int64_t)head * 2 * a.head_dim + a.head_dim + at) = hi;
+    }
+}
+
+// ---- scores ---------------------------------------------------------------------------------------------------------
+// With w = [min(q, 0) | max(q, 0)] a bound is the dot product of w with a block's [lo | hi], 2 head_dim contiguous floats.  It is
+// summed in 64 bits (every product of two fp32 numbers is exact there) and rounded once: which of two close blocks is
+// read does not hang on the order of a sum.  Sixteen lanes share a block, four blocks a wave; w stays in registers for HG
+// query heads at a time.  NV = float4s of [lo | hi] per lane.
+template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) nvk_block_score_kernel(const SparseArgs a, int slots)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, sub = lane >> 4;
+    unsigned  id = blockIdx.x;
+    const int kvh = (int)(id % (unsigned)a.n_kv_heads);
+    id /= (unsigned)a.n_kv_heads;
+    const int slot = (int)(id % (unsigned)slots), seq = (int)(id / (unsigned)slots);
+    const int ctx = context_of(a, seq), nb = (ctx + a.block_size - 1) / a.block_size;
+    const int begin = (slot * kSparseWaves + wave) * a.blocks_per_wave, end = min(begin + a.blocks_per_wave, nb);
+    if (nb <= a.top || begin >= end) // everything is read: no scores needed
+        return;
+    const int  hd = a.head_dim;
+    float     *score = a.scores + ((int64_t)seq * a.n_kv_heads + kvh) * a.max_nb;
+    const int *table = a.tables + (int64_t)seq * a.max_blocks;
+    for (int h0 = 0; h0 < a.group; h0 += HG) {
+        double w[HG][NV][4];
+#pragma unroll
+        for (int h = 0; h < HG; h++)
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int c = (l16 + 16 * j) * 4; // place in [lo | hi]
+                float4    x = make_float4(0.f, 0.f, 0.f, 0.f);
+                // (a set that ends beyond the group repeats its last head: the maximum is the same)
+                if (c < 2 * hd)
+                    x = *reinterpret_cast<const float4 *>(
+                        a.q + ((int64_t)seq * a.n_heads + kvh * a.group + min(h0 + h, a.group - 1)) * hd + (c < hd ? c : c - hd));
+                const bool low = c < hd;
+                w[h][j][0] = low ? fminf(x.x, 0.f) : fmaxf(x.x, 0.f), w[h][j][1] = low ? fminf(x.y, 0.f) : fmaxf(x.y, 0.f);
+                w[h][j][2] = low ? fminf(x.z, 0.f) : fmaxf(x.z, 0.f), w[h][j][3] = low ? fminf(x.w, 0.f) : fmaxf(x.w, 0.f);
+            }
+        for (int b0 = begin; b0 < end; b0 += 4) {
+            const int    b = min(b0 + sub, end - 1);
+            const int    pb = min(max(table[b], 0), a.num_blocks - 1);
+            const float *src = a.bounds + ((int64_t)pb * a.n_kv_heads + kvh) * 2 * hd;
+            double       s[HG];
+#pragma unroll
+            for (int h = 0; h < HG; h++)
+                s[h] = 0.0;
+            float4 x[NV];
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int c = (l16 + 16 * j) * 4;
+                x[j] = c < 2 * hd ? *reinterpret_cast<const float4 *>(src + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < NV; j++)
+#pragma unroll
+                for (int h = 0; h < HG; h++) {
+                    s[h] = fma(w[h][j][0], (double)x[j].x, s[h]), s[h] = fma(w[h][j][1], (double)x[j].y, s[h]);
+                    s[h] = fma(w[h][j][2], (double)x[j].z, s[h]), s[h] = fma(w[h][j][3], (double)x[j].w, s[h]);
+                }
+            // sums over the block's sixteen lanes; with several heads, each exchange halves the heads a lane carries
+            double mine;
+            if constexpr (HG == 4) {
+                const bool o1 = lane & 1, o2 = lane & 2;
+                double     t0 = o1 ? s[2] : s[0], t1 = o1 ? s[3] : s[1];
+                t0 += __shfl_xor(o1 ? s[0] : s[2], 1), t1 += __shfl_xor(o1 ? s[1] : s[3], 1);
+                mine = (o2 ? t1 : t0) + __shfl_xor(o2 ? t0 : t1, 2);
+            }
+            else if constexpr (HG == 2) {
+                const bool o1 = lane & 1;
+                mine = (o1 ? s[1] : s[0]) + __shfl_xor(o1 ? s[0] : s[1], 1);
+                mine += __shfl_xor(mine, 2);
+            }
+            else {
+                mine = s[0] + __shfl_xor(s[0], 1);
+                mine += __shfl_xor(mine, 2);
+            }
+            mine += __shfl_xor(mine, 4);
+            mine += __shfl_xor(mine, 8);
+            float best = (float)mine;
+            best       = best != best ? INFINITY : best; // no number: as high as can be
+            best       = fmaxf(best, __shfl_xor(best, 1));
+            best       = fmaxf(best, __shfl_xor(best, 2));
+            if (l16 == 0 && b0 + sub < end)
+                score[b] = h0 > 0 ? fmaxf(score[b], best) : best;
+        }
+    }
+}
+
+// ---- selection --------------------------------------------------------------------------------------------------------
+// One workgroup per (sequence, kv-head): the key of the last block that is read by four counting passes over the bytes of the
+// keys, then the blocks above it, and as many of those level with it as are left, lowest first, in ascending order.
+constexpr int kSelectThreads = 1024;
+
+__device__ __forceinline__ unsigned block_key(const SparseArgs &a, const float *score, int b, int nb)
+{
+    if (b < a.first || b >= nb - a.last)
+        return 0xffffffffu; // read always (no score maps there)
+    const unsigned u = __float_as_uint(score[b] + 0.f); // (-0 is 0)
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const SparseArgs a)
+{
+    __shared__ int      s_count[256];
+    __shared__ unsigned s_prefix;
+    __shared__ int      s_left;
+    __shared__ int      s_wave[2][kSelectThreads / 64];
+    const int    line = blockIdx.x, seq = line / a.n_kv_heads;
+    const int    tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int    ctx = context_of(a, seq), nb = (ctx + a.block_size - 1) / a.block_size;
+    int         *chosen = a.chosen + (int64_t)line * a.top;
+    const float *score = a.scores + (int64_t)line * a.max_nb;
+    if (nb <= a.top) {
+        for (int i = tid; i < a.top; i += kSelectThreads)
+            chosen[i] = i < nb ? i : -1;
+        return;
+    }
+    if (tid == 0)
+        s_prefix = 0, s_left = a.top;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256)
+            s_count[tid] = 0;
+        __syncthreads();
+        const unsigned prefix = s_prefix;
+        for (int b = tid; b < nb; b += kSelectThreads) {
+            const unsigned key = block_key(a, score, b, nb);
+            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
+                atomicAdd(&s_count[(key >> shift) & 255u], 1);
+        }
+        __syncthreads();
+        if (wave == 0) { // bins from the top: four to a lane
+            int c[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                c[i] = s_count[255 - (4 * lane + i)], sum += c[i];
+            int before = sum; // of the lanes before this one
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(before, o);
+                before += lane >= o ? x : 0;
+            }
+            before -= sum;
+            const int left = s_left;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (before < left && before + c[i] >= left) { // exactly one bin of one lane
+                    s_prefix = prefix | ((unsigned)(255 - (4 * lane + i)) << shift);
+                    s_left   = left - before;
+                }
+                before += c[i];
+            }
+        }
+        __syncthreads();
+    }
+    const unsigned edge = s_prefix;
+    const int      ties = s_left; // of the blocks with the edge's key, so many are read
+    int            placed = 0, level = 0;
+    for (int b0 = 0; b0 < nb; b0 += kSelectThreads) {
+        const int      b = b0 + tid;
+        const unsigned key = b < nb ? block_key(a, score, b, nb) : 0u;
+        const bool     above = b < nb && key > edge, even = b < nb && key == edge;
+        const unsigned long long below = ((unsigned long long)1 << lane) - 1;
+        const unsigned long long ma = __ballot(above), me = __ballot(even);
+        if (lane == 0)
+            s_wave[0][wave] = __popcll(ma), s_wave[1][wave] = __popcll(me);
+        __syncthreads();
+        int pa = 0, pe = 0, ta = 0, te = 0;
+        for (int w = 0; w < kSelectThreads / 64; w++) {
+            pa += w < wave ? s_wave[0][w] : 0, pe += w < wave ? s_wave[1][w] : 0;
+            ta += s_wave[0][w], te += s_wave[1][w];
+        }
+        pa += __popcll(ma & below), pe += __popcll(me & below);
+        // before this block: pa above it, and of the pe level ones those that are among the first `ties`
+        const int taken = min(max(ties - level, 0), pe);
+        if (above || (even && level + pe < ties))
+            chosen[placed + pa + taken] = b;
+        placed += ta + min(max(ties - level, 0), te);
+        level += te;
+        __syncthreads();
+    }
+}
+
+// ---- attention over the chosen blocks -----------------------------------------------------------------------------------
+// A wave takes eight tokens a step, eight lanes each: a lane holds NV float4s of the row (lane 8 apart: whole lines per
+// token), dots them with HG query heads, and keeps maximum, sum and output of its own eight-lane group -- nothing
+// crosses the groups before the end.  Bound by the keys and values it reads.
+template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) nvk_sparse_attn_kernel(const SparseArgs a)
+{
+    constexpr int kMostBlocks = 64; // of a chunk
+    __shared__ int   s_phys[kMostBlocks], s_first[kMostBlocks];
+    __shared__ float s_m[kSparseWaves][HG], s_l[kSparseWaves][HG];
+    __shared__ __attribute__((aligned(16))) float s_o[kSparseWaves][HG][32 * NV];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l8 = lane & 7, tg = lane >> 3;
+    unsigned  id = blockIdx.x;
+    const int kvh = (int)(id % (unsigned)a.n_kv_heads);
+    id /= (unsigned)a.n_kv_heads;
+    const int set = (int)(id % (unsigned)a.head_sets);
+    id /= (unsigned)a.head_sets;
+    const int chunk = (int)(id % (unsigned)a.chunks), seq = (int)(id / (unsigned)a.chunks);
+    const int hd = a.head_dim, bs = a.block_size;
+    const int ctx = context_of(a, seq), nb = (ctx + bs - 1) / bs, n = min(nb, a.top);
+    const int begin = chunk * a.blocks_per_chunk, count = min(a.blocks_per_chunk, n - begin);
+    if (chunk > 0 && count <= 0)
+        return;
+    const int *chosen = a.chosen + ((int64_t)seq * a.n_kv_heads + kvh) * a.top + begin;
+    if ((int)threadIdx.x < count) {
+        const int b = min(max(chosen[threadIdx.x], 0), max(nb - 1, 0));
+        s_first[threadIdx.x] = b * bs;
+        s_phys[threadIdx.x]  = min(max(a.tables[(int64_t)seq * a.max_blocks + b], 0), a.num_blocks - 1);
+    }
+    __syncthreads();
+
+    const int head0 = kvh * a.group + set * HG, heads = min(HG, a.group - set * HG);
+    float4    q[HG][NV], o[HG][NV];
+#pragma unroll
+    for (int h = 0; h < HG; h++)
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int c = (l8 + 8 * j) * 4;
+            q[h][j] = make_float4(0.f, 0.f, 0.f, 0.f), o[h][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (h < heads && c < hd)
+                q[h][j] = *reinterpret_cast<const float4 *>(a.q + ((int64_t)seq * a.n_heads + head0 + h) * hd + c);
+        }
+    // each lane carries the statistics of head lane % HG of its eight-lane group
+    float m = -INFINITY, l = 0.f;
+
+    const int tokens = max(count, 0) * bs, steps = (tokens + 7) / 8;
+    auto fetch = [&](int step, float4 (&k)[NV], float4 (&v)[NV]) -> bool {
+        const int  t = step * 8 + tg;
+        const int  e = min(t / bs, max(count - 1, 0)), off = t - t / bs * bs;
+        const bool there = t < tokens && s_first[e] + off < ctx;
+        const int64_t at = (((int64_t)s_phys[e] * bs + off) * a.n_kv_heads + kvh) * hd;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int c = (l8 + 8 * j) * 4;
+            k[j] = make_float4(0.f, 0.f, 0.f, 0.f), v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (there && c < hd) {
+                k[j] = *reinterpret_cast<const float4 *>(a.k + at + c);
+                v[j] = *reinterpret_cast<const float4 *>(a.v + at + c);
+            }
+        }
+        return there;
+    };
+    float4 kn[NV], vn[NV];
+    bool   next_there = false;
+    if (wave < steps)
+        next_there = fetch(wave, kn, vn);
+    for (int step = wave; step < steps; step += kSparseWaves) {
+        float4 k[NV], v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            k[j] = kn[j], v[j] = vn[j];
+        const bool there = next_there;
+        if (step + kSparseWaves < steps)
+            next_there = fetch(step + kSparseWaves, kn, vn);
+        float s[HG];
+#pragma unroll
+        for (int h = 0; h < HG; h++) {
+            s[h] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                s[h] = fmaf(q[h][j].x, k[j].x, s[h]), s[h] = fmaf(q[h][j].y, k[j].y, s[h]);
+                s[h] = fmaf(q[h][j].z, k[j].z, s[h]), s[h] = fmaf(q[h][j].w, k[j].w, s[h]);
+            }
+        }
+        float mine;
+        if constexpr (HG == 4) {
+            const bool o1 = lane & 1, o2 = lane & 2;
+            // after the first exchange odd lanes carry heads 1 and 3, so that a lane ends with head lane % 4
+            float t0 = o1 ? s[1] : s[0], t1 = o1 ? s[3] : s[2];
+            t0 += __shfl_xor(o1 ? s[0] : s[1], 1), t1 += __shfl_xor(o1 ? s[2] : s[3], 1);
+            mine = (o2 ? t1 : t0) + __shfl_xor(o2 ? t0 : t1, 2);
+        }
+        else if constexpr (HG == 2) {
+            const bool o1 = lane & 1;
+            mine = (o1 ? s[1] : s[0]) + __shfl_xor(o1 ? s[0] : s[1], 1);
+            mine += __shfl_xor(mine, 2);
+        }
+        else {
+            mine = s[0] + __shfl_xor(s[0], 1);
+            mine += __shfl_xor(mine, 2);
+        }
+        mine += __shfl_xor(mine, 4);
+        const float t = there ? mine * a.scale_log2e : -INFINITY;
+        if (__any(t > m)) {
+            const float m_new = fmaxf(m, t);
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int h = 0; h < HG; h++) {
+                const float x = __shfl(alpha, (lane & 56) | h);
+#pragma unroll
+                for (int j = 0; j < NV; j++)
+                    o[h][j].x *= x, o[h][j].y *= x, o[h][j].z *= x, o[h][j].w *= x;
+            }
+        }
+        const float p = there ? __builtin_amdgcn_exp2f(t - (m == -INFINITY ? 0.f : m)) : 0.f;
+        l += p;
+#pragma unroll
+        for (int h = 0; h < HG; h++) {
+            const float x = __shfl(p, (lane & 56) | h);
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                o[h][j].x = fmaf(x, v[j].x, o[h][j].x), o[h][j].y = fmaf(x, v[j].y, o[h][j].y);
+                o[h][j].z = fmaf(x, v[j].z, o[h][j].z), o[h][j].w = fmaf(x, v[j].w, o[h][j].w);
+            }
+        }
+    }
+
+    // the eight groups of the wave, then the waves
+    float M = m;
+    M       = fmaxf(M, __shfl_xor(M, 8));
+    M       = fmaxf(M, __shfl_xor(M, 16));
+    M       = fmaxf(M, __shfl_xor(M, 32));
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    l *= alpha;
+    l += __shfl_xor(l, 8);
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (lane < HG)
+        s_m[wave][lane] = M, s_l[wave][lane] = l;
+#pragma unroll
+    for (int h = 0; h < HG; h++) {
+        const float x = __shfl(alpha, (lane & 56) | h);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            float4 y = make_float4(o[h][j].x * x, o[h][j].y * x, o[h][j].z * x, o[h][j].w * x);
+#pragma unroll
+            for (int e = 8; e <= 32; e <<= 1)
+                y.x += __shfl_xor(y.x, e), y.y += __shfl_xor(y.y, e), y.z += __shfl_xor(y.z, e), y.w += __shfl_xor(y.w, e);
+            if (tg == 0)
+                *reinterpret_cast<float4 *>(&s_o[wave][h][(l8 + 8 * j) * 4]) = y;
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < heads * hd; e += 64 * kSparseWaves) {
+        const int h = e / hd, c = e % hd;
+        float     Mh = -INFINITY, L = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < kSparseWaves; w++)
+            Mh = fmaxf(Mh, s_m[w][h]);
+#pragma unroll
+        for (int w = 0; w < kSparseWaves; w++) {
+            const float f = s_m[w][h] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][h] - Mh);
+            L += s_l[w][h] * f;
+            x += s_o[w][h][c] * f;
+        }
+        const int64_t line = (int64_t)seq * a.n_heads + head0 + h;
+        if (a.chunks > 1) {
+            a.ws_o[(line * a.chunks + chunk) * hd + c] = x;
+            if (c == 0)
+                a.ws_ml[(line * a.chunks + chunk) * 2] = Mh, a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = L;
+        }
+        else
+            a.out[line * hd + c] = L == 0.f ? x : x / L; // (x is 0 then, or no number)
+    }
+}
+
+// joins the chunks of a (sequence, head): one wave each
+__global__ void __launch_bounds__(256) nvk_sparse_merge_kernel(const SparseArgs a)
+{
+    const int64_t line = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int     lane = threadIdx.x & 63;
+    if (line >= (int64_t)a.num_seqs * a.n_heads)
+        return;
+    const int    ctx = context_of(a, (int)(line / a.n_heads)), nb = (ctx + a.block_size - 1) / a.block_size;
+    const int    n = max((min(nb, a.top) + a.blocks_per_chunk - 1) / a.blocks_per_chunk, 1);
+    const float *ml = a.ws_ml + line * a.chunks * 2, *o = a.ws_o + line * a.chunks * a.head_dim;
+    float        M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < n; c++)
+        M = fmaxf(M, ml[2 * c]);
+    for (int c = 0; c < n; c++) {
+        const float w = ml[2 * c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * c] - M);
+        L += ml[2 * c + 1] * w;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (lane + 64 * i < a.head_dim)
+                x[i] += o[(int64_t)c * a.head_dim + lane + 64 * i] * w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (lane + 64 * i < a.head_dim)
+            a.out[line * a.head_dim + lane + 64 * i] = L == 0.f ? x[i] : x[i] / L;
+}
+
+} // namespace nvk
+
+namespace {
+
+using nvk::SparseArgs;
+
+constexpr int kCus = 256; // MI355X
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+struct SparseShape
+{
+    int    max_nb = 0, blocks_per_wave = 4, score_slots = 1, blocks_per_chunk = 1, chunks = 1, head_sets = 1, hg = 1;
+    size_t score_floats = 0, chosen_ints = 0, part_floats = 0;
+    size_t floats() const { return score_floats + chosen_ints + part_floats; }
+};
+
+size_t to_line(size_t floats) { return (floats + 31) / 32 * 32; }
+
+SparseShape sparse_shape(const nvk_block_index *x, int num_seqs, int n_heads, int max_ctx, int top)
+{
+    SparseShape s;
+    const int   group = n_heads / x->n_kv_heads;
+    s.max_nb = (int)ceil_div(max_ctx, x->block_size);
+    s.hg     = group == 1 ? 1 : group == 2 ? 2 : 4;
+    if (x->head_dim > 128) // registers
+        s.hg = std::min(s.hg, 2);
+    s.head_sets = (int)ceil_div(group, s.hg);
+    // scores: four blocks a wave at least, 64 at most, in between two workgroups for every CU
+    const long long lines = (long long)num_seqs * x->n_kv_heads;
+    const long long per = lines * s.max_nb / (2LL * kCus * nvk::kSparseWaves);
+    s.blocks_per_wave = (int)std::min(64LL, std::max(4LL, per / 4 * 4));
+    s.score_slots     = (int)std::max(1LL, ceil_div(s.max_nb, (long long)s.blocks_per_wave * nvk::kSparseWaves));
+    // attention: chunks of the chosen blocks until there are four workgroups for every CU, at least 32 tokens to a wave
+    const int       n = std::max(1, std::min(s.max_nb, top));
+    const long long tasks = lines * s.head_sets;
+    const long long wanted = ceil_div(4LL * kCus, std::max(tasks, 1LL));
+    const long long least = ceil_div(32LL * nvk::kSparseWaves, x->block_size);
+    s.blocks_per_chunk = (int)std::min(64LL, std::max(least, ceil_div(n, wanted)));
+    s.blocks_per_chunk = std::max(1, s.blocks_per_chunk);
+    s.chunks           = (int)ceil_div(n, s.blocks_per_chunk);
+    s.score_floats     = s.max_nb > top ? to_line((size_t)lines * s.max_nb) : 0;
+    s.chosen_ints      = to_line((size_t)lines * top);
+    s.part_floats      = s.chunks > 1 ? (size_t)num_seqs * n_heads * s.chunks * (x->head_dim + 2) : 0;
+    return s;
+}
+
+template <int NV, int HG> void launch_sparse(const SparseArgs &a, const SparseShape &s, bool score, hipStream_t st)
+{
+    const unsigned lines = (unsigned)a.num_seqs * (unsigned)a.n_kv_heads;
+    if (score)
+        hipLaunchKernelGGL((nvk::nvk_block_score_kernel<NV, HG>), dim3(lines * (unsigned)s.score_slots), dim3(64 * nvk::kSparseWaves), 0,
+                           st, a, s.score_slots);
+    hipLaunchKernelGGL(nvk::nvk_block_select_kernel, dim3(lines), dim3(nvk::kSelectThreads), 0, st, a);
+    hipLaunchKernelGGL((nvk::nvk_sparse_attn_kernel<NV, HG>), dim3(lines * (unsigned)s.head_sets * (unsigned)s.chunks),
+                       dim3(64 * nvk::kSparseWaves), 0, st, a);
+}
+
+template <int NV> void launch_heads(const SparseArgs &a, const SparseShape &s, bool score, hipStream_t st)
+{
+    if constexpr (NV < 8)
+        if (s.hg == 4) {
+            launch_sparse<NV, 4>(a, s, score, st);
+            return;
+        }
+    if (s.hg == 2)
+        launch_sparse<NV, 2>(a, s, score, st);
+    else
+        launch_sparse<NV, 1>(a, s, score, st);
+}
+
+int check_index(const nvk_block_index *x, int layer, const char *who)
+{
+    if (!x)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: null index", who);
+    if (layer < 0 || layer >= x->n_layers)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: layer %d outside [0,%d)", who, layer, x->n_layers);
+    return NVK_OK;
+}
+
+int fill_args(const nvk_block_index *x, int layer, SparseArgs *a)
+{
+    void     *k = nullptr, *v = nullptr;
+    const int rc = nvk_pool_layer_ptrs(x->pool, layer, &k, &v);
+    if (rc != NVK_OK)
+        return rc;
+    a->k = (const float *)k, a->v = (const float *)v, a->bounds = x->base + (size_t)layer * x->layer_floats;
+    a->n_kv_heads = x->n_kv_heads, a->head_dim = x->head_dim, a->num_blocks = x->num_blocks, a->block_size = x->block_size;
+    return NVK_OK;
+}
+
+int pool_stream(const nvk_block_index *x, void *stream, hipStream_t *st)
+{
+    if (stream) {
+        *st = (hipStream_t)stream;
+        return NVK_OK;
+    }
+    void     *own = nullptr;
+    const int rc = nvk_pool_stream(x->pool, &own);
+    *st          = (hipStream_t)own;
+    return rc;
+}
+
+int enqueue_update(nvk_block_index *x, int layer, int num_seqs, const int *tables, int max_blocks, const int *starts,
+                   const int *ctx_lens, int max_new, hipStream_t st, const char *who)
+{
+    SparseArgs a{};
+    const int  rc = fill_args(x, layer, &a);
+    if (rc != NVK_OK)
+        return rc;
+    a.tables = tables, a.max_blocks = max_blocks, a.starts = starts, a.ctx_lens = ctx_lens, a.num_seqs = num_seqs;
+    // max_new tokens lie in at most this many blocks
+    const long long slots = std::min((long long)max_blocks, ceil_div((long long)max_new + x->block_size - 1, x->block_size));
+    if (slots * num_seqs > 0x7fffffffLL)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %lld blocks", who, slots * num_seqs);
+    hipLaunchKernelGGL(nvk::nvk_index_update_kernel, dim3((unsigned)(slots * num_seqs)), dim3(256), 0, st, a, (int)slots);
+    NVK_HIP_TRY(hipGetLastError());
+    return NVK_OK;
+}
+
+int check_sparse(const nvk_block_index *x, int layer, int num_seqs, int n_heads, int max_blocks, int max_ctx, int top, int first,
+                 int last, const char *who)
+{
+    const int rc = check_index(x, layer, who);
+    if (rc != NVK_OK)
+        return rc;
+    if (num_seqs < 0 || max_blocks <= 0 || max_ctx < 0 || (long long)max_blocks * x->block_size > 0x7fffffffLL)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: bad sizes (num_seqs %d, max_blocks %d, max_ctx %d)", who, num_seqs, max_blocks, max_ctx);
+    if (n_heads <= 0 || n_heads % x->n_kv_heads != 0)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: n_heads %d is no multiple of n_kv_heads %d", who, n_heads, x->n_kv_heads);
+    if (first < 0 || last < 1 || top < 1 || (long long)first + last > top)
+        return nvk::fail(NVK_ERR_INVALID_ARG,
+                         "%s: first %d, last %d (at least 1: the newest block is always read) and top %d (at least both)", who,
+                         first, last, top);
+    return NVK_OK;
+}
+
+int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, const float *q, const int *tables, int max_blocks,
+                   const int *ctx_lens, int max_ctx, int top, int first, int last, float *out, int *selected, hipStream_t st,
+                   const char *who)
+{
+    const SparseShape s = sparse_shape(x, num_seqs, n_heads, max_ctx, top);
+    const long long   lines = (long long)num_seqs * x->n_kv_heads;
+    if (lines * s.score_slots > 0x7fffffffLL || lines * s.head_sets * s.chunks > 0x7fffffffLL)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: too many workgroups", who);
+    int rc = nvk::grow_workspace(&x->ws, &x->ws_floats, &x->ws_generation, s.floats(), st, who);
+    if (rc != NVK_OK)
+        return rc;
+    SparseArgs a{};
+    rc = fill_args(x, layer, &a);
+    if (rc != NVK_OK)
+        return rc;
+    a.q = q, a.out = out, a.tables = tables, a.max_blocks = max_blocks, a.ctx_lens = ctx_lens, a.num_seqs = num_seqs;
+    a.n_heads = n_heads, a.group = n_heads / x->n_kv_heads, a.top = top, a.first = first, a.last = last;
+    a.max_nb = s.max_nb, a.blocks_per_wave = s.blocks_per_wave, a.blocks_per_chunk = s.blocks_per_chunk, a.chunks = s.chunks;
+    a.head_sets = s.head_sets, a.scale_log2e = (float)(1.4426950408889634 / std::sqrt((double)x->head_dim));
+    a.scores = x->ws;
+    a.chosen = selected ? selected : (int *)(x->ws + s.score_floats);
+    a.ws_o   = x->ws + s.score_floats + s.chosen_ints;
+    a.ws_ml  = a.ws_o + (size_t)num_seqs * n_heads * s.chunks * x->head_dim;
+    const bool score = s.max_nb > top;
+    const int  nv = x->head_dim <= 32 ? 1 : x->head_dim <= 64 ? 2 : x->head_dim <= 128 ? 4 : 8;
+    switch (nv) {
+    case 1: launch_heads<1>(a, s, score, st); break;
+    case 2: launch_heads<2>(a, s, score, st); break;
+    case 4: launch_heads<4>(a, s, score, st); break;
+    default: launch_heads<8>(a, s, score, st); break;
+    }
+    NVK_HIP_TRY(hipGetLastError());
+    if (s.chunks > 1) {
+        hipLaunchKernelGGL(nvk::nvk_sparse_merge_kernel, dim3((unsigned)ceil_div((long long)num_seqs * n_heads, 4)), dim3(256), 0, st, a);
+        NVK_HIP_TRY(hipGetLastError());
+    }
+    return NVK_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+int nvk_block_index_create(nvk_pool *pool, nvk_block_index **out_index)
+{
+    if (!out_index)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_block_index_create: out_index is null");
+    *out_index = nullptr;
+    int g[6];
+    if (!pool || nvk_pool_geometry(pool, g) != NVK_OK)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_block_index_create: null pool");
+    if (g[4] % 4 != 0 || g[4] > 256)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_block_index_create: head_dim %d (a multiple of 4, at most 256)", g[4]);
+    nvk_block_index *x = new (std::nothrow) nvk_block_index();
+    if (!x)
+        return nvk::fail(NVK_ERR_OOM, "nvk_block_index_create: host allocation failed");
+    x->pool = pool, x->n_layers = g[0], x->num_blocks = g[1], x->block_size = g[2], x->n_kv_heads = g[3], x->head_dim = g[4];
+    x->device = g[5], x->layer_floats = (size_t)g[1] * g[3] * 2 * g[4];
+    nvk::DeviceScope scope(x->device);
+    const size_t     bytes = x->layer_floats * (size_t)x->n_layers * sizeof(float);
+    hipError_t       e = scope.ok ? hipMalloc((void **)&x->base, bytes) : hipErrorInvalidDevice;
+    if (e == hipSuccess)
+        e = hipMemset(x->base, 0, bytes); // the bounds of the zeros that a pool starts with
+    if (e == hipSuccess)
+        e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        const int rc = nvk::fail(e == hipErrorOutOfMemory ? NVK_ERR_OOM : NVK_ERR_HIP, "nvk_block_index_create: %s (%zu bytes requested)",
+                                 hipGetErrorString(e), bytes);
+        (void)hipGetLastError();
+        nvk_block_index_destroy(x);
+        return rc;
+    }
+    *out_index = x;
+    return NVK_OK;
+}
+
+int nvk_block_index_destroy(nvk_block_index *index)
+{
+    if (!index)
+        return NVK_OK;
+    nvk::DeviceScope scope(index->device); // (a release path: goes on whatever the switch returned)
+    (void)hipDeviceSynchronize();          // launches on any stream may still use it
+    if (index->base)
+        (void)hipFree(index->base);
+    if (index->ws)
+        (void)hipFree(index->ws);
+    delete index;
+    return NVK_OK;
+}
+
+int nvk_block_index_layer_ptr(const nvk_block_index *index, int layer, void **bounds_dev)
+{
+    const int rc = check_index(index, layer, "nvk_block_index_layer_ptr");
+    if (rc != NVK_OK)
+        return rc;
+    if (!bounds_dev)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_block_index_layer_ptr: null pointer");
+    *bounds_dev = index->base + (size_t)layer * index->layer_floats;
+    return NVK_OK;
+}
+
+long long nvk_block_index_workspace_generation(const nvk_block_index *index) { return index ? index->ws_generation : -1; }
+
+int nvk_block_index_reserve_workspace(nvk_block_index *index, int num_seqs, int n_heads, int max_ctx, int top_blocks)
+{
+    const char *who = "nvk_block_index_reserve_workspace";
+    const int   rc = check_sparse(index, 0, num_seqs, n_heads, 1, max_ctx, top_blocks, 0, 1, who);
+    if (rc != NVK_OK)
+        return rc;
+    NVK_SCOPE(index->device);
+    hipStream_t st = nullptr;
+    const int   rs = pool_stream(index, nullptr, &st);
+    if (rs != NVK_OK)
+        return rs;
+    return nvk::grow_workspace(&index->ws, &index->ws_floats, &index->ws_generation,
+                               sparse_shape(index, num_seqs, n_heads, max_ctx, top_blocks).floats(), st, who);
+}
+
+int nvk_block_index_update(nvk_block_index *index, int layer, int num_seqs, const int *block_tables, int max_blocks,
+                           const int *starts, const int *ctx_lens, int max_new, int ptr_kind, void *stream)
+{
+    const char *who = "nvk_block_index_update";
+    int         rc = check_index(index, layer, who);
+    if (rc != NVK_OK)
+        return rc;
+    if (ptr_kind != NVK_PTR_HOST && ptr_kind != NVK_PTR_DEVICE)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: ptr_kind %d", who, ptr_kind);
+    if (num_seqs < 0 || max_blocks <= 0 || max_new < 0 || (long long)max_blocks * index->block_size > 0x7fffffffLL)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: bad sizes (num_seqs %d, max_blocks %d, max_new %d)", who, num_seqs, max_blocks, max_new);
+    if (num_seqs == 0 || (max_new == 0 && ptr_kind == NVK_PTR_DEVICE))
+        return NVK_OK;
+    if (!block_tables || !starts || !ctx_lens)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: null pointer", who);
+    NVK_SCOPE(index->device);
+    hipStream_t st = nullptr;
+    rc             = pool_stream(index, ptr_kind == NVK_PTR_DEVICE ? stream : nullptr, &st);
+    if (rc != NVK_OK)
+        return rc;
+    if (ptr_kind == NVK_PTR_DEVICE)
+        return enqueue_update(index, layer, num_seqs, block_tables, max_blocks, starts, ctx_lens, max_new, st, who);
+
+    rc = nvk::check_tables(block_tables, num_seqs, max_blocks, ctx_lens, index->block_size, index->num_blocks, who);
+    if (rc != NVK_OK)
+        return rc;
+    int most = 0;
+    for (int s = 0; s < num_seqs; s++) {
+        if (starts[s] < 0 || starts[s] > ctx_lens[s])
+            return nvk::fail(NVK_ERR_INVALID_ARG, "%s: start %d of sequence %d, whose context is %d tokens", who, starts[s], s, ctx_lens[s]);
+        most = std::max(most, ctx_lens[s] - starts[s]);
+    }
+    if (most == 0)
+        return NVK_OK;
+    nvk::Staging g;
+    const int    it = g.add(block_tables, (size_t)num_seqs * max_blocks * sizeof(int)), is = g.add(starts, (size_t)num_seqs * sizeof(int)),
+              ic = g.add(ctx_lens, (size_t)num_seqs * sizeof(int));
+    NVK_HIP_TRY(g.upload(st));
+    rc = enqueue_update(index, layer, num_seqs, g.at<int>(it), max_blocks, g.at<int>(is), g.at<int>(ic), most, st, who);
+    NVK_HIP_TRY(hipStreamSynchronize(st));
+    return rc;
+}
+
+int nvk_sparse_decode_device(nvk_block_index *index, int layer, int num_seqs, int n_heads, const float *q_dev,
+                             const int *block_tables_dev, int max_blocks, const int *ctx_lens_dev, int max_ctx, int top_blocks,
+                             int first_blocks, int last_blocks, float *out_dev, int *selected_dev, void *stream)
+{
+    const char *who = "nvk_sparse_decode_device";
+    int         rc = check_sparse(index, layer, num_seqs, n_heads, max_blocks, max_ctx, top_blocks, first_blocks, last_blocks, who);
+    if (rc != NVK_OK || num_seqs == 0)
+        return rc;
+    if (!q_dev || !block_tables_dev || !ctx_lens_dev || !out_dev)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: null pointer", who);
+    if ((uintptr_t)q_dev % 16 != 0)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: q is not 16-byte aligned", who);
+    NVK_SCOPE(index->device);
+    hipStream_t st = nullptr;
+    rc             = pool_stream(index, stream, &st);
+    if (rc != NVK_OK)
+        return rc;
+    return enqueue_sparse(index, layer, num_seqs, n_heads, q_dev, block_tables_dev, max_blocks, ctx_lens_dev, max_ctx, top_blocks,
+                          first_blocks, last_blocks, out_dev, selected_dev, st, who);
+}
+
+int nvk_sparse_decode(nvk_block_index *index, int layer, int num_seqs, int n_heads, const float *q, const int *block_tables,
+                      int max_blocks, const int *ctx_lens, int top_blocks, int first_blocks, int last_blocks, float *out,
+                      int *selected)
+{
+    const char *who = "nvk_sparse_decode";
+    int         rc = check_sparse(index, layer, num_seqs, n_heads, max_blocks, 0, top_blocks, first_blocks, last_blocks, who);
+    if (rc != NVK_OK || num_seqs == 0)
+        return rc;
+    if (!q || !block_tables || !ctx_lens || !out)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: null pointer", who);
+    rc = nvk::check_tables(block_tables, num_seqs, max_blocks, ctx_lens, index->block_size, index->num_blocks, who);
+    if (rc != NVK_OK)
+        return rc;
+    NVK_SCOPE(index->device);
+    hipStream_t st = nullptr;
+    rc             = pool_stream(index, nullptr, &st);
+    if (rc != NVK_OK)
+        return rc;
+    const int    max_ctx = *std::max_element(ctx_lens, ctx_lens + num_seqs);
+    const size_t qb = (size_t)num_seqs * n_heads * index->head_dim * sizeof(float);
+    const size_t sb = (size_t)num_seqs * index->n_kv_heads * top_blocks * sizeof(int);
+    nvk::Staging g;
+    const int    iq = g.add(q, qb), io = g.add(nullptr, qb), it = g.add(block_tables, (size_t)num_seqs * max_blocks * sizeof(int)),
+              ic = g.add(ctx_lens, (size_t)num_seqs * sizeof(int)), is = g.add(nullptr, selected ? sb : 0);
+    NVK_HIP_TRY(g.upload(st));
+    rc = enqueue_sparse(index, layer, num_seqs, n_heads, g.at<float>(iq), g.at<int>(it), max_blocks, g.at<int>(ic), max_ctx, top_blocks,
+                        first_blocks, last_blocks, g.at<float>(io), selected ? g.at<int>(is) : nullptr, st, who);
+    if (rc == NVK_OK) {
+        NVK_HIP_TRY(hipMemcpyAsync(out, g.at<float>(io), qb, hipMemcpyDeviceToHost, st));
+        if (selected)
+            NVK_HIP_TRY(hipMemcpyAsync(selected, g.at<int>(is), sb, hipMemcpyDeviceToHost, st));
+    }
+    NVK_HIP_TRY(hipStreamSynchronize(st));
+    return rc;
+}
+
+} // extern "C"
