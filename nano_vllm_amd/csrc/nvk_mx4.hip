@@ -18,6 +18,12 @@
 
 namespace nvk {
 
+#ifndef MX4_AHEAD
+#define MX4_AHEAD 1
+#endif
+#ifndef MX4_WGS
+#define MX4_WGS 2LL
+#endif
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float  f32x4 __attribute__((ext_vector_type(4)));
@@ -136,9 +142,10 @@ template <int KK> __device__ __forceinline__ void load_tile(Mx4Raw<KK> &r, const
 // two lane exchanges a step.  WT waves of a workgroup take steps of 32 tokens in turn (few columns: decode) and join through
 // LDS at the end, or WC waves take different columns over the same tokens (prefill).
 template <int KK, int NC, int WT, int WC>
-__global__ void __launch_bounds__(64 * WT * WC) nvk_mx4_attn_kernel(const Mx4AttnArgs a)
+__global__ void __launch_bounds__(64 * WT * WC, KK == 8 ? 1 : 2) nvk_mx4_attn_kernel(const Mx4AttnArgs a)
 {
     constexpr int HDP = 32 * KK;
+    constexpr int AHEAD = MX4_AHEAD;
     static_assert(WT == 1 || (WC == 1 && NC == 1), "waves share either the tokens or the columns");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, l16 = lane & 15;
@@ -246,16 +253,22 @@ __global__ void __launch_bounds__(64 * WT * WC) nvk_mx4_attn_kernel(const Mx4Att
         }
     };
 
-    Mx4Raw<KK> next[2];
-    if (steps > 0)
-        fetch(next, 0);
+    Mx4Raw<KK> ahead[AHEAD][2]; // tiles on their way: steps i, i + 1, ..
+#pragma unroll
+    for (int d = 0; d < AHEAD; d++)
+        if (d < steps)
+            fetch(ahead[d], d);
     for (int i = 0; i < steps; i++) {
         Mx4Raw<KK> raw[2];
 #pragma unroll
-        for (int j = 0; j < 2; j++)
-            raw[j] = next[j];
-        if (i + 1 < steps)
-            fetch(next, i + 1);
+        for (int j = 0; j < 2; j++) {
+            raw[j] = ahead[0][j];
+#pragma unroll
+            for (int d = 0; d + 1 < AHEAD; d++)
+                ahead[d][j] = ahead[d + 1][j];
+        }
+        if (i + AHEAD < steps)
+            fetch(ahead[AHEAD - 1], i + AHEAD);
         const int t0 = begin + 32 * (wt + WT * i);
 
         // A group of K or V that holds no number (scale byte 255) is dealt with before any product: this compiler does not
@@ -518,18 +531,33 @@ __global__ void __launch_bounds__(256) nvk_mx4_merge_kernel(const Mx4AttnArgs a)
     const int limit = max(ctx - rows + (row - row0) + 1, 0);
     const int n = min(max((limit + a.chunk_tokens - 1) / a.chunk_tokens, 1), a.chunks);
     const float *ml = a.ws_ml + line * a.chunks * 2, *o = a.ws_o + line * a.chunks * a.mx.head_dim;
-    float M = -INFINITY;
-    for (int c = 0; c < n; c++)
+    // a lane takes every 64th chunk's maximum, then its weight; the outputs are summed in chunk order
+    float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = lane; c < n; c += 64)
         M = fmaxf(M, ml[2 * c]);
-    float L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < n; c++) {
-        const float w = ml[2 * c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * c] - M);
-        L += ml[2 * c + 1] * w;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < a.mx.head_dim)
-                x[i] += o[(int64_t)c * a.mx.head_dim + lane + 64 * i] * w;
+    for (int o = 32; o > 0; o >>= 1)
+        M = fmaxf(M, __shfl_xor(M, o));
+    for (int c0 = 0; c0 < n; c0 += 64) {
+        float w = 0.f;
+        if (c0 + lane < n) {
+            const float m = ml[2 * (c0 + lane)];
+            w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+            L += ml[2 * (c0 + lane) + 1] * w;
+        }
+        const int some = min(64, n - c0);
+#pragma unroll 4
+        for (int c = 0; c < some; c++) {
+            const float f = __shfl(w, c);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (lane + 64 * i < a.mx.head_dim)
+                    x[i] += o[(int64_t)(c0 + c) * a.mx.head_dim + lane + 64 * i] * f;
+        }
     }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        L += __shfl_xor(L, o);
     const float norm = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -566,7 +594,7 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     s.col_blocks = ceil_div((long long)max_rows * group, cols);
     const long long tasks = (long long)num_seqs * pool->n_kv_heads * s.col_blocks;
     // workgroups wanted: four to a CU; a chunk is worth its start and its join from 256 tokens on
-    const int wanted = ceil_div(4LL * pool->num_cus, std::max(tasks, 1LL));
+    const int wanted = ceil_div(MX4_WGS * pool->num_cus, std::max(tasks, 1LL));
     const int most = std::max(1, max_ctx / 256);
     s.chunks       = std::max(1, std::min(wanted, most));
     s.chunk_tokens = std::max(32, ceil_div(ceil_div(max_ctx, s.chunks), 32) * 32);
