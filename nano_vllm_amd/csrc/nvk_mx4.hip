@@ -18,15 +18,12 @@
 
 namespace nvk {
 
-#ifndef MX4_AHEAD
-#define MX4_AHEAD 1
-#endif
-#ifndef MX4_WGS
-#define MX4_WGS 2LL
-#endif
+constexpr int kDecodeWaves = 4, kPrefillWaves = 4;
+
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float  f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 struct Mx4AttnArgs
 {
@@ -95,7 +92,31 @@ __device__ __forceinline__ unsigned two_values_at(unsigned codes, float scale, i
     default: return two_values<3>(codes, scale);
     }
 }
-__device__ __forceinline__ float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }
+// The conversion looks at the exponent field of its scale alone (any sign and mantissa do), and makes NaN of exponent 255: a
+// scale byte needs a shift and no mask.
+__device__ __forceinline__ float scale_at(unsigned bytes, int b)
+{
+    return __uint_as_float(b < 3 ? bytes << (23 - 8 * b) : bytes >> 1);
+}
+// Non-zero where a byte of x is 255.
+__device__ __forceinline__ unsigned byte_255(unsigned x) { return (0xfefefefeu - x) & x & 0x80808080u; }
+
+// Over the four lanes of a quad.
+__device__ __forceinline__ float sum_of_quad(float x)
+{
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, true)); // lanes 1 0 3 2
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, true)); // lanes 2 3 0 1
+    return x;
+}
+// The largest of x over the four lanes (g, l16), g = 0 .. 3; their sum.
+__device__ __forceinline__ float max_of_g(float x)
+{
+    const unsigned u = __float_as_uint(x);
+    const auto     a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned v = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto     b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 
 // What a lane holds of one tile.
 template <int KK> struct Mx4Raw
@@ -105,215 +126,166 @@ template <int KK> struct Mx4Raw
     unsigned ks[KS];
 };
 
-template <int KK> __device__ __forceinline__ void load_tile(Mx4Raw<KK> &r, const unsigned char *tile, int lane)
+// Byte offsets of a lane's parts inside a tile: K, channels g*8*KK .. of token l16; V, channels l16*2*KK .. of tokens
+// 4g .. 4g+3; the scales of both.
+template <int KK> struct Mx4Places
 {
-    const int g = lane >> 4, l16 = lane & 15;
-    const unsigned *kc = reinterpret_cast<const unsigned *>(tile + l16 * 16 * KK + g * 4 * KK);
-    const unsigned *vc = reinterpret_cast<const unsigned *>(tile + mx4_v_at(KK) + lane * 4 * KK);
+    unsigned k, v, ks[Mx4Raw<KK>::KS], vs;
+    __device__ __forceinline__ explicit Mx4Places(int lane)
+    {
+        const int g = lane >> 4, l16 = lane & 15;
+        k = l16 * 16 * KK + g * 4 * KK;
+        v = mx4_v_at(KK) + lane * 4 * KK;
+#pragma unroll
+        for (int u = 0; u < Mx4Raw<KK>::KS; u++)
+            ks[u] = mx4_ks_at(KK) + (g * KK / 4 + u) * kMx4Tile + l16;
+        vs = mx4_vs_at(KK) + (l16 * KK / 16) * kMx4Tile + 4 * g;
+    }
+};
+
+// All of it.  (Each code is read by one wave of the launch: not worth keeping in the caches.)
+template <int KK> __device__ __forceinline__ void load_tile(Mx4Raw<KK> &r, const unsigned char *tile, const Mx4Places<KK> &at)
+{
+    const unsigned *kc = reinterpret_cast<const unsigned *>(tile + at.k);
+    const unsigned *vc = reinterpret_cast<const unsigned *>(tile + at.v);
     if constexpr (KK >= 4) {
 #pragma unroll
         for (int i = 0; i < KK; i += 4) {
-            const uint4 a = *reinterpret_cast<const uint4 *>(kc + i), b = *reinterpret_cast<const uint4 *>(vc + i);
-            r.k[i] = a.x, r.k[i + 1] = a.y, r.k[i + 2] = a.z, r.k[i + 3] = a.w;
-            r.v[i] = b.x, r.v[i + 1] = b.y, r.v[i + 2] = b.z, r.v[i + 3] = b.w;
+            const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kc + i));
+            const u32x4 y = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vc + i));
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                r.k[i + u] = x[u], r.v[i + u] = y[u];
         }
     }
-    else if constexpr (KK == 2) {
-        const uint2 a = *reinterpret_cast<const uint2 *>(kc), b = *reinterpret_cast<const uint2 *>(vc);
-        r.k[0] = a.x, r.k[1] = a.y, r.v[0] = b.x, r.v[1] = b.y;
-    }
     else
-        r.k[0] = kc[0], r.v[0] = vc[0];
-    // K: channels g*8*KK .. of token l16; V: channels l16*2*KK .. of tokens 4g .. 4g+3
-    if constexpr (KK == 8) {
-        r.ks[0] = tile[mx4_ks_at(KK) + (2 * g) * kMx4Tile + l16];
-        r.ks[1] = tile[mx4_ks_at(KK) + (2 * g + 1) * kMx4Tile + l16];
+#pragma unroll
+        for (int i = 0; i < KK; i++)
+            r.k[i] = kc[i], r.v[i] = vc[i];
+#pragma unroll
+    for (int u = 0; u < Mx4Raw<KK>::KS; u++)
+        r.ks[u] = tile[at.ks[u]];
+    r.vs = *reinterpret_cast<const unsigned *>(tile + at.vs);
+}
+// K where asked for, V where asked for, the V scales always.  (Read by many workgroups.)
+template <int KK>
+__device__ __forceinline__ void load_tile_part(Mx4Raw<KK> &r, const unsigned char *tile, const Mx4Places<KK> &at, bool k, bool v)
+{
+    auto codes = [](unsigned (&to)[KK], const unsigned char *from) {
+        if constexpr (KK >= 4) {
+#pragma unroll
+            for (int i = 0; i < KK; i += 4) {
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(from + 4 * i);
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    to[i + u] = x[u];
+            }
+        }
+        else
+#pragma unroll
+            for (int i = 0; i < KK; i++)
+                to[i] = reinterpret_cast<const unsigned *>(from)[i];
+    };
+    if (k) {
+        codes(r.k, tile + at.k);
+#pragma unroll
+        for (int u = 0; u < Mx4Raw<KK>::KS; u++)
+            r.ks[u] = tile[at.ks[u]];
     }
-    else
-        r.ks[0] = tile[mx4_ks_at(KK) + (g * KK / 4) * kMx4Tile + l16];
-    r.vs = *reinterpret_cast<const unsigned *>(tile + mx4_vs_at(KK) + (l16 * KK / 16) * kMx4Tile + 4 * g);
+    if (v)
+        codes(r.v, tile + at.v);
+    r.vs = *reinterpret_cast<const unsigned *>(tile + at.vs);
 }
 
-// One wave: NC * 16 columns ((row, head of the group) pairs of one kv-head) against the tokens of its part of a chunk.
+// ---- what both kernels are made of ------------------------------------------------------------------------------------
+// A wave holds NC tiles of columns, a column being a (row, head of the group) pair of one kv-head, and takes 32 tokens a step:
 //   S^T = K Q^T     A = K [16 tokens x 32 channels], B = Q^T [32 channels x 16 columns] -> lane (g, col): tokens 4g .. 4g+3
 //   O^T = V^T P^T   A = V^T [16 channels x 32 tokens], B = P^T [32 tokens x 16 columns]
 // The order of channels (in S) and of tokens (in O) along a contraction is free, so it is chosen such that the lane that holds
-// a probability after S is the lane that needs it for O: the softmax touches no LDS, and a column's statistics need
-// two lane exchanges a step.  WT waves of a workgroup take steps of 32 tokens in turn (few columns: decode) and join through
-// LDS at the end, or WC waves take different columns over the same tokens (prefill).
-template <int KK, int NC, int WT, int WC>
-__global__ void __launch_bounds__(64 * WT * WC, KK == 8 ? 1 : 2) nvk_mx4_attn_kernel(const Mx4AttnArgs a)
+// a probability after S is the lane that needs it for O: the softmax touches no LDS, and a column's maximum takes two lane
+// exchanges a step.
+// PACK: up to four columns, each four times in a tile: the first three copies carry one piece of q and of the probabilities
+// each, whose products then take a third of the instructions and registers, and the copies of a column are added (a quad of
+// lanes).
+template <int KK, int NC, bool PACK> struct Mx4Wave
 {
-    constexpr int HDP = 32 * KK;
-    constexpr int AHEAD = MX4_AHEAD;
-    static_assert(WT == 1 || (WC == 1 && NC == 1), "waves share either the tokens or the columns");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, l16 = lane & 15;
-    const int wt = WT > 1 ? wave : 0, wc = WC > 1 ? wave : 0;
+    static constexpr int COLS   = PACK ? 4 : 16; // columns of a tile
+    static constexpr int PIECES = PACK ? 1 : 3;
 
-    // workgroup -> (sequence, column block, chunk, kv-head); kv-heads change fastest: eight kv-heads are eight XCDs, and the
-    // column blocks of one kv-head meet in the L2 of one
-    unsigned  id = blockIdx.x;
-    const int kvh = (int)(id % (unsigned)a.mx.n_kv_heads);
-    id /= (unsigned)a.mx.n_kv_heads;
-    const int chunk = (int)(id % (unsigned)a.chunks);
-    id /= (unsigned)a.chunks;
-    const int cb = (int)(id % (unsigned)a.col_blocks);
-    const int seq = (int)(id / (unsigned)a.col_blocks);
-
-    int row0 = seq, rows = 1;
-    if (a.row_offsets) {
-        row0 = a.row_offsets[seq];
-        rows = min(a.row_offsets[seq + 1], a.total_rows) - row0;
-        if (row0 < 0 || rows <= 0)
-            return;
-    }
-    const int bs = a.mx.block_size;
-    const int ctx = min(max(a.ctx_lens[seq], 0), (int)min((int64_t)a.max_blocks * bs, (int64_t)0x7fffffff));
-    const int columns = rows * a.group;
-    const int col0 = (cb * WC + wc) * 16 * NC;
-    if (cb * WC * 16 * NC >= columns)
-        return;
-
-    // a column's row sees the tokens below `limit`: all up to its own, its place being at the end of the context
-    int limit[NC], out_row[NC], out_head[NC];
-    int most = 0; // the largest limit of the wave's columns, and of the workgroup's
-    const int last_row = min((cb + 1) * WC * 16 * NC - 1, columns - 1) / a.group;
-    const int block_most = max(ctx - rows + last_row + 1, 0);
-#pragma unroll
-    for (int n = 0; n < NC; n++) {
-        const int col = col0 + 16 * n + l16, r = col / a.group;
-        out_row[n] = col < columns ? row0 + r : -1;
-        out_head[n] = kvh * a.group + col % a.group;
-        limit[n] = col < columns ? max(ctx - rows + r + 1, 0) : 0;
-    }
-    {
-        const int r = min(col0 + 16 * NC - 1, columns - 1) / a.group;
-        most = col0 < columns ? max(ctx - rows + r + 1, 0) : 0;
-    }
-    const int least = col0 < columns ? max(ctx - rows + col0 / a.group + 1, 0) : 0; // the smallest limit
-    const int begin = chunk * a.chunk_tokens;
-    if (chunk > 0 && begin >= block_most) // nothing of this chunk is seen (the first one writes rows that see nothing)
-        return;
-    const int end = min(begin + a.chunk_tokens, most);
-
-    // Q^T operands: column l16, channels g*8*KK + kk*8 ..
-    Pieces q[NC][KK];
-#pragma unroll
-    for (int n = 0; n < NC; n++)
-#pragma unroll
-        for (int kk = 0; kk < KK; kk++) {
-            float x[8];
-            const int c0 = g * 8 * KK + kk * 8;
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                x[i] = 0.f;
-            if (out_row[n] >= 0 && c0 < a.mx.head_dim) {
-                const float *src = a.q + ((int64_t)out_row[n] * a.n_heads + out_head[n]) * a.mx.head_dim + c0;
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    x[i] = src[i];
-            }
-            q[n][kk] = split8(x);
-        }
-
-    f32x4 acc[NC][2 * KK];
-    float m[NC], l[NC];
-#pragma unroll
-    for (int n = 0; n < NC; n++) {
-        m[n] = -INFINITY, l[n] = 0.f;
-#pragma unroll
-        for (int ct = 0; ct < 2 * KK; ct++)
-            acc[n][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    int      lane, g, l16, lcol, piece; // lcol: the lane's column of a tile; PACK: `piece` is which copy of it
+    int      limit[NC], out_row[NC], out_head[NC]; // a column's row sees the tokens below `limit`: all up to its own
+    int      most, least;                          // the largest and the smallest limit of the wave's columns
+    bf16x8   q[NC][KK][PIECES];
+    f32x4    acc[NC][2 * KK]; // [ct][i]: channel (4 g + i) * 2 KK + ct
+    // m: what scores are taken relative to, a score that was the largest once (0 while lim is -inf: no token yet).  It is moved
+    // only where a score passes it by more than 8: probabilities up to 2^8 are as exact as those up to 1.
+    float    m[NC], lim[NC], l[NC];
     unsigned poisoned[NC]; // channel groups in which a token that the column sees holds no number
-#pragma unroll
-    for (int n = 0; n < NC; n++)
-        poisoned[n] = 0;
+    unsigned cut1, cut2;   // PACK: what a probability loses to become the lane's piece (the fourth copy's result is dropped)
 
-    // tiles of this wave: its step i covers the 32 tokens from begin + 32 * (wt + WT * i)
-    const int     steps = max(0, (end - begin + 31) / 32 - wt + WT - 1) / WT;
-    const int     last_tile = max((min(end, ctx) - 1) / kMx4Tile, 0);
-    const int     tiles_per_block = bs / kMx4Tile;
-    const int64_t head_at = (int64_t)kvh * mx4_tile_bytes(KK), tile_stride = (int64_t)a.mx.n_kv_heads * mx4_tile_bytes(KK);
-    const int    *table = a.tables + (int64_t)seq * a.max_blocks;
-    int           entry = 0; // lane L: the tile number in the layer of tile L % 2 of the wave's step (i & ~31) + L / 2
-    auto refill = [&](int i) {
-        const int t = min((begin >> 4) + 2 * (wt + WT * (i + (lane >> 1))) + (lane & 1), last_tile);
-        const int b = t / tiles_per_block;
-        entry = min(max(table[b], 0), a.mx.num_blocks - 1) * tiles_per_block + t % tiles_per_block;
-    };
-    auto fetch = [&](Mx4Raw<KK> (&r)[2], int i) {
-        if ((i & 31) == 0)
-            refill(i);
+    __device__ __forceinline__ void start(const Mx4AttnArgs &a, int row0, int rows, int ctx, int kvh, int col0)
+    {
+        lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
+        lcol = PACK ? l16 >> 2 : l16, piece = l16 & 3;
+        cut1 = piece > 0 ? 0xffff0000u : 0u, cut2 = piece > 1 ? 0xffff0000u : 0u;
+        const int columns = rows * a.group;
+        const int last = min(col0 + COLS * NC - 1, columns - 1) / a.group;
+        most  = col0 < columns ? max(ctx - rows + last + 1, 0) : 0;
+        least = col0 < columns ? max(ctx - rows + col0 / a.group + 1, 0) : 0;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int e = __builtin_amdgcn_readlane(entry, 2 * (i & 31) + j);
-            load_tile<KK>(r[j], a.mx.base + e * tile_stride + head_at, lane);
-        }
-    };
-
-    Mx4Raw<KK> ahead[AHEAD][2]; // tiles on their way: steps i, i + 1, ..
-#pragma unroll
-    for (int d = 0; d < AHEAD; d++)
-        if (d < steps)
-            fetch(ahead[d], d);
-    for (int i = 0; i < steps; i++) {
-        Mx4Raw<KK> raw[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            raw[j] = ahead[0][j];
-#pragma unroll
-            for (int d = 0; d + 1 < AHEAD; d++)
-                ahead[d][j] = ahead[d + 1][j];
-        }
-        if (i + AHEAD < steps)
-            fetch(ahead[AHEAD - 1], i + AHEAD);
-        const int t0 = begin + 32 * (wt + WT * i);
-
-        // A group of K or V that holds no number (scale byte 255) is dealt with before any product: this compiler does not
-        // keep the wait between a matrix instruction and the first read of its result across a branch, so none may stand there.
-        unsigned vs[2] = {raw[0].vs, raw[1].vs};
-        unsigned odd = 0; // bits 0..7: byte b of tile j's V scales; 8 + 2 j + u: K scale u of tile j
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-#pragma unroll
-            for (int b = 0; b < 4; b++)
-                odd |= (((vs[j] >> (8 * b)) & 255u) == 255u) ? 1u << (4 * j + b) : 0u;
-#pragma unroll
-            for (int u = 0; u < Mx4Raw<KK>::KS; u++)
-                odd |= raw[j].ks[u] == 255u ? 1u << (8 + 2 * j + u) : 0u;
-        }
-        // K, one operand after another; a token whose group of K holds no number has no scores either
-        bf16x8 k[2][KK];
-#pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int n = 0; n < NC; n++) {
+            const int col = col0 + COLS * n + lcol, r = col / a.group;
+            out_row[n]  = col < columns ? row0 + r : -1;
+            out_head[n] = kvh * a.group + col % a.group;
+            limit[n]    = col < columns ? max(ctx - rows + r + 1, 0) : 0;
+            // Q^T: channels g*8*KK + kk*8 .. of the column, in units in which a probability is a power of two
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
-                const float sc = scale_of(raw[j].ks[KK == 8 ? kk / 4 : 0]);
-                union
-                {
-                    unsigned u[4];
-                    bf16x8   v;
-                } w;
+                float     x[8];
+                const int c0 = g * 8 * KK + kk * 8;
 #pragma unroll
-                for (int b = 0; b < 4; b++)
-                    w.u[b] = two_values_at(raw[j].k[kk], sc, b);
-                k[j][kk] = w.v;
+                for (int i = 0; i < 8; i++)
+                    x[i] = 0.f;
+                if (out_row[n] >= 0 && c0 < a.mx.head_dim) {
+                    const float *src = a.q + ((int64_t)out_row[n] * a.n_heads + out_head[n]) * a.mx.head_dim + c0;
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        x[i] = src[i] * a.scale_log2e;
+                }
+                const Pieces three = split8(x);
+                if constexpr (PACK) {
+                    const u32x4 none = {0, 0, 0, 0};
+                    const u32x4 one  = piece == 0   ? __builtin_bit_cast(u32x4, three.p[0])
+                                       : piece == 1 ? __builtin_bit_cast(u32x4, three.p[1])
+                                       : piece == 2 ? __builtin_bit_cast(u32x4, three.p[2]) : none;
+                    q[n][kk][0] = __builtin_bit_cast(bf16x8, one);
+                }
+                else
+#pragma unroll
+                    for (int e = 0; e < 3; e++)
+                        q[n][kk][e] = three.p[e];
             }
-        if (__any(odd != 0)) {
-            const unsigned nan2 = 0x7fc07fc0u;
+            m[n] = 0.f, lim[n] = -INFINITY, l[n] = 0.f, poisoned[n] = 0;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int ct = 0; ct < 2 * KK; ct++)
+                acc[n][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    // A group of V that holds no number (scale byte 255): its scale is taken as 0, and the columns that see the token are marked.
+    // (One of K makes its token's scores NaN by itself.)  `vs`: the lane's V scales of the two tiles from token t0 on.
+    // Always before any product of a step: this compiler does not keep the wait between a matrix instruction and the first
+    // read of its result across a branch, so none may stand there.
+    __device__ __forceinline__ void mark(unsigned (&vs)[2], int t0)
+    {
+        if (__any((byte_255(vs[0]) | byte_255(vs[1])) != 0)) {
 #pragma unroll
-                for (int kk = 0; kk < KK; kk++)
-                    if ((odd >> (8 + 2 * j + (KK == 8 ? kk / 4 : 0))) & 1u)
-                        k[j][kk] = __builtin_bit_cast(bf16x8, make_uint4(nan2, nan2, nan2, nan2));
-                // V: the scale is taken as 0, and the columns that see the token are marked
+            for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
-                    unsigned long long who = __ballot((odd >> (4 * j + b)) & 1u);
-                    if ((odd >> (4 * j + b)) & 1u)
+                    const bool         odd = ((vs[j] >> (8 * b)) & 255u) == 255u;
+                    unsigned long long who = __ballot(odd);
+                    if (odd)
                         vs[j] &= ~(255u << (8 * b));
                     for (; who; who &= who - 1) { // lane (quad, c16) tells: token 4 quad + b of tile j, group of c16
                         const int from = __ffsll((long long)who) - 1;
@@ -324,184 +296,466 @@ __global__ void __launch_bounds__(64 * WT * WC, KK == 8 ? 1 : 2) nvk_mx4_attn_ke
                                 poisoned[n] |= 1u << ((from & 15) * KK / 16);
                     }
                 }
-            }
         }
+    }
 
-        // scores
-        f32x4 s[NC][2];
-#pragma unroll
-        for (int n = 0; n < NC; n++)
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-                s[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < KK; kk++)
-#pragma unroll
-            for (int p = 2; p >= 0; p--) // small pieces first
-#pragma unroll
-                for (int n = 0; n < NC; n++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-                        s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[j][kk], q[n][kk].p[p], s[n][j], 0, 0, 0);
+    // Where scores start: relative to m.
+    __device__ __forceinline__ f32x4 origin(int n) const
+    {
+        return PACK && piece ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{-m[n], -m[n], -m[n], -m[n]};
+    }
 
-        // softmax, in powers of two; p[n][j * 4 + i]: token t0 + 16 j + 4 g + i
-        Pieces p[NC];
+    // Scores of tile n (s[j][i]: token t0 + 16 j + 4 g + i) -> the pieces of its probabilities; maximum, sum and output follow.
+    __device__ __forceinline__ void softmax(int n, const f32x4 (&s)[2], int t0, bf16x8 (&p)[PIECES])
+    {
+        float t[8], top = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < NC; n++) {
-            float t[8], top = -INFINITY;
+        for (int e = 0; e < 8; e++) {
+            t[e] = s[e >> 2][e & 3];
+            if constexpr (PACK)
+                t[e] = sum_of_quad(t[e]);
+        }
+        if (t0 + 32 > least) {
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                t[e] = s[n][e >> 2][e & 3] * a.scale_log2e;
-            if (t0 + 32 > least) {
+                if (t0 + 16 * (e >> 2) + 4 * g + (e & 3) >= limit[n])
+                    t[e] = -INFINITY;
+        }
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (t0 + 16 * (e >> 2) + 4 * g + (e & 3) >= limit[n])
-                        t[e] = -INFINITY;
-            }
+        for (int e = 0; e < 8; e++)
+            top = fmaxf(top, t[e]);
+        top = max_of_g(top);
+        if (__any(top > lim[n])) {
+            const bool  over = top > lim[n];
+            const float up = over ? top : 0.f;
+            const float alpha = lim[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-up);
+            m[n] += up;
+            lim[n] = over ? 8.f : lim[n];
+            l[n] *= alpha;
+#pragma unroll
+            for (int ct = 0; ct < 2 * KK; ct++)
+                acc[n][ct] *= alpha;
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                top = fmaxf(top, t[e]);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            if (__any(top > m[n])) {
-                const float m_new = fmaxf(m[n], top);
-                const float alpha = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - m_new);
-                m[n] = m_new;
-                l[n] *= alpha;
-#pragma unroll
-                for (int ct = 0; ct < 2 * KK; ct++)
-                    acc[n][ct] *= alpha;
-            }
-            const float base = m[n] == -INFINITY ? 0.f : m[n];
-            float       sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                t[e] = __builtin_amdgcn_exp2f(t[e] - base);
-                sum += t[e];
-            }
-            l[n] += sum;
-            p[n] = split8(t);
+                t[e] -= up;
         }
-
-        // O += P V, two channels of a lane at a time
+        float sum = 0.f;
 #pragma unroll
-        for (int b = 0; b < KK; b++) {
-            unsigned w[2][4]; // tile, token: channels 2b and 2b + 1 of the lane's run
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-                    w[j][t] = two_values_at(raw[j].v[(t * KK + b) / 4], scale_of((vs[j] >> (8 * t)) & 255u), (t * KK + b) % 4);
+        for (int e = 0; e < 8; e++) {
+            t[e] = __builtin_amdgcn_exp2f(t[e]);
+            sum += t[e];
+        }
+        l[n] += sum;
+        if constexpr (PACK) { // the lane's own piece: what as many truncations leave
             union
             {
                 unsigned u[4];
                 bf16x8   v;
-            } lo, hi;
+            } w;
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int e = 0; e < 8; e++) {
+                t[e] -= __uint_as_float(__float_as_uint(t[e]) & cut1);
+                t[e] -= __uint_as_float(__float_as_uint(t[e]) & cut2);
+            }
 #pragma unroll
-                for (int t = 0; t < 4; t += 2) {
-                    lo.u[2 * j + t / 2] = __builtin_amdgcn_perm(w[j][t + 1], w[j][t], 0x05040100u);
-                    hi.u[2 * j + t / 2] = __builtin_amdgcn_perm(w[j][t + 1], w[j][t], 0x07060302u);
-                }
+            for (int e = 0; e < 4; e++)
+                w.u[e] = high_halves(t[2 * e], t[2 * e + 1]);
+            p[0] = w.v;
+        }
+        else {
+            const Pieces three = split8(t);
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                p[e] = three.p[e];
+        }
+    }
+
+    // After the last token: sums over the lanes that share a column; marked groups become NaN; m is -inf where no token was seen.
+    __device__ __forceinline__ void finish()
+    {
+        if constexpr (PACK) // the three copies of a column
 #pragma unroll
             for (int n = 0; n < NC; n++)
 #pragma unroll
-                for (int e = 2; e >= 0; e--) {
-                    acc[n][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo.v, p[n].p[e], acc[n][2 * b], 0, 0, 0);
-                    acc[n][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi.v, p[n].p[e], acc[n][2 * b + 1], 0, 0, 0);
-                }
-        }
-    }
-
-    // column sums over the four lane groups; marked groups become NaN.  acc[n][ct][i]: channel (4 g + i) * 2 KK + ct
+                for (int ct = 0; ct < 2 * KK; ct++)
 #pragma unroll
-    for (int n = 0; n < NC; n++) {
-        l[n] += __shfl_xor(l[n], 16);
-        l[n] += __shfl_xor(l[n], 32);
-        if (poisoned[n])
-#pragma unroll
-            for (int ct = 0; ct < 2 * KK; ct++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if ((poisoned[n] >> (((4 * g + i) * 2 * KK + ct) / 32)) & 1u)
-                        acc[n][ct][i] = __uint_as_float(0x7fc00000u);
-    }
-
-    if constexpr (WT == 1) {
+                    for (int i = 0; i < 4; i++)
+                        acc[n][ct][i] = sum_of_quad(piece == 3 ? 0.f : acc[n][ct][i]);
 #pragma unroll
         for (int n = 0; n < NC; n++) {
-            if (out_row[n] < 0)
-                continue;
-            const int64_t line = (int64_t)out_row[n] * a.n_heads + out_head[n];
-            float        *dst = a.out + line * a.mx.head_dim;
-            float         norm = l[n] == 0.f ? 0.f : 1.f / l[n];
-            if (a.chunks > 1) {
-                dst = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim;
-                norm = 1.f;
-                if (g == 0) {
-                    a.ws_ml[(line * a.chunks + chunk) * 2] = m[n];
-                    a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = l[n];
-                }
-            }
+            if (lim[n] == -INFINITY)
+                m[n] = -INFINITY;
+            l[n] += __shfl_xor(l[n], 16);
+            l[n] += __shfl_xor(l[n], 32);
+            if (poisoned[n])
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+                for (int ct = 0; ct < 2 * KK; ct++)
 #pragma unroll
-                for (int ct = 0; ct < 2 * KK; ct++) {
-                    const int c = (4 * g + i) * 2 * KK + ct;
-                    if (c < a.mx.head_dim)
-                        dst[c] = acc[n][ct][i] * norm;
-                }
+                    for (int i = 0; i < 4; i++)
+                        if ((poisoned[n] >> (((4 * g + i) * 2 * KK + ct) / 32)) & 1u)
+                            acc[n][ct][i] = __uint_as_float(0x7fc00000u);
         }
     }
-    else {
-        // join the waves: common maximum, then a sum over LDS, 16 columns x HDP channels in passes of one wave's results
-        __shared__ float s_m[WT][16], s_l[WT][16];
-        __shared__ __attribute__((aligned(16))) float s_o[WT][16][HDP + 4];
-        if (g == 0)
-            s_m[wave][l16] = m[0], s_l[wave][l16] = l[0];
-        __syncthreads();
-        float M = -INFINITY;
+};
+
+// K of a tile: 8 channels from one dword of codes.
+__device__ __forceinline__ bf16x8 k_operand(unsigned codes, float scale)
+{
+    union
+    {
+        unsigned u[4];
+        bf16x8   v;
+    } w;
 #pragma unroll
-        for (int w = 0; w < WT; w++)
-            M = fmaxf(M, s_m[w][l16]);
-        const float alpha = m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[0] - M);
+    for (int b = 0; b < 4; b++)
+        w.u[b] = two_values_at(codes, scale, b);
+    return w.v;
+}
+// V of two tiles: channels 2b and 2b + 1 of the lane's run, for its eight tokens.
+template <int KK>
+__device__ __forceinline__ void v_operands(const unsigned (&v0)[KK], const unsigned (&v1)[KK], const unsigned (&vs)[2], int b, bf16x8 &even,
+                                           bf16x8 &odd)
+{
+    unsigned w[2][4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        w[0][t] = two_values_at(v0[(t * KK + b) / 4], scale_at(vs[0], t), (t * KK + b) % 4);
+        w[1][t] = two_values_at(v1[(t * KK + b) / 4], scale_at(vs[1], t), (t * KK + b) % 4);
+    }
+    union
+    {
+        unsigned u[4];
+        bf16x8   v;
+    } lo, hi;
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int t = 0; t < 4; t += 2) {
+            lo.u[2 * j + t / 2] = __builtin_amdgcn_perm(w[j][t + 1], w[j][t], 0x05040100u);
+            hi.u[2 * j + t / 2] = __builtin_amdgcn_perm(w[j][t + 1], w[j][t], 0x07060302u);
+        }
+    even = lo.v, odd = hi.v;
+}
+
+// Where a workgroup's piece of context lies: tile `t` of the context -> its address.  A lane keeps one entry of the block
+// table; 64 tiles at a time.
+struct Mx4Tiles
+{
+    const unsigned char *base; // the layer, at the kv-head
+    const int           *table;
+    int64_t              stride; // bytes from one tile of the layer to the next
+    int                  per_block, last, num_blocks; // last: the last tile that may be asked for
+
+    __device__ __forceinline__ Mx4Tiles(const Mx4AttnArgs &a, int seq, int kvh, int last_tile)
+    {
+        base       = a.mx.base + (int64_t)kvh * mx4_tile_bytes(a.mx.kk);
+        table      = a.tables + (int64_t)seq * a.max_blocks;
+        stride     = (int64_t)a.mx.n_kv_heads * mx4_tile_bytes(a.mx.kk);
+        per_block  = a.mx.block_size / kMx4Tile;
+        last       = max(last_tile, 0);
+        num_blocks = a.mx.num_blocks;
+    }
+    // the tile's number in the layer (out of bounds entries are clamped)
+    __device__ __forceinline__ int entry(int t) const
+    {
+        t           = min(t, last);
+        const int b = t / per_block;
+        return min(max(table[b], 0), num_blocks - 1) * per_block + t % per_block;
+    }
+    __device__ __forceinline__ const unsigned char *at(int number) const { return base + number * stride; }
+};
+
+__device__ __forceinline__ int mx4_context(const Mx4AttnArgs &a, int seq)
+{
+    return min(max(a.ctx_lens[seq], 0), (int)min((int64_t)a.max_blocks * a.mx.block_size, (int64_t)0x7fffffff));
+}
+// rows of a sequence: [row0, row0 + rows)
+__device__ __forceinline__ int mx4_rows(const Mx4AttnArgs &a, int seq, int &row0)
+{
+    row0 = seq;
+    if (!a.row_offsets)
+        return 1;
+    row0 = a.row_offsets[seq];
+    return row0 < 0 ? 0 : min(a.row_offsets[seq + 1], a.total_rows) - row0;
+}
+
+// ---- few columns: the waves of a workgroup share the tokens --------------------------------------------------------------
+// Bound by the codes it reads while everything beside the loads hides behind them; what does not is the vector work of a
+// step.  WAVES waves take steps of 32 tokens in turn and join through LDS.
+template <int KK, bool PACK>
+__global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2) nvk_mx4_decode_kernel(const Mx4AttnArgs a)
+{
+    using Wave = Mx4Wave<KK, 1, PACK>;
+    constexpr int HDP = 32 * KK, COLS = Wave::COLS, W = kDecodeWaves;
+    const int     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // Workgroup -> (sequence, column block, chunk, kv-head).  Consecutive workgroups go to the eight XCDs in turn: the kv-heads
+    // of one piece of context are put side by side on one XCD, which then reads whole blocks of the cache.
+    const unsigned xcd = blockIdx.x % 8u, rest = blockIdx.x / 8u;
+    const int      kvh = (int)(rest % (unsigned)a.mx.n_kv_heads);
+    unsigned       unit = rest / (unsigned)a.mx.n_kv_heads * 8u + xcd;
+    const int      chunk = (int)(unit % (unsigned)a.chunks);
+    unit /= (unsigned)a.chunks;
+    const int cb = (int)(unit % (unsigned)a.col_blocks), seq = (int)(unit / (unsigned)a.col_blocks);
+    if (seq >= a.num_seqs)
+        return;
+    int       row0;
+    const int rows = mx4_rows(a, seq, row0), columns = rows * a.group, col0 = cb * COLS;
+    if (rows <= 0 || col0 >= columns)
+        return;
+    const int ctx = mx4_context(a, seq);
+    const int begin = chunk * a.chunk_tokens;
+    Wave      w;
+    w.start(a, row0, rows, ctx, kvh, col0);
+    if (chunk > 0 && begin >= w.most) // nothing of this chunk is seen (the first one writes rows that see nothing)
+        return;
+    const int end = min(begin + a.chunk_tokens, w.most);
+
+    // step i of this wave covers the 32 tokens from begin + 32 * (wave + W * i)
+    const int             steps = max(0, (end - begin + 31) / 32 - wave + W - 1) / W;
+    const Mx4Tiles        tiles(a, seq, kvh, (min(end, ctx) - 1) / kMx4Tile);
+    const Mx4Places<KK>   places(w.lane);
+    int                   entry = 0; // lane L: tile L % 2 of the wave's step (i & ~31) + L / 2
+    auto                  fetch = [&](Mx4Raw<KK> (&r)[2], int i) {
+        if ((i & 31) == 0)
+            entry = tiles.entry((begin >> 4) + 2 * (wave + W * (i + (w.lane >> 1))) + (w.lane & 1));
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            load_tile<KK>(r[j], tiles.at(__builtin_amdgcn_readlane(entry, 2 * (i & 31) + j)), places);
+    };
+    // one step on `raw`, while the next one's tiles are on their way into `next`
+    auto step = [&](int i, const Mx4Raw<KK> (&raw)[2], Mx4Raw<KK> (&next)[2]) {
+        if (i + 1 < steps)
+            fetch(next, i + 1);
+        const int t0 = begin + 32 * (wave + W * i);
+        unsigned  vs[2] = {raw[0].vs, raw[1].vs};
+        w.mark(vs, t0);
+        bf16x8 k[2][KK];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+                k[j][kk] = k_operand(raw[j].k[kk], scale_at(raw[j].ks[KK == 8 ? kk / 4 : 0], 0));
+        // the large pieces of q first: the sums of the small ones then round at the size of what is left
+        f32x4 s[2] = {w.origin(0), w.origin(0)};
+#pragma unroll
+        for (int e = 0; e < Wave::PIECES; e++)
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[j][kk], w.q[0][kk][e], s[j], 0, 0, 0);
+        bf16x8 p[Wave::PIECES];
+        w.softmax(0, s, t0, p);
+#pragma unroll
+        for (int b = 0; b < KK; b++) {
+            bf16x8 even, odd;
+            v_operands<KK>(raw[0].v, raw[1].v, vs, b, even, odd);
+#pragma unroll
+            for (int e = Wave::PIECES - 1; e >= 0; e--) {
+                w.acc[0][2 * b]     = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p[e], w.acc[0][2 * b], 0, 0, 0);
+                w.acc[0][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p[e], w.acc[0][2 * b + 1], 0, 0, 0);
+            }
+        }
+    };
+    Mx4Raw<KK> even[2], odd[2]; // in turn: no copies between the steps
+    if (steps > 0)
+        fetch(even, 0);
+    for (int i = 0; i < steps; i += 2) {
+        step(i, even, odd);
+        if (i + 1 < steps)
+            step(i + 1, odd, even);
+    }
+    w.finish();
+
+    // join the waves: common maximum, then a sum over LDS
+    __shared__ float s_m[W][COLS], s_l[W][COLS];
+    __shared__ __attribute__((aligned(16))) float s_o[W][COLS][HDP + 4];
+    const bool writes = !PACK || w.piece == 0;
+    if (w.g == 0 && writes)
+        s_m[wave][w.lcol] = w.m[0], s_l[wave][w.lcol] = w.l[0];
+    __syncthreads();
+    float M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < W; x++)
+        M = fmaxf(M, s_m[x][w.lcol]);
+    const float alpha = w.m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m[0] - M);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int ct = 0; ct < 2 * KK; ct++)
+            if (writes)
+                s_o[wave][w.lcol][(4 * w.g + i) * 2 * KK + ct] = w.acc[0][ct][i] * alpha;
+    __syncthreads();
+    for (int e = threadIdx.x; e < COLS * (HDP / 4); e += 64 * W) {
+        const int c16 = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
+        const int col = col0 + c16;
+        if (col >= columns || c >= a.mx.head_dim)
+            continue;
+        float Mc = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int x = 0; x < W; x++)
+            Mc = fmaxf(Mc, s_m[x][c16]);
+        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < W; x++) {
+            L += s_m[x][c16] == -INFINITY ? 0.f : s_l[x][c16] * __builtin_amdgcn_exp2f(s_m[x][c16] - Mc);
+            o += *reinterpret_cast<const f32x4 *>(&s_o[x][c16][c]);
+        }
+        const int64_t line = (int64_t)(row0 + col / a.group) * a.n_heads + kvh * a.group + col % a.group;
+        float        *dst = a.out + line * a.mx.head_dim + c;
+        if (a.chunks > 1) {
+            dst = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim + c;
+            if (c == 0) {
+                a.ws_ml[(line * a.chunks + chunk) * 2]     = Mc;
+                a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = L;
+            }
+        }
+        else
+            o *= L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            dst[i] = o[i];
+    }
+}
+
+// ---- many columns: the waves of a workgroup share the operands -------------------------------------------------------------
+// Bound by the matrix instructions (48 for a tile of columns, a step and 128 channels) once the codes are turned into operands
+// only once: the four waves of a workgroup convert a quarter of a step's K and V each into LDS, a step ahead, and read all
+// of it as 16-byte operands.  One barrier a step: a buffer is written while the other is read.
+template <int KK, int NC>
+__global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 : 2) nvk_mx4_prefill_kernel(const Mx4AttnArgs a)
+{
+    using Wave = Mx4Wave<KK, NC, false>;
+    constexpr int COLS = Wave::COLS * NC, W = kPrefillWaves;
+    __shared__ __attribute__((aligned(16))) bf16x8 s_k[2][2 * KK][64], s_v[2][2 * KK][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // Workgroup -> (kv-head, column block, chunk, sequence): kv-heads in turn, so that with eight of them the column blocks
+    // that read the same codes meet in the L2 of one XCD; the last column blocks, which see the most tokens, first.
+    unsigned  id = blockIdx.x;
+    const int kvh = (int)(id % (unsigned)a.mx.n_kv_heads);
+    id /= (unsigned)a.mx.n_kv_heads;
+    const int seq = (int)(id % (unsigned)a.num_seqs);
+    id /= (unsigned)a.num_seqs;
+    const int chunk = (int)(id % (unsigned)a.chunks);
+    const int cb = a.col_blocks - 1 - (int)(id / (unsigned)a.chunks);
+    int       row0;
+    const int rows = mx4_rows(a, seq, row0), columns = rows * a.group;
+    if (rows <= 0 || cb * W * COLS >= columns)
+        return;
+    const int ctx = mx4_context(a, seq);
+    const int begin = chunk * a.chunk_tokens;
+    const int last_row = min((cb + 1) * W * COLS - 1, columns - 1) / a.group;
+    const int block_most = max(ctx - rows + last_row + 1, 0); // the largest limit of the workgroup's columns
+    if (chunk > 0 && begin >= block_most)
+        return;
+    Wave w;
+    w.start(a, row0, rows, ctx, kvh, (cb * W + wave) * COLS);
+    const int end = min(begin + a.chunk_tokens, block_most);
+    const int steps = max(0, (end - begin + 31) / 32);
+
+    // This wave's share of a step: K operands kk of tile j for item = wave, wave + W, .. of (kk, j), V channel pairs b = wave, ..
+    const Mx4Tiles      tiles(a, seq, kvh, (min(end, ctx) - 1) / kMx4Tile);
+    const Mx4Places<KK> places(w.lane);
+    const int           tile_j = wave & 1; // (W is even: all K items of a wave lie in one tile)
+    Mx4Raw<KK>          raw[2];
+    int                 entry = 0; // lane L: tile L of the current 32 steps
+    auto                fetch = [&](int i) {
+        if ((i & 31) == 0)
+            entry = tiles.entry((begin >> 4) + 2 * i + w.lane);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            load_tile_part<KK>(raw[j], tiles.at(__builtin_amdgcn_readlane(entry, 2 * (i & 31) + j)), places, j == tile_j, wave < KK);
+    };
+    auto convert = [&](int i) {
+        unsigned vs[2] = {raw[0].vs, raw[1].vs};
+        w.mark(vs, begin + 32 * i);
+        const int   buf = i & 1;
+        const auto &mine = tile_j ? raw[1] : raw[0];
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
+            if ((kk * 2 + tile_j) % W == wave)
+                s_k[buf][kk * 2 + tile_j][w.lane] = k_operand(mine.k[kk], scale_at(mine.ks[KK == 8 ? kk / 4 : 0], 0));
+#pragma unroll
+        for (int b = 0; b < KK; b++)
+            if (b % W == wave) {
+                bf16x8 even, odd;
+                v_operands<KK>(raw[0].v, raw[1].v, vs, b, even, odd);
+                s_v[buf][2 * b][w.lane] = even, s_v[buf][2 * b + 1][w.lane] = odd;
+            }
+    };
+    if (steps > 0) {
+        fetch(0);
+        convert(0);
+        if (steps > 1)
+            fetch(1);
+    }
+    __syncthreads();
+    for (int i = 0; i < steps; i++) {
+        if (i + 1 < steps) {
+            convert(i + 1);
+            if (i + 2 < steps)
+                fetch(i + 2);
+        }
+        const int t0 = begin + 32 * i, buf = i & 1;
+        if (t0 < w.most) {
+            f32x4 s[NC][2];
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+                s[n][0] = w.origin(n), s[n][1] = w.origin(n);
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const bf16x8 k = s_k[buf][kk * 2 + j][w.lane];
+#pragma unroll
+                        for (int n = 0; n < NC; n++)
+                            s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, w.q[n][kk][e], s[n][j], 0, 0, 0);
+                    }
+            bf16x8 p[NC][3];
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+                w.softmax(n, s[n], t0, p[n]);
+#pragma unroll
+            for (int ct = 0; ct < 2 * KK; ct++) {
+                const bf16x8 v = s_v[buf][ct][w.lane];
+#pragma unroll
+                for (int n = 0; n < NC; n++)
+#pragma unroll
+                    for (int e = 2; e >= 0; e--)
+                        w.acc[n][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n][e], w.acc[n][ct], 0, 0, 0);
+            }
+        }
+        __syncthreads();
+    }
+    w.finish();
+
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        if (w.out_row[n] < 0)
+            continue;
+        const int64_t line = (int64_t)w.out_row[n] * a.n_heads + w.out_head[n];
+        float        *dst = a.out + line * a.mx.head_dim;
+        float         norm = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
+        if (a.chunks > 1) {
+            dst  = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim;
+            norm = 1.f;
+            if (w.g == 0) {
+                a.ws_ml[(line * a.chunks + chunk) * 2]     = w.m[n];
+                a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = w.l[n];
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int ct = 0; ct < 2 * KK; ct++)
-                s_o[wave][l16][(4 * g + i) * 2 * KK + ct] = acc[0][ct][i] * alpha;
-        __syncthreads();
-        for (int e = threadIdx.x; e < 16 * (HDP / 4); e += 64 * WT) {
-            const int c16 = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
-            const int col = col0 + c16;
-            if (col >= columns || c >= a.mx.head_dim)
-                continue;
-            float Mc = -INFINITY, L = 0.f;
-#pragma unroll
-            for (int w = 0; w < WT; w++)
-                Mc = fmaxf(Mc, s_m[w][c16]);
-            f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < WT; w++) {
-                L += s_m[w][c16] == -INFINITY ? 0.f : s_l[w][c16] * __builtin_amdgcn_exp2f(s_m[w][c16] - Mc);
-                o += *reinterpret_cast<const f32x4 *>(&s_o[w][c16][c]);
+            for (int ct = 0; ct < 2 * KK; ct++) {
+                const int c = (4 * w.g + i) * 2 * KK + ct;
+                if (c < a.mx.head_dim)
+                    dst[c] = w.acc[n][ct][i] * norm;
             }
-            const int64_t line = (int64_t)(row0 + col / a.group) * a.n_heads + kvh * a.group + col % a.group;
-            float        *dst = a.out + line * a.mx.head_dim + c;
-            if (a.chunks > 1) {
-                dst = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim + c;
-                if (c == 0) {
-                    a.ws_ml[(line * a.chunks + chunk) * 2] = Mc;
-                    a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = L;
-                }
-            }
-            else
-                o *= L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                dst[i] = o[i];
-        }
     }
 }
 
@@ -571,12 +825,12 @@ namespace {
 
 using nvk::Mx4AttnArgs;
 
-constexpr int kDecodeWaves = 4, kPrefillWaves = 4;
+using nvk::kDecodeWaves, nvk::kPrefillWaves;
 constexpr int prefill_cols(int kk) { return kk == 8 ? 1 : 2; } // columns of a prefill wave: 16 times this (registers)
 
 struct Mx4Shape
 {
-    bool   prefill = false;
+    bool   prefill = false, pack = false;
     int    col_blocks = 1, chunk_tokens = 32, chunks = 1;
     size_t ws_floats = 0;
 };
@@ -589,14 +843,16 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     Mx4Shape  s;
     const int group = n_heads / pool->n_kv_heads;
     // Waves that share the tokens while one wave holds a sequence's columns; else waves that share the columns.
-    s.prefill    = (long long)max_rows * group > 16;
+    s.prefill = (long long)max_rows * group > 16;
+    s.pack    = (long long)max_rows * group <= 4;
     const int cols = s.prefill ? 16 * prefill_cols(pool->kk) * kPrefillWaves : 16;
     s.col_blocks = ceil_div((long long)max_rows * group, cols);
     const long long tasks = (long long)num_seqs * pool->n_kv_heads * s.col_blocks;
-    // workgroups wanted: four to a CU; a chunk is worth its start and its join from 256 tokens on
-    const int wanted = ceil_div(MX4_WGS * pool->num_cus, std::max(tasks, 1LL));
-    const int most = std::max(1, max_ctx / 256);
-    s.chunks       = std::max(1, std::min(wanted, most));
+    // Cut the context while everything still runs at once (workgroups of four waves: so many fit a CU), into chunks of 256
+    // tokens at least.
+    const long long fit = (s.pack && pool->kk <= 4 ? 3LL : 2LL) * pool->num_cus;
+    const int       most = std::max(1, max_ctx / 256);
+    s.chunks       = (int)std::max(1LL, std::min(fit / std::max(tasks, 1LL), (long long)most));
     s.chunk_tokens = std::max(32, ceil_div(ceil_div(max_ctx, s.chunks), 32) * 32);
     s.chunks       = std::max(1, ceil_div(max_ctx, s.chunk_tokens));
     s.ws_floats    = s.chunks > 1 ? (size_t)total_rows * n_heads * s.chunks * (pool->head_dim + 2) : 0;
@@ -606,10 +862,11 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
 template <int KK> void launch_attn(const Mx4AttnArgs &a, const Mx4Shape &s, unsigned blocks, hipStream_t st)
 {
     if (s.prefill)
-        hipLaunchKernelGGL((nvk::nvk_mx4_attn_kernel<KK, prefill_cols(KK), 1, kPrefillWaves>), dim3(blocks),
-                           dim3(64 * kPrefillWaves), 0, st, a);
+        hipLaunchKernelGGL((nvk::nvk_mx4_prefill_kernel<KK, prefill_cols(KK)>), dim3(blocks), dim3(64 * kPrefillWaves), 0, st, a);
+    else if (s.pack)
+        hipLaunchKernelGGL((nvk::nvk_mx4_decode_kernel<KK, true>), dim3(blocks), dim3(64 * kDecodeWaves), 0, st, a);
     else
-        hipLaunchKernelGGL((nvk::nvk_mx4_attn_kernel<KK, 1, kDecodeWaves, 1>), dim3(blocks), dim3(64 * kDecodeWaves), 0, st, a);
+        hipLaunchKernelGGL((nvk::nvk_mx4_decode_kernel<KK, false>), dim3(blocks), dim3(64 * kDecodeWaves), 0, st, a);
 }
 
 int check_attention(const nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, int total_rows, int max_rows, int max_blocks,
@@ -634,7 +891,8 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
                       float *out, hipStream_t st, const char *who)
 {
     const Mx4Shape  s = mx4_shape(pool, num_seqs, n_heads, total_rows, max_rows, max_ctx);
-    const long long blocks = (long long)num_seqs * pool->n_kv_heads * s.col_blocks * s.chunks;
+    const long long units = (long long)num_seqs * s.col_blocks * s.chunks;
+    const long long blocks = (s.prefill ? units : (units + 7) / 8 * 8) * pool->n_kv_heads; // (decode: whole rounds of the XCDs)
     if (blocks > 0x7fffffffLL)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %lld workgroups", who, blocks);
     int rc = nvk::grow_workspace(&pool->ws, &pool->ws_floats, &pool->ws_generation, s.ws_floats, st, who);
