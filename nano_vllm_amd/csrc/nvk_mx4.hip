@@ -13,6 +13,7 @@
 #include <cmath>
 #include <new>
 
+#include "nvk_chunk_join.hip.h"
 #include "nvk_hip_util.h"
 #include "nvk_mx4.hip.h"
 
@@ -759,17 +760,14 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 
     }
 }
 
-// Joins the chunks of a (row, head): one wave each.
-__global__ void __launch_bounds__(256) nvk_mx4_merge_kernel(const Mx4AttnArgs a)
+// a workgroup per (row, head)
+__global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_kernel(const Mx4AttnArgs a)
 {
-    const int64_t line = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int     lane = threadIdx.x & 63;
-    if (line >= (int64_t)a.total_rows * a.n_heads)
-        return;
-    const int row = (int)(line / a.n_heads);
-    int       seq = row, rows = 1, row0 = row;
-    if (a.row_offsets) { // the sequence whose rows hold this one
-        int lo = 0, hi = a.num_seqs; // offsets[lo] <= row < offsets[hi]
+    const int64_t line = blockIdx.x;
+    const int     row = (int)(line / a.n_heads);
+    int           seq = row, rows = 1, row0 = row;
+    if (a.row_offsets) { // the sequence whose rows hold this one: offsets[lo] <= row < offsets[hi]
+        int lo = 0, hi = a.num_seqs;
         if (row < a.row_offsets[0] || row >= a.row_offsets[a.num_seqs])
             return;
         while (hi - lo > 1) {
@@ -779,44 +777,12 @@ __global__ void __launch_bounds__(256) nvk_mx4_merge_kernel(const Mx4AttnArgs a)
             else
                 hi = mid;
         }
-        seq = lo, row0 = a.row_offsets[lo], rows = min(a.row_offsets[lo + 1], a.total_rows) - row0;
+        seq  = lo;
+        rows = mx4_rows(a, seq, row0);
     }
-    const int ctx = min(max(a.ctx_lens[seq], 0), (int)min((int64_t)a.max_blocks * a.mx.block_size, (int64_t)0x7fffffff));
-    const int limit = max(ctx - rows + (row - row0) + 1, 0);
+    const int limit = max(mx4_context(a, seq) - rows + (row - row0) + 1, 0);
     const int n = min(max((limit + a.chunk_tokens - 1) / a.chunk_tokens, 1), a.chunks);
-    const float *ml = a.ws_ml + line * a.chunks * 2, *o = a.ws_o + line * a.chunks * a.mx.head_dim;
-    // a lane takes every 64th chunk's maximum, then its weight; the outputs are summed in chunk order
-    float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = lane; c < n; c += 64)
-        M = fmaxf(M, ml[2 * c]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        M = fmaxf(M, __shfl_xor(M, o));
-    for (int c0 = 0; c0 < n; c0 += 64) {
-        float w = 0.f;
-        if (c0 + lane < n) {
-            const float m = ml[2 * (c0 + lane)];
-            w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-            L += ml[2 * (c0 + lane) + 1] * w;
-        }
-        const int some = min(64, n - c0);
-#pragma unroll 4
-        for (int c = 0; c < some; c++) {
-            const float f = __shfl(w, c);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (lane + 64 * i < a.mx.head_dim)
-                    x[i] += o[(int64_t)(c0 + c) * a.mx.head_dim + lane + 64 * i] * f;
-        }
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        L += __shfl_xor(L, o);
-    const float norm = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (lane + 64 * i < a.mx.head_dim)
-            a.out[line * a.mx.head_dim + lane + 64 * i] = x[i] * norm;
+    join_chunks(a.ws_o + line * a.chunks * a.mx.head_dim, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim, a.out + line * a.mx.head_dim);
 }
 
 } // namespace nvk
@@ -893,7 +859,7 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
     const Mx4Shape  s = mx4_shape(pool, num_seqs, n_heads, total_rows, max_rows, max_ctx);
     const long long units = (long long)num_seqs * s.col_blocks * s.chunks;
     const long long blocks = (s.prefill ? units : (units + 7) / 8 * 8) * pool->n_kv_heads; // (decode: whole rounds of the XCDs)
-    if (blocks > 0x7fffffffLL)
+    if (blocks > 0x7fffffffLL || (long long)total_rows * n_heads > 0x7fffffffLL)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %lld workgroups", who, blocks);
     int rc = nvk::grow_workspace(&pool->ws, &pool->ws_floats, &pool->ws_generation, s.ws_floats, st, who);
     if (rc != NVK_OK)
@@ -915,7 +881,7 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
     }
     NVK_HIP_TRY(hipGetLastError());
     if (s.chunks > 1) {
-        hipLaunchKernelGGL(nvk::nvk_mx4_merge_kernel, dim3((unsigned)(((long long)total_rows * n_heads + 3) / 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(nvk::nvk_mx4_join_kernel, dim3((unsigned)(total_rows * n_heads)), dim3(nvk::kJoinThreads), 0, st, a);
         NVK_HIP_TRY(hipGetLastError());
     }
     return NVK_OK;

@@ -15,6 +15,7 @@
 #include <cmath>
 #include <new>
 
+#include "nvk_chunk_join.hip.h"
 #include "nvk_hip_util.h"
 
 struct nvk_block_index
@@ -50,6 +51,50 @@ struct SparseArgs
     float        scale_log2e;
     float       *ws_o, *ws_ml;
 };
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// rows of keys, values and bounds are read once by a launch: not worth keeping in the caches
+__device__ __forceinline__ float4 load_once(const float *p)
+{
+    const f32x4 t = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(p));
+    return make_float4(t.x, t.y, t.z, t.w);
+}
+
+// Exchanges inside a row of sixteen lanes, on the vector pipe.
+// lane ^ 1, lane ^ 2, lane ^ 7, and turned by 4 and by 8
+constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kFlip8 = 0x141, kTurn4 = 0x124, kTurn8 = 0x128;
+template <int C> __device__ __forceinline__ float across(float x)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), C, 0xF, 0xF, true));
+}
+template <int C> __device__ __forceinline__ double across(double x)
+{
+    const long long b = __double_as_longlong(x);
+    const int       lo = __builtin_amdgcn_update_dpp(0, (int)b, C, 0xF, 0xF, true);
+    const int       hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), C, 0xF, 0xF, true);
+    return __longlong_as_double((long long)hi << 32 | (unsigned)lo);
+}
+// Sums of a over lanes l and l ^ 32 in the lower half of the wave, of b in the upper; of a over l and l ^ 16 in rows 0 and 2, of
+// b in rows 1 and 3.
+__device__ __forceinline__ float fold32(float a, float b)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float fold16(float a, float b)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Of a value that lane l carries for head l % HG: head h's (a constant after unrolling), in every lane of the quad.
+template <int HG> __device__ __forceinline__ float of_head(float x, int h)
+{
+    if constexpr (HG == 1)
+        return x;
+    return h == 0 ? across<0x00>(x) : h == 1 ? across<0x55>(x) : h == 2 ? across<0xAA>(x) : across<0xFF>(x);
+}
 
 __device__ __forceinline__ int context_of(const SparseArgs &a, int seq)
 {
@@ -109,7 +154,8 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
         return;
     const int  hd = a.head_dim;
     float     *score = a.scores + ((int64_t)seq * a.n_kv_heads + kvh) * a.max_nb;
-    const int *table = a.tables + (int64_t)seq * a.max_blocks;
+    // (a wave's blocks are at most 64: a lane keeps the place of one)
+    const int entry = min(max(a.tables[(int64_t)seq * a.max_blocks + min(begin + lane, end - 1)], 0), a.num_blocks - 1);
     for (int h0 = 0; h0 < a.group; h0 += HG) {
         double w[HG][NV][4];
 #pragma unroll
@@ -126,20 +172,23 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
                 w[h][j][0] = low ? fminf(x.x, 0.f) : fmaxf(x.x, 0.f), w[h][j][1] = low ? fminf(x.y, 0.f) : fmaxf(x.y, 0.f);
                 w[h][j][2] = low ? fminf(x.z, 0.f) : fmaxf(x.z, 0.f), w[h][j][3] = low ? fminf(x.w, 0.f) : fmaxf(x.w, 0.f);
             }
-        for (int b0 = begin; b0 < end; b0 += 4) {
-            const int    b = min(b0 + sub, end - 1);
-            const int    pb = min(max(table[b], 0), a.num_blocks - 1);
+        float4 x[2][NV]; // two groups of four blocks: one in work, one on its way
+        auto   fetch = [&](float4 (&to)[NV], int b0) {
+            const int    pb = __shfl(entry, min(b0 + sub, end - 1) - begin);
             const float *src = a.bounds + ((int64_t)pb * a.n_kv_heads + kvh) * 2 * hd;
-            double       s[HG];
-#pragma unroll
-            for (int h = 0; h < HG; h++)
-                s[h] = 0.0;
-            float4 x[NV];
 #pragma unroll
             for (int j = 0; j < NV; j++) {
                 const int c = (l16 + 16 * j) * 4;
-                x[j] = c < 2 * hd ? *reinterpret_cast<const float4 *>(src + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                to[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c < 2 * hd)
+                    to[j] = load_once(src + c);
             }
+        };
+        auto take = [&](const float4 (&x)[NV], int b0) {
+            double s[HG];
+#pragma unroll
+            for (int h = 0; h < HG; h++)
+                s[h] = 0.0;
 #pragma unroll
             for (int j = 0; j < NV; j++)
 #pragma unroll
@@ -150,28 +199,38 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
             // sums over the block's sixteen lanes; with several heads, each exchange halves the heads a lane carries
             double mine;
             if constexpr (HG == 4) {
-                const bool o1 = lane & 1, o2 = lane & 2;
-                double     t0 = o1 ? s[2] : s[0], t1 = o1 ? s[3] : s[1];
-                t0 += __shfl_xor(o1 ? s[0] : s[2], 1), t1 += __shfl_xor(o1 ? s[1] : s[3], 1);
-                mine = (o2 ? t1 : t0) + __shfl_xor(o2 ? t0 : t1, 2);
+                const bool   o1 = lane & 1, o2 = lane & 2;
+                const double t0 = (o1 ? s[2] : s[0]) + across<kSwap1>(o1 ? s[0] : s[2]);
+                const double t1 = (o1 ? s[3] : s[1]) + across<kSwap1>(o1 ? s[1] : s[3]);
+                mine = (o2 ? t1 : t0) + across<kSwap2>(o2 ? t0 : t1);
             }
             else if constexpr (HG == 2) {
                 const bool o1 = lane & 1;
-                mine = (o1 ? s[1] : s[0]) + __shfl_xor(o1 ? s[0] : s[1], 1);
-                mine += __shfl_xor(mine, 2);
+                mine = (o1 ? s[1] : s[0]) + across<kSwap1>(o1 ? s[0] : s[1]);
+                mine += across<kSwap2>(mine);
             }
             else {
-                mine = s[0] + __shfl_xor(s[0], 1);
-                mine += __shfl_xor(mine, 2);
+                mine = s[0] + across<kSwap1>(s[0]);
+                mine += across<kSwap2>(mine);
             }
-            mine += __shfl_xor(mine, 4);
-            mine += __shfl_xor(mine, 8);
+            mine += across<kTurn4>(mine);
+            mine += across<kTurn8>(mine);
             float best = (float)mine;
             best       = best != best ? INFINITY : best; // no number: as high as can be
-            best       = fmaxf(best, __shfl_xor(best, 1));
-            best       = fmaxf(best, __shfl_xor(best, 2));
+            best       = fmaxf(best, across<kSwap1>(best));
+            best       = fmaxf(best, across<kSwap2>(best));
             if (l16 == 0 && b0 + sub < end)
-                score[b] = h0 > 0 ? fmaxf(score[b], best) : best;
+                score[b0 + sub] = h0 > 0 ? fmaxf(score[b0 + sub], best) : best;
+        };
+        fetch(x[0], begin);
+        for (int b0 = begin; b0 < end; b0 += 8) {
+            if (b0 + 4 < end)
+                fetch(x[1], b0 + 4);
+            take(x[0], b0);
+            if (b0 + 8 < end)
+                fetch(x[0], b0 + 8);
+            if (b0 + 4 < end)
+                take(x[1], b0 + 4);
         }
     }
 }
@@ -325,8 +384,8 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
             const int c = (l8 + 8 * j) * 4;
             k[j] = make_float4(0.f, 0.f, 0.f, 0.f), v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (there && c < hd) {
-                k[j] = *reinterpret_cast<const float4 *>(a.k + at + c);
-                v[j] = *reinterpret_cast<const float4 *>(a.v + at + c);
+                k[j] = load_once(a.k + at + c);
+                v[j] = load_once(a.v + at + c);
             }
         }
         return there;
@@ -353,24 +412,26 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
                 s[h] = fmaf(q[h][j].z, k[j].z, s[h]), s[h] = fmaf(q[h][j].w, k[j].w, s[h]);
             }
         }
+        // over the token's eight lanes (l and l ^ 7 first); afterwards lane l carries head l % HG
+#pragma unroll
+        for (int h = 0; h < HG; h++)
+            s[h] += across<kFlip8>(s[h]);
         float mine;
         if constexpr (HG == 4) {
-            const bool o1 = lane & 1, o2 = lane & 2;
-            // after the first exchange odd lanes carry heads 1 and 3, so that a lane ends with head lane % 4
-            float t0 = o1 ? s[1] : s[0], t1 = o1 ? s[3] : s[2];
-            t0 += __shfl_xor(o1 ? s[0] : s[1], 1), t1 += __shfl_xor(o1 ? s[2] : s[3], 1);
-            mine = (o2 ? t1 : t0) + __shfl_xor(o2 ? t0 : t1, 2);
+            const bool  o1 = lane & 1, o2 = lane & 2;
+            const float t0 = (o1 ? s[1] : s[0]) + across<kSwap1>(o1 ? s[0] : s[1]);
+            const float t1 = (o1 ? s[3] : s[2]) + across<kSwap1>(o1 ? s[2] : s[3]);
+            mine = (o2 ? t1 : t0) + across<kSwap2>(o2 ? t0 : t1);
         }
         else if constexpr (HG == 2) {
             const bool o1 = lane & 1;
-            mine = (o1 ? s[1] : s[0]) + __shfl_xor(o1 ? s[0] : s[1], 1);
-            mine += __shfl_xor(mine, 2);
+            mine = (o1 ? s[1] : s[0]) + across<kSwap1>(o1 ? s[0] : s[1]);
+            mine += across<kSwap2>(mine);
         }
         else {
-            mine = s[0] + __shfl_xor(s[0], 1);
-            mine += __shfl_xor(mine, 2);
+            mine = s[0] + across<kSwap1>(s[0]);
+            mine += across<kSwap2>(mine);
         }
-        mine += __shfl_xor(mine, 4);
         const float t = there ? mine * a.scale_log2e : -INFINITY;
         if (__any(t > m)) {
             const float m_new = fmaxf(m, t);
@@ -379,7 +440,7 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
             l *= alpha;
 #pragma unroll
             for (int h = 0; h < HG; h++) {
-                const float x = __shfl(alpha, (lane & 56) | h);
+                const float x = of_head<HG>(alpha, h);
 #pragma unroll
                 for (int j = 0; j < NV; j++)
                     o[h][j].x *= x, o[h][j].y *= x, o[h][j].z *= x, o[h][j].w *= x;
@@ -389,7 +450,7 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
         l += p;
 #pragma unroll
         for (int h = 0; h < HG; h++) {
-            const float x = __shfl(p, (lane & 56) | h);
+            const float x = of_head<HG>(p, h);
 #pragma unroll
             for (int j = 0; j < NV; j++) {
                 o[h][j].x = fmaf(x, v[j].x, o[h][j].x), o[h][j].y = fmaf(x, v[j].y, o[h][j].y);
@@ -412,15 +473,14 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
         s_m[wave][lane] = M, s_l[wave][lane] = l;
 #pragma unroll
     for (int h = 0; h < HG; h++) {
-        const float x = __shfl(alpha, (lane & 56) | h);
+        const float x = of_head<HG>(alpha, h);
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            float4 y = make_float4(o[h][j].x * x, o[h][j].y * x, o[h][j].z * x, o[h][j].w * x);
-#pragma unroll
-            for (int e = 8; e <= 32; e <<= 1)
-                y.x += __shfl_xor(y.x, e), y.y += __shfl_xor(y.y, e), y.z += __shfl_xor(y.z, e), y.w += __shfl_xor(y.w, e);
-            if (tg == 0)
-                *reinterpret_cast<float4 *>(&s_o[wave][h][(l8 + 8 * j) * 4]) = y;
+            // row r of the wave ends with component r, twice in its sixteen lanes
+            float y = fold16(fold32(o[h][j].x * x, o[h][j].z * x), fold32(o[h][j].y * x, o[h][j].w * x));
+            y += across<kTurn8>(y);
+            if ((lane & 8) == 0)
+                s_o[wave][h][(l8 + 8 * j) * 4 + (lane >> 4)] = y;
         }
     }
     __syncthreads();
@@ -447,31 +507,13 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
     }
 }
 
-// joins the chunks of a (sequence, head): one wave each
-__global__ void __launch_bounds__(256) nvk_sparse_merge_kernel(const SparseArgs a)
+// a workgroup per (sequence, head)
+__global__ void __launch_bounds__(kJoinThreads) nvk_sparse_join_kernel(const SparseArgs a)
 {
-    const int64_t line = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int     lane = threadIdx.x & 63;
-    if (line >= (int64_t)a.num_seqs * a.n_heads)
-        return;
-    const int    ctx = context_of(a, (int)(line / a.n_heads)), nb = (ctx + a.block_size - 1) / a.block_size;
-    const int    n = max((min(nb, a.top) + a.blocks_per_chunk - 1) / a.blocks_per_chunk, 1);
-    const float *ml = a.ws_ml + line * a.chunks * 2, *o = a.ws_o + line * a.chunks * a.head_dim;
-    float        M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < n; c++)
-        M = fmaxf(M, ml[2 * c]);
-    for (int c = 0; c < n; c++) {
-        const float w = ml[2 * c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * c] - M);
-        L += ml[2 * c + 1] * w;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < a.head_dim)
-                x[i] += o[(int64_t)c * a.head_dim + lane + 64 * i] * w;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (lane + 64 * i < a.head_dim)
-            a.out[line * a.head_dim + lane + 64 * i] = L == 0.f ? x[i] : x[i] / L;
+    const int64_t line = blockIdx.x;
+    const int     ctx = context_of(a, (int)(line / a.n_heads)), nb = (ctx + a.block_size - 1) / a.block_size;
+    const int     n = max((min(nb, a.top) + a.blocks_per_chunk - 1) / a.blocks_per_chunk, 1);
+    join_chunks(a.ws_o + line * a.chunks * a.head_dim, a.ws_ml + line * a.chunks * 2, n, a.head_dim, a.out + line * a.head_dim);
 }
 
 } // namespace nvk
@@ -617,7 +659,7 @@ int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, con
 {
     const SparseShape s = sparse_shape(x, num_seqs, n_heads, max_ctx, top);
     const long long   lines = (long long)num_seqs * x->n_kv_heads;
-    if (lines * s.score_slots > 0x7fffffffLL || lines * s.head_sets * s.chunks > 0x7fffffffLL)
+    if (lines * s.score_slots > 0x7fffffffLL || (long long)num_seqs * n_heads > 0x7fffffffLL || lines * s.head_sets * s.chunks > 0x7fffffffLL)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: too many workgroups", who);
     int rc = nvk::grow_workspace(&x->ws, &x->ws_floats, &x->ws_generation, s.floats(), st, who);
     if (rc != NVK_OK)
@@ -644,7 +686,7 @@ int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, con
     }
     NVK_HIP_TRY(hipGetLastError());
     if (s.chunks > 1) {
-        hipLaunchKernelGGL(nvk::nvk_sparse_merge_kernel, dim3((unsigned)ceil_div((long long)num_seqs * n_heads, 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(nvk::nvk_sparse_join_kernel, dim3((unsigned)(num_seqs * n_heads)), dim3(nvk::kJoinThreads), 0, st, a);
         NVK_HIP_TRY(hipGetLastError());
     }
     return NVK_OK;
