@@ -172,7 +172,8 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
                 w[h][j][0] = low ? fminf(x.x, 0.f) : fmaxf(x.x, 0.f), w[h][j][1] = low ? fminf(x.y, 0.f) : fmaxf(x.y, 0.f);
                 w[h][j][2] = low ? fminf(x.z, 0.f) : fmaxf(x.z, 0.f), w[h][j][3] = low ? fminf(x.w, 0.f) : fmaxf(x.w, 0.f);
             }
-        float4 x[2][NV]; // two groups of four blocks: one in work, one on its way
+        constexpr int RING = NV < 8 ? 3 : 2; // groups of four blocks: one in work, the others on their way
+        float4        x[RING][NV];
         auto   fetch = [&](float4 (&to)[NV], int b0) {
             const int    pb = __shfl(entry, min(b0 + sub, end - 1) - begin);
             const float *src = a.bounds + ((int64_t)pb * a.n_kv_heads + kvh) * 2 * hd;
@@ -222,15 +223,18 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
             if (l16 == 0 && b0 + sub < end)
                 score[b0 + sub] = h0 > 0 ? fmaxf(score[b0 + sub], best) : best;
         };
-        fetch(x[0], begin);
-        for (int b0 = begin; b0 < end; b0 += 8) {
-            if (b0 + 4 < end)
-                fetch(x[1], b0 + 4);
-            take(x[0], b0);
-            if (b0 + 8 < end)
-                fetch(x[0], b0 + 8);
-            if (b0 + 4 < end)
-                take(x[1], b0 + 4);
+#pragma unroll
+        for (int d = 0; d + 1 < RING; d++)
+            if (begin + 4 * d < end)
+                fetch(x[d], begin + 4 * d);
+        for (int b0 = begin; b0 < end; b0 += 4 * RING) {
+#pragma unroll
+            for (int d = 0; d < RING; d++)
+                if (b0 + 4 * d < end) {
+                    if (b0 + 4 * (d + RING - 1) < end)
+                        fetch(x[(d + RING - 1) % RING], b0 + 4 * (d + RING - 1));
+                    take(x[d], b0 + 4 * d);
+                }
         }
     }
 }
@@ -238,7 +242,8 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
 // ---- selection --------------------------------------------------------------------------------------------------------
 // One workgroup per (sequence, kv-head): the key of the last block that is read by four counting passes over the bytes of the
 // keys, then the blocks above it, and as many of those level with it as are left, lowest first, in ascending order.
-constexpr int kSelectThreads = 1024;
+// T threads; HELD: a thread keeps its (at most kHeldKeys) keys, else it reads the scores again for every pass.
+constexpr int kHeldKeys = 8;
 
 __device__ __forceinline__ unsigned block_key(const SparseArgs &a, const float *score, int b, int nb)
 {
@@ -248,40 +253,59 @@ __device__ __forceinline__ unsigned block_key(const SparseArgs &a, const float *
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const SparseArgs a)
+template <int T, bool HELD> __global__ void __launch_bounds__(T) nvk_block_select_kernel(const SparseArgs a)
 {
-    __shared__ int      s_count[256];
+    constexpr int W = T / 64;
+    __shared__ int      s_count[4][256];
     __shared__ unsigned s_prefix;
     __shared__ int      s_left;
-    __shared__ int      s_wave[2][kSelectThreads / 64];
+    __shared__ int      s_wave[2][2][W];
     const int    line = blockIdx.x, seq = line / a.n_kv_heads;
     const int    tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int    ctx = context_of(a, seq), nb = (ctx + a.block_size - 1) / a.block_size;
     int         *chosen = a.chosen + (int64_t)line * a.top;
     const float *score = a.scores + (int64_t)line * a.max_nb;
     if (nb <= a.top) {
-        for (int i = tid; i < a.top; i += kSelectThreads)
+        for (int i = tid; i < a.top; i += T)
             chosen[i] = i < nb ? i : -1;
         return;
     }
+    unsigned held[HELD ? kHeldKeys : 1];
+    if constexpr (HELD)
+#pragma unroll
+        for (int i = 0; i < kHeldKeys; i++)
+            held[i] = tid + T * i < nb ? block_key(a, score, tid + T * i, nb) : 0u;
+    // f(block, key) for every block of this thread
+    auto each = [&](auto f) {
+        if constexpr (HELD) {
+#pragma unroll
+            for (int i = 0; i < kHeldKeys; i++)
+                if (tid + T * i < nb)
+                    f(tid + T * i, held[i]);
+        }
+        else
+            for (int b = tid; b < nb; b += T)
+                f(b, block_key(a, score, b, nb));
+    };
+    for (int i = tid; i < 4 * 256; i += T)
+        s_count[i / 256][i % 256] = 0;
     if (tid == 0)
         s_prefix = 0, s_left = a.top;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256)
-            s_count[tid] = 0;
-        __syncthreads();
+    __syncthreads();
+#pragma unroll
+    for (int pass = 0; pass < 4; pass++) {
+        const int      shift = 24 - 8 * pass;
         const unsigned prefix = s_prefix;
-        for (int b = tid; b < nb; b += kSelectThreads) {
-            const unsigned key = block_key(a, score, b, nb);
-            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-                atomicAdd(&s_count[(key >> shift) & 255u], 1);
-        }
+        each([&](int, unsigned key) {
+            if (pass == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
+                atomicAdd(&s_count[pass][(key >> shift) & 255u], 1);
+        });
         __syncthreads();
         if (wave == 0) { // bins from the top: four to a lane
             int c[4], sum = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                c[i] = s_count[255 - (4 * lane + i)], sum += c[i];
+                c[i] = s_count[pass][255 - (4 * lane + i)], sum += c[i];
             int before = sum; // of the lanes before this one
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -304,19 +328,19 @@ __global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const 
     const unsigned edge = s_prefix;
     const int      ties = s_left; // of the blocks with the edge's key, so many are read
     int            placed = 0, level = 0;
-    for (int b0 = 0; b0 < nb; b0 += kSelectThreads) {
-        const int      b = b0 + tid;
-        const unsigned key = b < nb ? block_key(a, score, b, nb) : 0u;
-        const bool     above = b < nb && key > edge, even = b < nb && key == edge;
+    auto           place = [&](int b0, unsigned key, int turn) { // the T blocks from b0 on
+        const int  b = b0 + tid;
+        const bool above = b < nb && key > edge, even = b < nb && key == edge;
         const unsigned long long below = ((unsigned long long)1 << lane) - 1;
         const unsigned long long ma = __ballot(above), me = __ballot(even);
         if (lane == 0)
-            s_wave[0][wave] = __popcll(ma), s_wave[1][wave] = __popcll(me);
+            s_wave[turn][0][wave] = __popcll(ma), s_wave[turn][1][wave] = __popcll(me);
         __syncthreads();
         int pa = 0, pe = 0, ta = 0, te = 0;
-        for (int w = 0; w < kSelectThreads / 64; w++) {
-            pa += w < wave ? s_wave[0][w] : 0, pe += w < wave ? s_wave[1][w] : 0;
-            ta += s_wave[0][w], te += s_wave[1][w];
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            pa += w < wave ? s_wave[turn][0][w] : 0, pe += w < wave ? s_wave[turn][1][w] : 0;
+            ta += s_wave[turn][0][w], te += s_wave[turn][1][w];
         }
         pa += __popcll(ma & below), pe += __popcll(me & below);
         // before this block: pa above it, and of the pe level ones those that are among the first `ties`
@@ -325,8 +349,17 @@ __global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const 
             chosen[placed + pa + taken] = b;
         placed += ta + min(max(ties - level, 0), te);
         level += te;
-        __syncthreads();
+    };
+    // (the counts alternate between two places: one barrier a turn)
+    if constexpr (HELD) {
+#pragma unroll
+        for (int i = 0; i < kHeldKeys; i++)
+            if (T * i < nb)
+                place(T * i, held[i], i & 1);
     }
+    else
+        for (int b0 = 0, turn = 0; b0 < nb; b0 += T, turn ^= 1)
+            place(b0, b0 + tid < nb ? block_key(a, score, b0 + tid, nb) : 0u, turn);
 }
 
 // ---- attention over the chosen blocks -----------------------------------------------------------------------------------
@@ -522,6 +555,12 @@ namespace {
 
 using nvk::SparseArgs;
 
+#ifndef SP_FIT
+#define SP_FIT 2LL
+#endif
+#ifndef SP_LEAST
+#define SP_LEAST 8LL
+#endif
 constexpr int kCus = 256; // MI355X
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -549,12 +588,13 @@ SparseShape sparse_shape(const nvk_block_index *x, int num_seqs, int n_heads, in
     const long long per = lines * s.max_nb / (2LL * kCus * nvk::kSparseWaves);
     s.blocks_per_wave = (int)std::min(64LL, std::max(4LL, per / 4 * 4));
     s.score_slots     = (int)std::max(1LL, ceil_div(s.max_nb, (long long)s.blocks_per_wave * nvk::kSparseWaves));
-    // attention: chunks of the chosen blocks until there are four workgroups for every CU, at least 32 tokens to a wave
+    // attention: the chosen blocks are cut while all workgroups still run at once (two fit a CU), into pieces of eight tokens a
+    // wave at least and 64 blocks at most
     const int       n = std::max(1, std::min(s.max_nb, top));
     const long long tasks = lines * s.head_sets;
-    const long long wanted = ceil_div(4LL * kCus, std::max(tasks, 1LL));
-    const long long least = ceil_div(32LL * nvk::kSparseWaves, x->block_size);
-    s.blocks_per_chunk = (int)std::min(64LL, std::max(least, ceil_div(n, wanted)));
+    const long long fit = std::max(1LL, SP_FIT * kCus / std::max(tasks, 1LL));
+    const long long least = ceil_div(SP_LEAST * nvk::kSparseWaves, x->block_size);
+    s.blocks_per_chunk = (int)std::min(64LL, std::max(least, ceil_div(n, fit)));
     s.blocks_per_chunk = std::max(1, s.blocks_per_chunk);
     s.chunks           = (int)ceil_div(n, s.blocks_per_chunk);
     s.score_floats     = s.max_nb > top ? to_line((size_t)lines * s.max_nb) : 0;
@@ -569,7 +609,12 @@ template <int NV, int HG> void launch_sparse(const SparseArgs &a, const SparseSh
     if (score)
         hipLaunchKernelGGL((nvk::nvk_block_score_kernel<NV, HG>), dim3(lines * (unsigned)s.score_slots), dim3(64 * nvk::kSparseWaves), 0,
                            st, a, s.score_slots);
-    hipLaunchKernelGGL(nvk::nvk_block_select_kernel, dim3(lines), dim3(nvk::kSelectThreads), 0, st, a);
+    if (a.max_nb <= 256 * nvk::kHeldKeys)
+        hipLaunchKernelGGL((nvk::nvk_block_select_kernel<256, true>), dim3(lines), dim3(256), 0, st, a);
+    else if (a.max_nb <= 1024 * nvk::kHeldKeys)
+        hipLaunchKernelGGL((nvk::nvk_block_select_kernel<1024, true>), dim3(lines), dim3(1024), 0, st, a);
+    else
+        hipLaunchKernelGGL((nvk::nvk_block_select_kernel<1024, false>), dim3(lines), dim3(1024), 0, st, a);
     hipLaunchKernelGGL((nvk::nvk_sparse_attn_kernel<NV, HG>), dim3(lines * (unsigned)s.head_sets * (unsigned)s.chunks),
                        dim3(64 * nvk::kSparseWaves), 0, st, a);
 }
