@@ -2,6 +2,8 @@
 //
 // Chunk c of a line, a (row, head), left o_c = sum p v, m_c and l_c = sum p with p = 2^(score - m_c); the result is
 // sum_c w_c o_c / sum_c w_c l_c with w_c = 2^(m_c - max m).  Sums run in a fixed order.
+// Up to kJoinInside chunks it is done by the workgroup that finishes last (no launch of its own: 2-3 us less), beyond that
+// by a kernel whose workgroups spread over the chip.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -62,6 +64,65 @@ __device__ __forceinline__ void join_chunks(const float *__restrict__ o, const f
         const float sum = (s_o[0][c] + s_o[1][c]) + (s_o[2][c] + s_o[3][c]);
         out[c]          = L == 0.f ? sum : sum / L; // (no token: 0, or no number where one was met)
     }
+}
+
+// ---- inside the kernel that made the partial results ------------------------------------------------------------------
+// Partial results are stored write-through (agent scope); every wave waits for its stores, the workgroup meets, one lane counts
+// it in.  Who finds all others counted drops what its CU may hold of their lines and reads them.  Nobody waits for anybody,
+// and the counter is zero again for the next launch.
+constexpr int kJoinInside = 16; // chunks
+
+__device__ __forceinline__ void store_through(float *p, float v)
+{
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Whether this workgroup, whose partial results have just been stored, is the last of `n`.  Called by all its threads.
+__device__ __forceinline__ bool arrived_last(int *counter, int n)
+{
+    __shared__ int s_last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+        if (last)
+            __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = last;
+    }
+    __syncthreads();
+    if (!s_last)
+        return false;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    return true;
+}
+
+// Four channels of a line from its n <= kJoinInside chunks, stored hd (o) and 2 (ml) floats apart.
+__device__ __forceinline__ float4 join_few(const float *o, const float *ml, int n, int hd)
+{
+    float4 y[kJoinInside];
+    float2 w[kJoinInside];
+#pragma unroll
+    for (int c = 0; c < kJoinInside; c++)
+        if (c < n) {
+            w[c] = *reinterpret_cast<const float2 *>(ml + 2 * c);
+            y[c] = *reinterpret_cast<const float4 *>(o + (int64_t)c * hd);
+        }
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int c = 0; c < kJoinInside; c++)
+        if (c < n)
+            M = fmaxf(M, w[c].x);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < kJoinInside; c++)
+        if (c < n) {
+            const float f = w[c].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w[c].x - M);
+            L += w[c].y * f;
+            x.x += y[c].x * f, x.y += y[c].y * f, x.z += y[c].z * f, x.w += y[c].w * f;
+        }
+    if (L != 0.f)
+        x.x /= L, x.y /= L, x.z /= L, x.w /= L;
+    return x;
 }
 
 } // namespace nvk

@@ -44,6 +44,35 @@ inline int grow_workspace(float **ws, size_t *have, long long *generation, size_
     return NVK_OK;
 }
 
+// Counters that every launch finds at zero and leaves at zero, grown like the workspace.
+inline int grow_counters(int **counters, size_t *have, long long *generation, size_t want, hipStream_t stream, const char *who)
+{
+    if (want <= *have)
+        return NVK_OK;
+    want = want < 4096 ? 4096 : want;
+    int *fresh = nullptr;
+    if (stream_is_capturing(stream))
+        return fail(NVK_ERR_INVALID_ARG,
+                    "%s: the workspace would have to grow while the stream is being captured: size it first, outside the "
+                    "capture (the reserve_workspace entry point, or one direct call of the same shape)", who);
+    NVK_HIP_TRY(hipDeviceSynchronize()); // launches on any stream may still use the old ones
+    if (*counters)
+        NVK_HIP_TRY(hipFree(*counters));
+    *counters = nullptr, *have = 0;
+    NVK_HIP_TRY(hipMalloc((void **)&fresh, want * sizeof(int)));
+    // (the fill may still run when hipMemset returns, and a non-blocking stream does not wait for it)
+    hipError_t e = hipMemset(fresh, 0, want * sizeof(int));
+    if (e == hipSuccess)
+        e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        (void)hipFree(fresh);
+        return fail(NVK_ERR_HIP, "%s: clearing the counters failed: %s", who, hipGetErrorString(e));
+    }
+    *counters = fresh, *have = want;
+    ++*generation;
+    return NVK_OK;
+}
+
 // Device copies of a host-pointer call's arrays: one allocation, freed with the scope.
 class Staging
 {

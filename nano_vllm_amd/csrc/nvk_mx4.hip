@@ -39,6 +39,8 @@ struct Mx4AttnArgs
     int          chunks;       // chunks along the longest context
     float        scale_log2e;  // log2(e) / sqrt(head_dim)
     float       *ws_o, *ws_ml; // partial results where chunks > 1: [rows * heads][chunks][head_dim], [..][2]
+    int          whole_lines;  // the decode kernel ran
+    int         *arrivals;     // decode: one for each (sequence, column block, kv-head), or null: the join kernel follows
 };
 
 // The three bf16 numbers whose sum is x, packed for two values at a time.  Truncation: each residual is exact.
@@ -508,7 +510,9 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
     const int begin = chunk * a.chunk_tokens;
     Wave      w;
     w.start(a, row0, rows, ctx, kvh, col0);
-    if (chunk > 0 && begin >= w.most) // nothing of this chunk is seen (the first one writes rows that see nothing)
+    // the chunks that some column sees; the first one writes rows that see nothing
+    const int parts = max(min((w.most + a.chunk_tokens - 1) / a.chunk_tokens, a.chunks), 1);
+    if (chunk >= parts)
         return;
     const int end = min(begin + a.chunk_tokens, w.most);
 
@@ -604,19 +608,29 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
             o += *reinterpret_cast<const f32x4 *>(&s_o[x][c16][c]);
         }
         const int64_t line = (int64_t)(row0 + col / a.group) * a.n_heads + kvh * a.group + col % a.group;
-        float        *dst = a.out + line * a.mx.head_dim + c;
-        if (a.chunks > 1) {
-            dst = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim + c;
-            if (c == 0) {
-                a.ws_ml[(line * a.chunks + chunk) * 2]     = Mc;
-                a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = L;
-            }
-        }
-        else
-            o *= L == 0.f ? 0.f : 1.f / L;
+        if (parts > 1) {
+            float *dst = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim + c, *ml = a.ws_ml + (line * a.chunks + chunk) * 2;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            dst[i] = o[i];
+            for (int i = 0; i < 4; i++)
+                store_through(dst + i, o[i]);
+            if (c == 0)
+                store_through(ml, Mc), store_through(ml + 1, L);
+        }
+        else {
+            o *= L == 0.f ? 0.f : 1.f / L;
+            *reinterpret_cast<f32x4 *>(a.out + line * a.mx.head_dim + c) = o;
+        }
+    }
+    if (parts == 1 || !a.arrivals || !arrived_last(a.arrivals + ((int64_t)seq * a.col_blocks + cb) * a.mx.n_kv_heads + kvh, parts))
+        return;
+    for (int e = threadIdx.x; e < COLS * (HDP / 4); e += 64 * W) {
+        const int col = col0 + e / (HDP / 4), c = (e % (HDP / 4)) * 4;
+        if (col >= columns || c >= a.mx.head_dim)
+            continue;
+        const int64_t line = (int64_t)(row0 + col / a.group) * a.n_heads + kvh * a.group + col % a.group;
+        // (a row of a short context was not seen by the later chunks of a longer one: they hold nothing for it)
+        *reinterpret_cast<float4 *>(a.out + line * a.mx.head_dim + c) =
+            join_few(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, parts, a.mx.head_dim);
     }
 }
 
@@ -780,8 +794,10 @@ __global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_kernel(const Mx4Att
         seq  = lo;
         rows = mx4_rows(a, seq, row0);
     }
-    const int limit = max(mx4_context(a, seq) - rows + (row - row0) + 1, 0);
+    const int ctx = mx4_context(a, seq), limit = max(ctx - rows + (row - row0) + 1, 0);
     const int n = min(max((limit + a.chunk_tokens - 1) / a.chunk_tokens, 1), a.chunks);
+    if (a.whole_lines && min(max((ctx + a.chunk_tokens - 1) / a.chunk_tokens, 1), a.chunks) == 1)
+        return; // (decode writes a sequence of one chunk straight to `out`)
     join_chunks(a.ws_o + line * a.chunks * a.mx.head_dim, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim, a.out + line * a.mx.head_dim);
 }
 
@@ -796,9 +812,9 @@ constexpr int prefill_cols(int kk) { return kk == 8 ? 1 : 2; } // columns of a p
 
 struct Mx4Shape
 {
-    bool   prefill = false, pack = false;
+    bool   prefill = false, pack = false, inside = false; // inside: the decode kernel joins the chunks itself
     int    col_blocks = 1, chunk_tokens = 32, chunks = 1;
-    size_t ws_floats = 0;
+    size_t ws_floats = 0, arrivals = 0;
 };
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -814,15 +830,25 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     const int cols = s.prefill ? 16 * prefill_cols(pool->kk) * kPrefillWaves : 16;
     s.col_blocks = ceil_div((long long)max_rows * group, cols);
     const long long tasks = (long long)num_seqs * pool->n_kv_heads * s.col_blocks;
-    // Cut the context while everything still runs at once (workgroups of four waves: so many fit a CU), into chunks of 256
-    // tokens at least.
+    // Cut the context while everything still runs at once (workgroups of four waves: so many fit a CU), into chunks of 64
+    // tokens at least; not into more than can be joined inside unless those were long.  (One sequence of 777 tokens: 8.05 us
+    // in chunks of 256 tokens, 7.45 of 64; 64 x 2048, two workgroups a CU: 28.1 us uncut, 39.6 in two rounds.)
     const long long fit = (s.pack && pool->kk <= 4 ? 3LL : 2LL) * pool->num_cus;
-    const int       most = std::max(1, max_ctx / 256);
-    s.chunks       = (int)std::max(1LL, std::min(fit / std::max(tasks, 1LL), (long long)most));
+    s.chunks = (int)std::max(1LL, std::min(fit / std::max(tasks, 1LL), (long long)max_ctx / 64));
+    if (!s.prefill && s.chunks > nvk::kJoinInside && max_ctx <= 512 * nvk::kJoinInside)
+        s.chunks = nvk::kJoinInside;
     s.chunk_tokens = std::max(32, ceil_div(ceil_div(max_ctx, s.chunks), 32) * 32);
     s.chunks       = std::max(1, ceil_div(max_ctx, s.chunk_tokens));
+    s.inside       = !s.prefill && s.chunks > 1 && s.chunks <= nvk::kJoinInside;
+    s.arrivals     = s.inside ? (size_t)tasks : 0;
     s.ws_floats    = s.chunks > 1 ? (size_t)total_rows * n_heads * s.chunks * (pool->head_dim + 2) : 0;
     return s;
+}
+
+int reserve(nvk_mx4_pool *pool, const Mx4Shape &s, hipStream_t st, const char *who)
+{
+    const int rc = nvk::grow_workspace(&pool->ws, &pool->ws_floats, &pool->ws_generation, s.ws_floats, st, who);
+    return rc != NVK_OK ? rc : nvk::grow_counters(&pool->arrivals, &pool->arrivals_cap, &pool->ws_generation, s.arrivals, st, who);
 }
 
 template <int KK> void launch_attn(const Mx4AttnArgs &a, const Mx4Shape &s, unsigned blocks, hipStream_t st)
@@ -861,7 +887,7 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
     const long long blocks = (s.prefill ? units : (units + 7) / 8 * 8) * pool->n_kv_heads; // (decode: whole rounds of the XCDs)
     if (blocks > 0x7fffffffLL || (long long)total_rows * n_heads > 0x7fffffffLL)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %lld workgroups", who, blocks);
-    int rc = nvk::grow_workspace(&pool->ws, &pool->ws_floats, &pool->ws_generation, s.ws_floats, st, who);
+    int rc = reserve(pool, s, st, who);
     if (rc != NVK_OK)
         return rc;
     Mx4AttnArgs a{};
@@ -869,6 +895,8 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
     a.num_seqs = num_seqs, a.max_blocks = max_blocks, a.n_heads = n_heads, a.group = n_heads / pool->n_kv_heads;
     a.total_rows = total_rows, a.col_blocks = s.col_blocks, a.chunk_tokens = s.chunk_tokens, a.chunks = s.chunks;
     a.scale_log2e = (float)(1.4426950408889634 / std::sqrt((double)pool->head_dim));
+    a.whole_lines = !s.prefill;
+    a.arrivals    = s.inside ? pool->arrivals : nullptr;
     if (s.chunks > 1) {
         a.ws_o  = pool->ws;
         a.ws_ml = pool->ws + (size_t)total_rows * n_heads * s.chunks * pool->head_dim;
@@ -880,7 +908,7 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
     default: launch_attn<8>(a, s, (unsigned)blocks, st); break;
     }
     NVK_HIP_TRY(hipGetLastError());
-    if (s.chunks > 1) {
+    if (s.chunks > 1 && !s.inside) {
         hipLaunchKernelGGL(nvk::nvk_mx4_join_kernel, dim3((unsigned)(total_rows * n_heads)), dim3(nvk::kJoinThreads), 0, st, a);
         NVK_HIP_TRY(hipGetLastError());
     }
@@ -1006,6 +1034,8 @@ int nvk_mx4_pool_destroy(nvk_mx4_pool *pool)
         (void)hipFree(pool->base);
     if (pool->ws)
         (void)hipFree(pool->ws);
+    if (pool->arrivals)
+        (void)hipFree(pool->arrivals);
     if (pool->stream)
         (void)hipStreamDestroy(pool->stream);
     delete pool;
@@ -1058,7 +1088,7 @@ int nvk_mx4_pool_reserve_workspace(nvk_mx4_pool *pool, int num_seqs, int n_heads
         return rc;
     NVK_SCOPE(pool->device);
     const Mx4Shape s = mx4_shape(pool, num_seqs, n_heads, total_rows, std::max(max_rows, 1), max_ctx);
-    return nvk::grow_workspace(&pool->ws, &pool->ws_floats, &pool->ws_generation, s.ws_floats, pool->stream, who);
+    return reserve(pool, s, pool->stream, who);
 }
 
 int nvk_mx4_decode_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, const float *q_dev,

@@ -102,6 +102,8 @@ struct nvk_mx4_pool
     // partial results of sequences that are cut into chunks (grown on demand, never under stream capture)
     float    *ws            = nullptr;
     size_t    ws_floats     = 0;
+    int      *arrivals      = nullptr; // of the join inside the decode kernel, zero between launches
+    size_t    arrivals_cap  = 0;
     long long ws_generation = 0;
 
     nvk::Mx4Layer layer(int l) const

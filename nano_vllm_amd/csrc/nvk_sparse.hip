@@ -6,8 +6,8 @@
 // best-scored others, and attends to their tokens alone (Attention::paged_attention, include/core/attention.hpp:82-159, over
 // a subset): with block_size 16 it moves 1/16 of the keys for the scores and top / blocks of keys and values.
 //
-// Four kernels: nvk_index_update_kernel behind an append, and for a decode call score, select and attend (and the join of
-// chunks).  gfx950 only; no CPU path.
+// Kernels: nvk_index_update_kernel behind an append, and for a decode call score and attend, with the selection and the join of
+// chunks inside or beside the latter.  gfx950 only; no CPU path.
 
 #include <hip/hip_runtime.h>
 
@@ -26,6 +26,8 @@ struct nvk_block_index
     float    *base = nullptr;   // [layer][block][kv-head][lo | hi][head_dim]
     float    *ws = nullptr;     // scores | chosen blocks | partial results
     size_t    ws_floats = 0;
+    int      *arrivals = nullptr; // of the join inside the attention kernel, zero between launches
+    size_t    arrivals_cap = 0;
     long long ws_generation = 0;
 };
 
@@ -43,13 +45,14 @@ struct SparseArgs
     int          num_seqs, max_blocks, n_heads, group, n_kv_heads, head_dim, num_blocks, block_size;
     int          top, first, last;
     float       *scores; // [num_seqs, n_kv_heads, max_nb]
-    int         *chosen; // [num_seqs, n_kv_heads, top]
+    int         *chosen; // [num_seqs, n_kv_heads, top]; may be null where the attention kernel selects
     int          max_nb; // blocks of the longest context
     int          blocks_per_wave;          // score
     int          blocks_per_chunk, chunks; // attend
     int          head_sets;                // attend: workgroups along the group's heads
     float        scale_log2e;
     float       *ws_o, *ws_ml;
+    int         *arrivals; // one for each (sequence, set of heads, kv-head), or null: the join kernel follows
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -240,10 +243,11 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
 }
 
 // ---- selection --------------------------------------------------------------------------------------------------------
-// One workgroup per (sequence, kv-head): the key of the last block that is read by four counting passes over the bytes of the
-// keys, then the blocks above it, and as many of those level with it as are left, lowest first, in ascending order.
-// T threads; HELD: a thread keeps its (at most kHeldKeys) keys, else it reads the scores again for every pass.
-constexpr int kHeldKeys = 8;
+// The key of the last block that is read is found by four counting passes over the bytes of the keys; read are the blocks above
+// it, and as many of those level with it as are left, lowest first, in ascending order.  Where a workgroup can keep all keys
+// (2048 blocks, eight a thread) every workgroup of the attention kernel selects for itself; beyond that a kernel of its own does.
+constexpr int kHeldKeys  = 8;
+constexpr int kHeldBlocks = 64 * kSparseWaves * kHeldKeys;
 
 __device__ __forceinline__ unsigned block_key(const SparseArgs &a, const float *score, int b, int nb)
 {
@@ -253,84 +257,76 @@ __device__ __forceinline__ unsigned block_key(const SparseArgs &a, const float *
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-template <int T, bool HELD> __global__ void __launch_bounds__(T) nvk_block_select_kernel(const SparseArgs a)
+// sum over the lanes up to and with this one
+__device__ __forceinline__ int scan_wave(int x)
 {
-    constexpr int W = T / 64;
-    __shared__ int      s_count[4][256];
-    __shared__ unsigned s_prefix;
-    __shared__ int      s_left;
-    __shared__ int      s_wave[2][2][W];
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false); // from 1, 2, 4, 8 lanes below in the row
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false); // the last lane of row 0 to row 1, of row 2 to row 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false); // the last lane of the lower half to the upper
+    return x;
+}
+
+// One pass, after the counts of byte (key >> shift) of the keys with this prefix are complete: extends the prefix by the byte
+// in which the `left`-th key from above lies, and takes the keys above it off `left`.  Every wave does it for itself.
+__device__ __forceinline__ void next_byte(const int *count, int shift, unsigned &prefix, int &left)
+{
+    const int  lane = threadIdx.x & 63;
+    const int4 c4 = *reinterpret_cast<const int4 *>(count + 252 - 4 * lane); // bins from the top: four to a lane
+    const int  c[4] = {c4.w, c4.z, c4.y, c4.x};
+    const int  sum = (c[0] + c[1]) + (c[2] + c[3]);
+    int        before = scan_wave(sum) - sum; // of the lanes before this one
+    int        bin = -1, rest = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (before < left && before + c[i] >= left) // exactly one bin of one lane
+            bin = 255 - (4 * lane + i), rest = left - before;
+        before += c[i];
+    }
+    const int from = __ffsll((unsigned long long)__ballot(bin >= 0)) - 1;
+    prefix |= (unsigned)__builtin_amdgcn_readlane(bin, from) << shift;
+    left = __builtin_amdgcn_readlane(rest, from);
+}
+
+constexpr int kSelectThreads = 1024;
+
+__global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const SparseArgs a)
+{
+    constexpr int W = kSelectThreads / 64;
+    __shared__ __attribute__((aligned(16))) int s_count[4][256];
+    __shared__ int s_wave[2][2][W];
     const int    line = blockIdx.x, seq = line / a.n_kv_heads;
     const int    tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int    ctx = context_of(a, seq), nb = (ctx + a.block_size - 1) / a.block_size;
     int         *chosen = a.chosen + (int64_t)line * a.top;
     const float *score = a.scores + (int64_t)line * a.max_nb;
     if (nb <= a.top) {
-        for (int i = tid; i < a.top; i += T)
+        for (int i = tid; i < a.top; i += kSelectThreads)
             chosen[i] = i < nb ? i : -1;
         return;
     }
-    unsigned held[HELD ? kHeldKeys : 1];
-    if constexpr (HELD)
-#pragma unroll
-        for (int i = 0; i < kHeldKeys; i++)
-            held[i] = tid + T * i < nb ? block_key(a, score, tid + T * i, nb) : 0u;
-    // f(block, key) for every block of this thread
-    auto each = [&](auto f) {
-        if constexpr (HELD) {
-#pragma unroll
-            for (int i = 0; i < kHeldKeys; i++)
-                if (tid + T * i < nb)
-                    f(tid + T * i, held[i]);
-        }
-        else
-            for (int b = tid; b < nb; b += T)
-                f(b, block_key(a, score, b, nb));
-    };
-    for (int i = tid; i < 4 * 256; i += T)
-        s_count[i / 256][i % 256] = 0;
-    if (tid == 0)
-        s_prefix = 0, s_left = a.top;
+    s_count[tid >> 8][tid & 255] = 0;
     __syncthreads();
+    unsigned edge = 0;
+    int      ties = a.top; // in the end: of the blocks with the edge's key, so many are read
 #pragma unroll
     for (int pass = 0; pass < 4; pass++) {
-        const int      shift = 24 - 8 * pass;
-        const unsigned prefix = s_prefix;
-        each([&](int, unsigned key) {
-            if (pass == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
+        const int shift = 24 - 8 * pass;
+        for (int b = tid; b < nb; b += kSelectThreads) {
+            const unsigned key = block_key(a, score, b, nb);
+            if (pass == 0 || (key >> (shift + 8)) == (edge >> (shift + 8)))
                 atomicAdd(&s_count[pass][(key >> shift) & 255u], 1);
-        });
-        __syncthreads();
-        if (wave == 0) { // bins from the top: four to a lane
-            int c[4], sum = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                c[i] = s_count[pass][255 - (4 * lane + i)], sum += c[i];
-            int before = sum; // of the lanes before this one
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int x = __shfl_up(before, o);
-                before += lane >= o ? x : 0;
-            }
-            before -= sum;
-            const int left = s_left;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (before < left && before + c[i] >= left) { // exactly one bin of one lane
-                    s_prefix = prefix | ((unsigned)(255 - (4 * lane + i)) << shift);
-                    s_left   = left - before;
-                }
-                before += c[i];
-            }
         }
         __syncthreads();
+        next_byte(s_count[pass], shift, edge, ties);
     }
-    const unsigned edge = s_prefix;
-    const int      ties = s_left; // of the blocks with the edge's key, so many are read
-    int            placed = 0, level = 0;
-    auto           place = [&](int b0, unsigned key, int turn) { // the T blocks from b0 on
-        const int  b = b0 + tid;
-        const bool above = b < nb && key > edge, even = b < nb && key == edge;
+    int placed = 0, level = 0;
+    for (int b0 = 0, turn = 0; b0 < nb; b0 += kSelectThreads, turn ^= 1) { // (the counts alternate between two places)
+        const int      b = b0 + tid;
+        const unsigned key = b < nb ? block_key(a, score, b, nb) : 0u;
+        const bool     above = b < nb && key > edge, even = b < nb && key == edge;
         const unsigned long long below = ((unsigned long long)1 << lane) - 1;
         const unsigned long long ma = __ballot(above), me = __ballot(even);
         if (lane == 0)
@@ -344,29 +340,75 @@ template <int T, bool HELD> __global__ void __launch_bounds__(T) nvk_block_selec
         }
         pa += __popcll(ma & below), pe += __popcll(me & below);
         // before this block: pa above it, and of the pe level ones those that are among the first `ties`
-        const int taken = min(max(ties - level, 0), pe);
         if (above || (even && level + pe < ties))
-            chosen[placed + pa + taken] = b;
+            chosen[placed + pa + min(max(ties - level, 0), pe)] = b;
         placed += ta + min(max(ties - level, 0), te);
         level += te;
-    };
-    // (the counts alternate between two places: one barrier a turn)
-    if constexpr (HELD) {
+    }
+}
+
+// The same by the 256 threads of an attention workgroup, for nb <= kHeldBlocks: picks of the selection, ascending, the ones
+// numbered [begin, begin + count) into `mine`; all of them also to `all` where that is not null.
+__device__ __forceinline__ void select_blocks(const SparseArgs &a, const float *score, int nb, int begin, int count, int *mine, int *all)
+{
+    __shared__ __attribute__((aligned(16))) int s_count[4][256];
+    __shared__ int s_wave[kSparseWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    unsigned  key[kHeldKeys]; // of blocks 8 tid ..
+#pragma unroll
+    for (int i = 0; i < kHeldKeys; i++)
+        key[i] = kHeldKeys * tid + i < nb ? block_key(a, score, kHeldKeys * tid + i, nb) : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        s_count[i][tid] = 0;
+    __syncthreads();
+    unsigned edge = 0;
+    int      ties = a.top;
+#pragma unroll
+    for (int pass = 0; pass < 4; pass++) {
+        const int shift = 24 - 8 * pass;
 #pragma unroll
         for (int i = 0; i < kHeldKeys; i++)
-            if (T * i < nb)
-                place(T * i, held[i], i & 1);
+            if (kHeldKeys * tid + i < nb && (pass == 0 || (key[i] >> (shift + 8)) == (edge >> (shift + 8))))
+                atomicAdd(&s_count[pass][(key[i] >> shift) & 255u], 1);
+        __syncthreads();
+        next_byte(s_count[pass], shift, edge, ties);
     }
-    else
-        for (int b0 = 0, turn = 0; b0 < nb; b0 += T, turn ^= 1)
-            place(b0, b0 + tid < nb ? block_key(a, score, b0 + tid, nb) : 0u, turn);
+    int above = 0, even = 0; // up to 2048 of each: one number holds both
+#pragma unroll
+    for (int i = 0; i < kHeldKeys; i++) {
+        const bool there = kHeldKeys * tid + i < nb;
+        above += there && key[i] > edge, even += there && key[i] == edge;
+    }
+    const int own = above | even << 16, upto = scan_wave(own);
+    if (lane == 63)
+        s_wave[wave] = upto;
+    __syncthreads();
+    int before = upto - own;
+#pragma unroll
+    for (int w = 0; w < kSparseWaves; w++)
+        before += w < wave ? s_wave[w] : 0;
+    int pa = before & 0xffff, pe = before >> 16;
+#pragma unroll
+    for (int i = 0; i < kHeldKeys; i++) {
+        const int  b = kHeldKeys * tid + i;
+        const bool hi = b < nb && key[i] > edge, level = b < nb && key[i] == edge;
+        if (hi || (level && pe < ties)) {
+            const int at = pa + min(pe, ties);
+            if (at >= begin && at < begin + count)
+                mine[at - begin] = b;
+            if (all)
+                all[at] = b;
+        }
+        pa += hi, pe += level;
+    }
 }
 
 // ---- attention over the chosen blocks -----------------------------------------------------------------------------------
 // A wave takes eight tokens a step, eight lanes each: a lane holds NV float4s of the row (lane 8 apart: whole lines per
 // token), dots them with HG query heads, and keeps maximum, sum and output of its own eight-lane group -- nothing
 // crosses the groups before the end.  Bound by the keys and values it reads.
-template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) nvk_sparse_attn_kernel(const SparseArgs a)
+template <int NV, int HG, bool SELECT> __global__ void __launch_bounds__(64 * kSparseWaves) nvk_sparse_attn_kernel(const SparseArgs a)
 {
     constexpr int kMostBlocks = 64; // of a chunk
     __shared__ int   s_phys[kMostBlocks], s_first[kMostBlocks];
@@ -382,11 +424,26 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
     const int hd = a.head_dim, bs = a.block_size;
     const int ctx = context_of(a, seq), nb = (ctx + bs - 1) / bs, n = min(nb, a.top);
     const int begin = chunk * a.blocks_per_chunk, count = min(a.blocks_per_chunk, n - begin);
-    if (chunk > 0 && count <= 0)
+    const int parts = max((n + a.blocks_per_chunk - 1) / a.blocks_per_chunk, 1);
+    if (chunk >= parts)
         return;
-    const int *chosen = a.chosen + ((int64_t)seq * a.n_kv_heads + kvh) * a.top + begin;
+    const int64_t pair = (int64_t)seq * a.n_kv_heads + kvh;
+    int          *chosen = a.chosen ? a.chosen + pair * a.top : nullptr;
+    if constexpr (SELECT) {
+        int *all = chunk == 0 && set == 0 ? chosen : nullptr; // one workgroup tells
+        if (nb > a.top)
+            select_blocks(a, a.scores + pair * a.max_nb, nb, begin, count, s_first, all);
+        else {
+            if ((int)threadIdx.x < count)
+                s_first[threadIdx.x] = begin + threadIdx.x;
+            if (all)
+                for (int i = threadIdx.x; i < a.top; i += 64 * kSparseWaves)
+                    all[i] = i < nb ? i : -1;
+        }
+        __syncthreads();
+    }
     if ((int)threadIdx.x < count) {
-        const int b = min(max(chosen[threadIdx.x], 0), max(nb - 1, 0));
+        const int b = SELECT ? s_first[threadIdx.x] : min(max(chosen[begin + threadIdx.x], 0), max(nb - 1, 0));
         s_first[threadIdx.x] = b * bs;
         s_phys[threadIdx.x]  = min(max(a.tables[(int64_t)seq * a.max_blocks + b], 0), a.num_blocks - 1);
     }
@@ -530,13 +587,23 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
             x += s_o[w][h][c] * f;
         }
         const int64_t line = (int64_t)seq * a.n_heads + head0 + h;
-        if (a.chunks > 1) {
-            a.ws_o[(line * a.chunks + chunk) * hd + c] = x;
-            if (c == 0)
-                a.ws_ml[(line * a.chunks + chunk) * 2] = Mh, a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = L;
+        if (parts > 1) {
+            store_through(a.ws_o + (line * a.chunks + chunk) * hd + c, x);
+            if (c == 0) {
+                store_through(a.ws_ml + (line * a.chunks + chunk) * 2, Mh);
+                store_through(a.ws_ml + (line * a.chunks + chunk) * 2 + 1, L);
+            }
         }
         else
             a.out[line * hd + c] = L == 0.f ? x : x / L; // (x is 0 then, or no number)
+    }
+    if (parts == 1 || !a.arrivals || !arrived_last(a.arrivals + ((int64_t)seq * a.head_sets + set) * a.n_kv_heads + kvh, parts))
+        return;
+    for (int e = threadIdx.x; e < heads * (hd / 4); e += 64 * kSparseWaves) {
+        const int64_t line = (int64_t)seq * a.n_heads + head0 + e / (hd / 4);
+        const int     c = e % (hd / 4) * 4;
+        *reinterpret_cast<float4 *>(a.out + line * hd + c) =
+            join_few(a.ws_o + line * a.chunks * hd + c, a.ws_ml + line * a.chunks * 2, parts, hd);
     }
 }
 
@@ -546,6 +613,8 @@ __global__ void __launch_bounds__(kJoinThreads) nvk_sparse_join_kernel(const Spa
     const int64_t line = blockIdx.x;
     const int     ctx = context_of(a, (int)(line / a.n_heads)), nb = (ctx + a.block_size - 1) / a.block_size;
     const int     n = max((min(nb, a.top) + a.blocks_per_chunk - 1) / a.blocks_per_chunk, 1);
+    if (n == 1)
+        return; // (written straight to `out`)
     join_chunks(a.ws_o + line * a.chunks * a.head_dim, a.ws_ml + line * a.chunks * 2, n, a.head_dim, a.out + line * a.head_dim);
 }
 
@@ -555,12 +624,6 @@ namespace {
 
 using nvk::SparseArgs;
 
-#ifndef SP_FIT
-#define SP_FIT 2LL
-#endif
-#ifndef SP_LEAST
-#define SP_LEAST 8LL
-#endif
 constexpr int kCus = 256; // MI355X
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -568,7 +631,8 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 struct SparseShape
 {
     int    max_nb = 0, blocks_per_wave = 4, score_slots = 1, blocks_per_chunk = 1, chunks = 1, head_sets = 1, hg = 1;
-    size_t score_floats = 0, chosen_ints = 0, part_floats = 0;
+    bool   inside = false, select_inside = false; // the attention kernel joins the chunks itself, selects itself
+    size_t score_floats = 0, chosen_ints = 0, part_floats = 0, arrivals = 0;
     size_t floats() const { return score_floats + chosen_ints + part_floats; }
 };
 
@@ -592,15 +656,27 @@ SparseShape sparse_shape(const nvk_block_index *x, int num_seqs, int n_heads, in
     // wave at least and 64 blocks at most
     const int       n = std::max(1, std::min(s.max_nb, top));
     const long long tasks = lines * s.head_sets;
-    const long long fit = std::max(1LL, SP_FIT * kCus / std::max(tasks, 1LL));
-    const long long least = ceil_div(SP_LEAST * nvk::kSparseWaves, x->block_size);
+    const long long fit = std::max(1LL, 2LL * kCus / std::max(tasks, 1LL));
+    const long long least = ceil_div(8LL * nvk::kSparseWaves, x->block_size);
     s.blocks_per_chunk = (int)std::min(64LL, std::max(least, ceil_div(n, fit)));
+    // (rather sixteen pieces, which the kernel joins itself, than more short ones)
+    if (ceil_div(n, s.blocks_per_chunk) > nvk::kJoinInside && ceil_div(n, nvk::kJoinInside) * x->block_size <= 256)
+        s.blocks_per_chunk = (int)std::min(64LL, ceil_div(n, nvk::kJoinInside));
     s.blocks_per_chunk = std::max(1, s.blocks_per_chunk);
     s.chunks           = (int)ceil_div(n, s.blocks_per_chunk);
     s.score_floats     = s.max_nb > top ? to_line((size_t)lines * s.max_nb) : 0;
-    s.chosen_ints      = to_line((size_t)lines * top);
+    s.select_inside    = s.max_nb <= nvk::kHeldBlocks;
+    s.chosen_ints      = s.select_inside ? 0 : to_line((size_t)lines * top);
+    s.inside           = s.chunks > 1 && s.chunks <= nvk::kJoinInside;
+    s.arrivals         = s.inside ? (size_t)tasks : 0;
     s.part_floats      = s.chunks > 1 ? (size_t)num_seqs * n_heads * s.chunks * (x->head_dim + 2) : 0;
     return s;
+}
+
+int reserve(nvk_block_index *x, const SparseShape &s, hipStream_t st, const char *who)
+{
+    const int rc = nvk::grow_workspace(&x->ws, &x->ws_floats, &x->ws_generation, s.floats(), st, who);
+    return rc != NVK_OK ? rc : nvk::grow_counters(&x->arrivals, &x->arrivals_cap, &x->ws_generation, s.arrivals, st, who);
 }
 
 template <int NV, int HG> void launch_sparse(const SparseArgs &a, const SparseShape &s, bool score, hipStream_t st)
@@ -609,14 +685,13 @@ template <int NV, int HG> void launch_sparse(const SparseArgs &a, const SparseSh
     if (score)
         hipLaunchKernelGGL((nvk::nvk_block_score_kernel<NV, HG>), dim3(lines * (unsigned)s.score_slots), dim3(64 * nvk::kSparseWaves), 0,
                            st, a, s.score_slots);
-    if (a.max_nb <= 256 * nvk::kHeldKeys)
-        hipLaunchKernelGGL((nvk::nvk_block_select_kernel<256, true>), dim3(lines), dim3(256), 0, st, a);
-    else if (a.max_nb <= 1024 * nvk::kHeldKeys)
-        hipLaunchKernelGGL((nvk::nvk_block_select_kernel<1024, true>), dim3(lines), dim3(1024), 0, st, a);
-    else
-        hipLaunchKernelGGL((nvk::nvk_block_select_kernel<1024, false>), dim3(lines), dim3(1024), 0, st, a);
-    hipLaunchKernelGGL((nvk::nvk_sparse_attn_kernel<NV, HG>), dim3(lines * (unsigned)s.head_sets * (unsigned)s.chunks),
-                       dim3(64 * nvk::kSparseWaves), 0, st, a);
+    const dim3 grid(lines * (unsigned)s.head_sets * (unsigned)s.chunks), block(64 * nvk::kSparseWaves);
+    if (s.select_inside)
+        hipLaunchKernelGGL((nvk::nvk_sparse_attn_kernel<NV, HG, true>), grid, block, 0, st, a);
+    else {
+        hipLaunchKernelGGL(nvk::nvk_block_select_kernel, dim3(lines), dim3(nvk::kSelectThreads), 0, st, a);
+        hipLaunchKernelGGL((nvk::nvk_sparse_attn_kernel<NV, HG, false>), grid, block, 0, st, a);
+    }
 }
 
 template <int NV> void launch_heads(const SparseArgs &a, const SparseShape &s, bool score, hipStream_t st)
@@ -706,7 +781,7 @@ int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, con
     const long long   lines = (long long)num_seqs * x->n_kv_heads;
     if (lines * s.score_slots > 0x7fffffffLL || (long long)num_seqs * n_heads > 0x7fffffffLL || lines * s.head_sets * s.chunks > 0x7fffffffLL)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: too many workgroups", who);
-    int rc = nvk::grow_workspace(&x->ws, &x->ws_floats, &x->ws_generation, s.floats(), st, who);
+    int rc = reserve(x, s, st, who);
     if (rc != NVK_OK)
         return rc;
     SparseArgs a{};
@@ -718,9 +793,10 @@ int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, con
     a.max_nb = s.max_nb, a.blocks_per_wave = s.blocks_per_wave, a.blocks_per_chunk = s.blocks_per_chunk, a.chunks = s.chunks;
     a.head_sets = s.head_sets, a.scale_log2e = (float)(1.4426950408889634 / std::sqrt((double)x->head_dim));
     a.scores = x->ws;
-    a.chosen = selected ? selected : (int *)(x->ws + s.score_floats);
+    a.chosen = selected || s.select_inside ? selected : (int *)(x->ws + s.score_floats);
     a.ws_o   = x->ws + s.score_floats + s.chosen_ints;
     a.ws_ml  = a.ws_o + (size_t)num_seqs * n_heads * s.chunks * x->head_dim;
+    a.arrivals = s.inside ? x->arrivals : nullptr;
     const bool score = s.max_nb > top;
     const int  nv = x->head_dim <= 32 ? 1 : x->head_dim <= 64 ? 2 : x->head_dim <= 128 ? 4 : 8;
     switch (nv) {
@@ -730,7 +806,7 @@ int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, con
     default: launch_heads<8>(a, s, score, st); break;
     }
     NVK_HIP_TRY(hipGetLastError());
-    if (s.chunks > 1) {
+    if (s.chunks > 1 && !s.inside) {
         hipLaunchKernelGGL(nvk::nvk_sparse_join_kernel, dim3((unsigned)(num_seqs * n_heads)), dim3(nvk::kJoinThreads), 0, st, a);
         NVK_HIP_TRY(hipGetLastError());
     }
@@ -784,6 +860,8 @@ int nvk_block_index_destroy(nvk_block_index *index)
         (void)hipFree(index->base);
     if (index->ws)
         (void)hipFree(index->ws);
+    if (index->arrivals)
+        (void)hipFree(index->arrivals);
     delete index;
     return NVK_OK;
 }
@@ -812,8 +890,7 @@ int nvk_block_index_reserve_workspace(nvk_block_index *index, int num_seqs, int 
     const int   rs = pool_stream(index, nullptr, &st);
     if (rs != NVK_OK)
         return rs;
-    return nvk::grow_workspace(&index->ws, &index->ws_floats, &index->ws_generation,
-                               sparse_shape(index, num_seqs, n_heads, max_ctx, top_blocks).floats(), st, who);
+    return reserve(index, sparse_shape(index, num_seqs, n_heads, max_ctx, top_blocks), st, who);
 }
 
 int nvk_block_index_update(nvk_block_index *index, int layer, int num_seqs, const int *block_tables, int max_blocks,
