@@ -81,13 +81,17 @@ __device__ __forceinline__ int mx4_scale_byte(double amax)
 }
 
 // Nearest code, ties to the even code; x already divided by the group's scale (a power of two: exact).
-// Counting thresholds that lie below x does the rounding: a tie counts exactly where the upper code is the even one.
+// Counting thresholds that lie below |x| does the rounding: a tie counts exactly where the upper code is the even one.  All
+// thresholds have an empty lower half, so the comparison is made on the upper half and whether anything is left below it.
 __device__ __forceinline__ unsigned mx4_code(double x)
 {
-    const double a = fabs(x);
-    const unsigned mag = (unsigned)(a > 0.25) + (unsigned)(a >= 0.75) + (unsigned)(a > 1.25) + (unsigned)(a >= 1.75)
-                         + (unsigned)(a > 2.5) + (unsigned)(a >= 3.5) + (unsigned)(a > 5.0);
-    return mag | (x < 0.0 ? 8u : 0u);
+    const unsigned long long bits = (unsigned long long)__double_as_longlong(x);
+    const unsigned a = (unsigned)(bits >> 32) << 1 | ((unsigned)bits != 0u); // (the sign is shifted out)
+    constexpr unsigned q1 = 2u * 0x3fd00000u, q3 = 2u * 0x3fe80000u, q5 = 2u * 0x3ff40000u, q7 = 2u * 0x3ffc0000u, // .25 .75 1.25 1.75
+        h5 = 2u * 0x40040000u, h7 = 2u * 0x400c0000u, five = 2u * 0x40140000u;                                      // 2.5 3.5 5
+    const unsigned mag = (unsigned)(a > q1) + (unsigned)(a >= q3) + (unsigned)(a > q5) + (unsigned)(a >= q7) + (unsigned)(a > h5)
+                         + (unsigned)(a >= h7) + (unsigned)(a > five);
+    return mag | (unsigned)(bits >> 60 & 8u);
 }
 
 } // namespace nvk

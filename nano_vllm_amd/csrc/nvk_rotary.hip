@@ -29,7 +29,7 @@ struct nvk_rope
 {
     int                 head_dim = 0, rotary_dim = 0, layout = 0, device = 0;
     double              factor   = 1.0; // m, on cos and sin
-    double             *freq_dev = nullptr;
+    double             *freq_dev = nullptr; // half turns per position: no reduction by pi on the device
     std::vector<double> freq;
 };
 
@@ -45,7 +45,7 @@ struct RotaryArgs
     float        *q_out;
     const float  *q_weight, *k_weight; // [head_dim] or null
     double        eps;
-    const double *freq; // [rotary_dim / 2] or null
+    const double *freq; // [rotary_dim / 2], in half turns per position; or null
     double        factor;
     int           rotary_dim, half_layout;
     const int    *row_seqs, *positions, *tables;
@@ -64,109 +64,166 @@ __device__ __forceinline__ void pair_channels(const RotaryArgs &a, int p, int &i
         ia = 2 * p, ib = 2 * p + 1;
 }
 
-// One workgroup takes row blockIdx.x; its waves (and those of gridDim.y workgroups) share the row's heads in batches of
-// kRotaryBatch values.  W lanes hold one head row, PPL pairs each; U head rows are in flight in a lane.
-// For the 4-bit cache the batch then crosses LDS, after which a lane holds eight neighbouring channels: one dword of codes.
+// Exchanges of doubles on the vector pipe: lane ^ 1, lane ^ 2, turns by 4 and 8 inside sixteen lanes, a quad's lane to all four.
+template <int C> __device__ __forceinline__ double across(double x)
+{
+    const long long b = __double_as_longlong(x);
+    const int       lo = __builtin_amdgcn_update_dpp(0, (int)b, C, 0xF, 0xF, true);
+    const int       hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), C, 0xF, 0xF, true);
+    return __longlong_as_double((long long)hi << 32 | (unsigned)lo);
+}
+// x of this lane and of lane ^ 16 (ROW) or lane ^ 32, added
+template <bool ROW> __device__ __forceinline__ double fold(double x)
+{
+    const unsigned long long b = (unsigned long long)__double_as_longlong(x);
+    const unsigned           lo = (unsigned)b, hi = (unsigned)(b >> 32);
+    const auto l = ROW ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto h = ROW ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    return __longlong_as_double((long long)((unsigned long long)h[0] << 32 | l[0]))
+           + __longlong_as_double((long long)((unsigned long long)h[1] << 32 | l[1]));
+}
+template <int W> __device__ __forceinline__ double sum_over(double x) // over W = 16, 32 or 64 neighbouring lanes
+{
+    x += across<0xB1>(x);
+    x += across<0x4E>(x);
+    x += across<0x124>(x);
+    x += across<0x128>(x);
+    if constexpr (W >= 32)
+        x = fold<true>(x);
+    if constexpr (W >= 64)
+        x = fold<false>(x);
+    return x;
+}
+
+// A wave takes a row, or one of `parts` shares of its heads where rows are few (each share computes the row's angles again, side
+// by side); its heads come in batches of kRotaryBatch values, the next one on its way while one is worked on.  W lanes hold
+// one head row, PPL pairs each, so that a lane's angles stay in its registers; U head rows are in flight in a lane.
+// For the 4-bit cache a batch of keys or values then crosses LDS, after which a lane holds eight neighbouring channels: one
+// dword of codes.
 template <int W, int PPL, bool MX4>
-__global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel(const RotaryArgs a)
+__global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel(const RotaryArgs a, int rows, int parts)
 {
     constexpr int U = PPL == 2 ? 2 : 4; // head rows per lane at a time
     constexpr int R = 64 / W;           // head rows side by side in a wave
     constexpr int HB = U * R;           // head rows per batch
-    __shared__ double2 s_cs[kRotaryMaxHead / 2];
-    __shared__ double  s_row[MX4 ? kRotaryWaves : 1][MX4 ? kRotaryBatch : 1];
+    __shared__ double s_row[MX4 ? kRotaryWaves : 1][MX4 ? kRotaryBatch : 1];
 
-    const int row = blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = blockIdx.x * kRotaryWaves + wave; // (rows * parts fits: checked on the host)
+    const int row = id / parts, part = id - row * parts;
+    if (row >= rows)
+        return;
     const int pos = a.positions[row];
     const int seq = a.row_seqs ? a.row_seqs[row] : row;
     const int bs = a.mx.block_size;
-    // rows of padding, and rows that have no place in their table, are left alone (uniform over the workgroup)
+    // rows of padding, and rows that have no place in their table, are left alone
     if (pos < 0 || (a.k && (seq < 0 || seq >= a.num_seqs || pos / bs >= a.max_blocks)))
         return;
     const int  hd = a.mx.head_dim, pairs = hd >> 1, kv = a.mx.n_kv_heads;
-    const int  turned = a.freq ? a.rotary_dim >> 1 : 0;
-    if (turned) {
-        for (int p = threadIdx.x; p < turned; p += blockDim.x) {
-            double s, c;
-            sincos((double)pos * a.freq[p], &s, &c);
-            s_cs[p] = make_double2(a.factor * c, a.factor * s);
-        }
-        __syncthreads();
-    }
     const int  block = a.k ? a.tables[(int64_t)seq * a.max_blocks + pos / bs] : 0;
     const int  offset = pos % bs;
     const bool keep = a.k && block >= 0 && block < a.mx.num_blocks;
+    const int  lane = threadIdx.x & 63;
+    const int  sub = lane / W, lw = lane % W; // which of the wave's head rows, and the lane's place in it
+    int        ia[PPL], ib[PPL];
+#pragma unroll
+    for (int j = 0; j < PPL; j++)
+        pair_channels(a, lw + j * W, ia[j], ib[j]);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int sub = lane / W, lw = lane % W; // which of the wave's head rows, and the lane's place in it
+    // batches: keys, values, queries; this wave's are part, part + parts, ..
     const int kb = a.k ? (kv + HB - 1) / HB : 0, qb = a.q ? (a.n_heads + HB - 1) / HB : 0;
-    const int batches = 2 * kb + qb; // keys, values, queries
-
-    for (int t = blockIdx.y * kRotaryWaves + wave; t < batches; t += gridDim.y * kRotaryWaves) {
-        const int    kind = t < kb ? 0 : t < 2 * kb ? 1 : 2; // key, value, query
-        const int    head0 = (t - (kind == 0 ? 0 : kind == 1 ? kb : 2 * kb)) * HB;
-        const int    heads = kind == 2 ? a.n_heads : kv;
+    const int batches = 2 * kb + qb;
+    auto      kind_of = [&](int t) { return t < kb ? 0 : t < 2 * kb ? 1 : 2; }; // key, value, query
+    auto      fetch = [&](int t, float2 (&x)[U][PPL]) {
+        const int    kind = kind_of(t);
+        const int    head0 = (t - kind * kb) * HB, heads = kind == 2 ? a.n_heads : kv;
         const float *src = (kind == 0 ? a.k : kind == 1 ? a.v : a.q) + (int64_t)row * heads * hd;
-        const float *weight = kind == 0 ? a.k_weight : kind == 1 ? nullptr : a.q_weight;
-        const int    turn = kind == 1 ? 0 : turned;
-        if (kind < 2 && !keep)
-            continue;
-
-        float2 x[U][PPL];
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
             for (int j = 0; j < PPL; j++) {
-                const int head = head0 + u * R + sub, p = lw + j * W;
-                int       ia, ib;
-                pair_channels(a, p, ia, ib);
+                const int head = head0 + u * R + sub;
                 x[u][j] = make_float2(0.f, 0.f);
-                if (head < heads && p < pairs)
-                    x[u][j] = make_float2(src[head * hd + ia], src[head * hd + ib]);
+                if (head < heads && lw + j * W < pairs)
+                    x[u][j] = make_float2(src[head * hd + ia[j]], src[head * hd + ib[j]]);
             }
+    };
+    float2 next[U][PPL];
+    int    t = part;
+    if (t < batches)
+        fetch(t, next);
+
+    const int turned = a.freq ? a.rotary_dim >> 1 : 0;
+    double    cs[PPL], sn[PPL];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int head = head0 + u * R + sub;
-            double    scale = 1.0;
-            if (weight) {
-                double ss = 0.0;
+    for (int j = 0; j < PPL; j++) {
+        cs[j] = 1.0, sn[j] = 0.0;
+        if (lw + j * W < turned) {
+            sincospi((double)pos * a.freq[lw + j * W], &sn[j], &cs[j]);
+            cs[j] *= a.factor, sn[j] *= a.factor;
+        }
+    }
+
+    for (; t < batches; t += parts) {
+        const int    kind = kind_of(t);
+        const int    head0 = (t - kind * kb) * HB, heads = kind == 2 ? a.n_heads : kv;
+        const float *weight = kind == 0 ? a.k_weight : kind == 1 ? nullptr : a.q_weight;
+        float2       x[U][PPL];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < PPL; j++)
+                x[u][j] = next[u][j];
+        if (t + parts < batches)
+            fetch(t + parts, next);
+        if (kind < 2 && !keep)
+            continue;
+
+        double scale = 1.0; // of head row u: in lane u of every quad
+        if (weight) {
+            double ss[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                ss[u] = 0.0;
 #pragma unroll
                 for (int j = 0; j < PPL; j++)
-                    ss = fma((double)x[u][j].x, (double)x[u][j].x, fma((double)x[u][j].y, (double)x[u][j].y, ss));
-#pragma unroll
-                for (int o = W / 2; o > 0; o >>= 1)
-                    ss += __shfl_xor(ss, o);
-                scale = 1.0 / sqrt(ss / hd + a.eps);
+                    ss[u] = fma((double)x[u][j].x, (double)x[u][j].x, fma((double)x[u][j].y, (double)x[u][j].y, ss[u]));
+                ss[u] = sum_over<W>(ss[u]);
             }
+            double mine = ss[0];
+#pragma unroll
+            for (int u = 1; u < U; u++)
+                mine = (lane & 3) == u ? ss[u] : mine;
+            scale = rsqrt(mine / hd + a.eps);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int    head = head0 + u * R + sub;
+            const double by = u == 0 ? across<0x00>(scale) : u == 1 ? across<0x55>(scale) : u == 2 ? across<0xAA>(scale) : across<0xFF>(scale);
 #pragma unroll
             for (int j = 0; j < PPL; j++) {
-                const int p = lw + j * W;
-                int       ia, ib;
-                pair_channels(a, p, ia, ib);
-                const bool there = head < heads && p < pairs;
+                const bool there = head < heads && lw + j * W < pairs;
                 double     ya = x[u][j].x, yb = x[u][j].y;
                 if (weight && there)
-                    ya = ya * scale * (double)weight[ia], yb = yb * scale * (double)weight[ib];
-                if (p < turn) {
-                    const double2 cs = s_cs[p];
-                    const double  na = ya * cs.x - yb * cs.y;
-                    yb               = ya * cs.y + yb * cs.x;
-                    ya               = na;
+                    ya = ya * by * (double)weight[ia[j]], yb = yb * by * (double)weight[ib[j]];
+                if (kind != 1) {
+                    const double na = ya * cs[j] - yb * sn[j];
+                    yb              = ya * sn[j] + yb * cs[j];
+                    ya              = na;
                 }
                 if (!there)
                     continue;
                 if (MX4 && kind < 2) {
-                    s_row[wave][(u * R + sub) * hd + ia] = ya;
-                    s_row[wave][(u * R + sub) * hd + ib] = yb;
+                    s_row[wave][(u * R + sub) * hd + ia[j]] = ya;
+                    s_row[wave][(u * R + sub) * hd + ib[j]] = yb;
                 }
                 else {
                     float *dst;
                     if (kind == 2)
                         dst = a.q_out + ((int64_t)row * heads + head) * hd;
                     else
-                        dst = (kind == 0 ? a.k_slab : a.v_slab)
-                              + row_float_index(block, offset, head, bs, kv, hd);
-                    dst[ia] = (float)ya, dst[ib] = (float)yb;
+                        dst = (kind == 0 ? a.k_slab : a.v_slab) + row_float_index(block, offset, head, bs, kv, hd);
+                    dst[ia[j]] = (float)ya, dst[ib[j]] = (float)yb;
                 }
             }
         }
@@ -228,35 +285,42 @@ __global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel
 
 // ---- the values of cached rows: one thread per 8 channels of (row, kv-head) -----------------------------------------
 __global__ void __launch_bounds__(256)
-    nvk_mx4_read_rows_kernel(const Mx4Layer mx, const int *__restrict__ row_seqs, const int *__restrict__ positions,
+    nvk_mx4_read_rows_kernel(const Mx4Layer mx, int rows, const int *__restrict__ row_seqs, const int *__restrict__ positions,
                              const int *__restrict__ tables, int num_seqs, int max_blocks, float *__restrict__ k_out,
                              float *__restrict__ v_out)
 {
-    const int row = blockIdx.x;
-    const int pos = positions[row], seq = row_seqs ? row_seqs[row] : row, bs = mx.block_size;
+    const unsigned octets = mx.head_dim >> 3, per_row = mx.n_kv_heads * octets;
+    const int64_t  id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t  row = id / per_row;
+    if (row >= rows)
+        return;
+    const unsigned i = (unsigned)(id - row * per_row);
+    const int      pos = positions[row], seq = row_seqs ? row_seqs[row] : (int)row, bs = mx.block_size;
     if (pos < 0 || seq < 0 || seq >= num_seqs || pos / bs >= max_blocks)
         return;
     const int block = tables[(int64_t)seq * max_blocks + pos / bs], offset = pos % bs, tok = offset % kMx4Tile;
     if (block < 0 || block >= mx.num_blocks)
         return;
-    const int octets = mx.head_dim >> 3, kk = mx.kk;
-    for (int i = threadIdx.x; i < mx.n_kv_heads * octets; i += blockDim.x) {
-        const int            head = i / octets, c0 = (i % octets) * 8;
-        const unsigned char *tile = mx.tile(block, offset, head);
-        unsigned             kw = *reinterpret_cast<const unsigned *>(tile + tok * 16 * kk + c0 / 2), vw = 0;
-        if (kk >= 4)
-            vw = *reinterpret_cast<const unsigned *>(tile + mx4_v_at(kk) + mx4_v_byte(tok, c0, kk));
-        else
+    const int            head = i / octets, c0 = (i % octets) * 8, kk = mx.kk;
+    const unsigned char *tile = mx.tile(block, offset, head);
+    unsigned             kw = *reinterpret_cast<const unsigned *>(tile + tok * 16 * kk + c0 / 2), vw = 0;
+    if (kk >= 4)
+        vw = *reinterpret_cast<const unsigned *>(tile + mx4_v_at(kk) + mx4_v_byte(tok, c0, kk));
+    else
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                vw |= (unsigned)tile[mx4_v_at(kk) + mx4_v_byte(tok, c0 + 2 * j, kk)] << (8 * j);
-        const unsigned ks = tile[mx4_ks_at(kk) + (c0 / 32) * kMx4Tile + tok], vs = tile[mx4_vs_at(kk) + (c0 / 32) * kMx4Tile + tok];
-        const int64_t  at = ((int64_t)row * mx.n_kv_heads + head) * mx.head_dim + c0;
+        for (int j = 0; j < 4; j++)
+            vw |= (unsigned)tile[mx4_v_at(kk) + mx4_v_byte(tok, c0 + 2 * j, kk)] << (8 * j);
+    const unsigned ks = tile[mx4_ks_at(kk) + (c0 / 32) * kMx4Tile + tok], vs = tile[mx4_vs_at(kk) + (c0 / 32) * kMx4Tile + tok];
+    const int64_t  at = (row * mx.n_kv_heads + head) * mx.head_dim + c0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            k_out[at + j] = mx4_value((kw >> (4 * j)) & 15u, ks);
-            v_out[at + j] = mx4_value((vw >> (4 * j)) & 15u, vs);
-        }
+    for (int h = 0; h < 2; h++) {
+        float4 k, v;
+        k.x = mx4_value((kw >> (16 * h)) & 15u, ks), k.y = mx4_value((kw >> (16 * h + 4)) & 15u, ks);
+        k.z = mx4_value((kw >> (16 * h + 8)) & 15u, ks), k.w = mx4_value((kw >> (16 * h + 12)) & 15u, ks);
+        v.x = mx4_value((vw >> (16 * h)) & 15u, vs), v.y = mx4_value((vw >> (16 * h + 4)) & 15u, vs);
+        v.z = mx4_value((vw >> (16 * h + 8)) & 15u, vs), v.w = mx4_value((vw >> (16 * h + 12)) & 15u, vs);
+        *reinterpret_cast<float4 *>(k_out + at + 4 * h) = k;
+        *reinterpret_cast<float4 *>(v_out + at + 4 * h) = v;
     }
 }
 
@@ -274,19 +338,18 @@ template <bool MX4> void launch_rotary(const RotaryArgs &a, int rows, hipStream_
     const int w = pairs <= 16 ? 16 : pairs <= 32 ? 32 : 64;
     const int hb = pairs > 64 ? 2 : 4 * (64 / w);
     const int batches = (a.k ? 2 * ((a.mx.n_kv_heads + hb - 1) / hb) : 0) + (a.q ? (a.n_heads + hb - 1) / hb : 0);
-    // Few rows: a row's batches are spread over several workgroups (each computes the row's angles again, side by side), up
-    // to one batch per wave, until the launch has two workgroups for every CU.
-    const int most = (batches + nvk::kRotaryWaves - 1) / nvk::kRotaryWaves;
-    const int parts = std::max(1, std::min(most, (2 * kCus + rows - 1) / rows));
-    const dim3 grid((unsigned)rows, (unsigned)parts), block(64 * nvk::kRotaryWaves);
+    // Few rows: a row's batches are spread over several waves, one each at most, while there are
+    // no more than sixteen waves for every CU.
+    const int  parts = (int)std::max(1LL, std::min((long long)batches, 16LL * kCus / rows));
+    const dim3 grid((unsigned)(((long long)rows * parts + nvk::kRotaryWaves - 1) / nvk::kRotaryWaves)), block(64 * nvk::kRotaryWaves);
     if (pairs > 64)
-        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<64, 2, MX4>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<64, 2, MX4>), grid, block, 0, st, a, rows, parts);
     else if (w == 64)
-        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<64, 1, MX4>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<64, 1, MX4>), grid, block, 0, st, a, rows, parts);
     else if (w == 32)
-        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<32, 1, MX4>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<32, 1, MX4>), grid, block, 0, st, a, rows, parts);
     else
-        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<16, 1, MX4>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<16, 1, MX4>), grid, block, 0, st, a, rows, parts);
 }
 
 // Host-pointer calls: every row has a place of its own.  (Two rows in one slot: whichever comes last would stay, or a mix.)
@@ -444,12 +507,15 @@ int nvk_rope_create(int head_dim, int rotary_dim, int layout, double theta, int 
         delete r;
         return nvk::fail(NVK_ERR_OOM, "nvk_rope_create: host allocation failed");
     }
+    double half_turns[nvk::kRotaryMaxHead / 2];
+    for (size_t i = 0; i < r->freq.size(); i++)
+        half_turns[i] = r->freq[i] / M_PI;
     nvk::DeviceScope scope(device);
     hipError_t       e = scope.ok ? hipSuccess : hipErrorInvalidDevice;
     if (e == hipSuccess)
         e = hipMalloc((void **)&r->freq_dev, r->freq.size() * sizeof(double));
     if (e == hipSuccess)
-        e = hipMemcpy(r->freq_dev, r->freq.data(), r->freq.size() * sizeof(double), hipMemcpyHostToDevice);
+        e = hipMemcpy(r->freq_dev, half_turns, r->freq.size() * sizeof(double), hipMemcpyHostToDevice);
     if (e != hipSuccess) {
         const int rc = nvk::fail(e == hipErrorOutOfMemory ? NVK_ERR_OOM : NVK_ERR_HIP, "nvk_rope_create: %s", hipGetErrorString(e));
         if (r->freq_dev)
@@ -539,9 +605,12 @@ int nvk_mx4_pool_read_rows(nvk_mx4_pool *pool, int layer, int rows, const int *r
         return NVK_OK;
     NVK_SCOPE(pool->device);
     hipStream_t st = (ptr_kind == NVK_PTR_DEVICE && stream) ? (hipStream_t)stream : pool->stream;
-    const dim3  grid((unsigned)rows), block(256);
+    const long long threads = (long long)rows * pool->n_kv_heads * (pool->head_dim / 8);
+    if (threads > 0x7fffffffLL * 256)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %d rows", who, rows);
+    const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
     if (ptr_kind == NVK_PTR_DEVICE) {
-        hipLaunchKernelGGL(nvk::nvk_mx4_read_rows_kernel, grid, block, 0, st, pool->layer(layer), row_seqs, positions,
+        hipLaunchKernelGGL(nvk::nvk_mx4_read_rows_kernel, grid, block, 0, st, pool->layer(layer), rows, row_seqs, positions,
                            block_tables, num_seqs, max_blocks, k_out, v_out);
         NVK_HIP_TRY(hipGetLastError());
         return NVK_OK;
@@ -555,7 +624,7 @@ int nvk_mx4_pool_read_rows(nvk_mx4_pool *pool, int layer, int rows, const int *r
     const int    ik = s.add(k_out, kb), iv = s.add(v_out, kb), ip = s.add(positions, rb), is = s.add(row_seqs, row_seqs ? rb : 0),
               it = s.add(block_tables, (size_t)num_seqs * max_blocks * sizeof(int));
     NVK_HIP_TRY(s.upload(st));
-    hipLaunchKernelGGL(nvk::nvk_mx4_read_rows_kernel, grid, block, 0, st, pool->layer(layer),
+    hipLaunchKernelGGL(nvk::nvk_mx4_read_rows_kernel, grid, block, 0, st, pool->layer(layer), rows,
                        row_seqs ? s.at<int>(is) : (const int *)nullptr, s.at<int>(ip), s.at<int>(it), num_seqs, max_blocks,
                        s.at<float>(ik), s.at<float>(iv));
     NVK_HIP_TRY(hipGetLastError());
