@@ -42,6 +42,17 @@ def _devptr(x) -> C.c_void_p:
     return C.c_void_p(int(x))
 
 
+def _address(x):
+    """What :func:`_devptr` gives, as the int that ctypes takes for a pointer (half the time: the calls of small steps are
+    bound by it)."""
+    if x is None or type(x) is int:
+        return x
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return x if isinstance(x, C.c_void_p) else int(x)
+
+
 class PagedKVPool:
     def __init__(self, n_layers: int, num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int,
                  device: int = 0):

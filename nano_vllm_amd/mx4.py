@@ -11,7 +11,7 @@ from typing import Optional, Tuple
 import numpy as np
 
 from . import _capi
-from .kv_pool import _devptr, _f32, _i32, _ptr
+from .kv_pool import _address, _f32, _i32, _ptr
 
 
 class Mx4KVPool:
@@ -24,7 +24,7 @@ class Mx4KVPool:
         self.n_kv_heads, self.head_dim, self.device = int(n_kv_heads), int(head_dim), int(device)
 
     def close(self) -> None:
-        if getattr(self, "_h", None):
+        if getattr(self, "_h", None) and _capi.lib is not None:  # (None: the interpreter is going down)
             _capi.lib.nvk_mx4_pool_destroy(self._h)
             self._h = None
 
@@ -87,9 +87,9 @@ class Mx4KVPool:
 
     def read_rows_device(self, layer: int, rows: int, row_seqs_dev, positions_dev, block_tables_dev, num_seqs: int, max_blocks: int,
                          k_out_dev, v_out_dev, stream=None) -> None:
-        _capi.check(_capi.lib.nvk_mx4_pool_read_rows(self.handle, int(layer), int(rows), _devptr(row_seqs_dev), _devptr(positions_dev),
-                                                     _devptr(block_tables_dev), int(num_seqs), int(max_blocks), _devptr(k_out_dev),
-                                                     _devptr(v_out_dev), _capi.PTR_DEVICE, _devptr(stream)))
+        _capi.check(_capi.lib.nvk_mx4_pool_read_rows(self.handle, int(layer), int(rows), _address(row_seqs_dev), _address(positions_dev),
+                                                     _address(block_tables_dev), int(num_seqs), int(max_blocks), _address(k_out_dev),
+                                                     _address(v_out_dev), _capi.PTR_DEVICE, _address(stream)))
 
 
 def _lens(pool, block_tables, ctx_lens):
@@ -127,14 +127,14 @@ def mx4_prefill(pool: Mx4KVPool, layer: int, q, block_tables, chunk_lens, ctx_le
 def mx4_decode_device(pool: Mx4KVPool, layer: int, num_seqs: int, n_heads: int, q_dev, block_tables_dev, max_blocks: int, ctx_lens_dev,
                       max_ctx: int, out_dev, stream=None) -> None:
     """Asynchronous layer-call on device pointers."""
-    _capi.check(_capi.lib.nvk_mx4_decode_device(pool.handle, int(layer), int(num_seqs), int(n_heads), _devptr(q_dev),
-                                                _devptr(block_tables_dev), int(max_blocks), _devptr(ctx_lens_dev), int(max_ctx),
-                                                _devptr(out_dev), _devptr(stream)))
+    _capi.check(_capi.lib.nvk_mx4_decode_device(pool.handle, int(layer), int(num_seqs), int(n_heads), _address(q_dev),
+                                                _address(block_tables_dev), int(max_blocks), _address(ctx_lens_dev), int(max_ctx),
+                                                _address(out_dev), _address(stream)))
 
 
 def mx4_prefill_device(pool: Mx4KVPool, layer: int, num_seqs: int, n_heads: int, total_rows: int, q_dev, row_offsets_dev, max_rows: int,
                        block_tables_dev, max_blocks: int, ctx_lens_dev, max_ctx: int, out_dev, stream=None) -> None:
     """Asynchronous form; row_offsets_dev [num_seqs + 1] are the first rows of the sequences' chunks."""
-    _capi.check(_capi.lib.nvk_mx4_prefill_device(pool.handle, int(layer), int(num_seqs), int(n_heads), int(total_rows), _devptr(q_dev),
-                                                 _devptr(row_offsets_dev), int(max_rows), _devptr(block_tables_dev), int(max_blocks),
-                                                 _devptr(ctx_lens_dev), int(max_ctx), _devptr(out_dev), _devptr(stream)))
+    _capi.check(_capi.lib.nvk_mx4_prefill_device(pool.handle, int(layer), int(num_seqs), int(n_heads), int(total_rows), _address(q_dev),
+                                                 _address(row_offsets_dev), int(max_rows), _address(block_tables_dev), int(max_blocks),
+                                                 _address(ctx_lens_dev), int(max_ctx), _address(out_dev), _address(stream)))

@@ -12,7 +12,7 @@ from typing import Optional
 import numpy as np
 
 from . import _capi
-from .kv_pool import PagedKVPool, _devptr, _f32, _i32, _ptr
+from .kv_pool import PagedKVPool, _address, _f32, _i32, _ptr
 
 ROPE_INTERLEAVED = _capi.ROPE_INTERLEAVED
 ROPE_HALF = _capi.ROPE_HALF
@@ -35,7 +35,7 @@ class RotaryTable:
         self.head_dim, self.rotary_dim, self.layout, self.device = int(head_dim), int(rotary_dim), int(layout), int(device)
 
     def close(self) -> None:
-        if getattr(self, "_h", None):
+        if getattr(self, "_h", None) and _capi.lib is not None:  # (None: the interpreter is going down)
             _capi.lib.nvk_rope_destroy(self._h)
             self._h = None
 
@@ -65,9 +65,9 @@ def norm_rope_append_device(pool, layer: int, rope: Optional[RotaryTable], rows:
                             num_seqs: int, max_blocks: int, stream=None) -> None:
     """Asynchronous form on device pointers; see ``nvk_pool_norm_rope_append`` for what may be None."""
     _capi.check(_entry(pool)(pool.handle, int(layer), rope.handle if rope is not None else None, int(rows), int(n_heads),
-                             _devptr(q_dev), _devptr(q_out_dev), _devptr(k_rows_dev), _devptr(v_rows_dev), _devptr(q_weight_dev),
-                             _devptr(k_weight_dev), float(eps), _devptr(row_seqs_dev), _devptr(positions_dev),
-                             _devptr(block_tables_dev), int(num_seqs), int(max_blocks), _capi.PTR_DEVICE, _devptr(stream)))
+                             _address(q_dev), _address(q_out_dev), _address(k_rows_dev), _address(v_rows_dev), _address(q_weight_dev),
+                             _address(k_weight_dev), float(eps), _address(row_seqs_dev), _address(positions_dev),
+                             _address(block_tables_dev), int(num_seqs), int(max_blocks), _capi.PTR_DEVICE, _address(stream)))
 
 
 def norm_rope_append(pool, layer: int, rope: Optional[RotaryTable], q, k_rows, v_rows, block_tables, positions, row_seqs=None,

@@ -11,7 +11,7 @@ from typing import Tuple
 import numpy as np
 
 from . import _capi
-from .kv_pool import PagedKVPool, _devptr, _f32, _i32, _ptr
+from .kv_pool import PagedKVPool, _address, _f32, _i32, _ptr
 
 
 class BlockIndex:
@@ -21,7 +21,7 @@ class BlockIndex:
         self._h, self.pool = h, pool  # keeps the pool alive
 
     def close(self) -> None:
-        if getattr(self, "_h", None):
+        if getattr(self, "_h", None) and _capi.lib is not None:  # (None: the interpreter is going down)
             _capi.lib.nvk_block_index_destroy(self._h)
             self._h = None
 
@@ -64,9 +64,9 @@ class BlockIndex:
 
     def update_device(self, layer: int, num_seqs: int, block_tables_dev, max_blocks: int, starts_dev, ctx_lens_dev, max_new: int,
                       stream=None) -> None:
-        _capi.check(_capi.lib.nvk_block_index_update(self.handle, int(layer), int(num_seqs), _devptr(block_tables_dev), int(max_blocks),
-                                                     _devptr(starts_dev), _devptr(ctx_lens_dev), int(max_new), _capi.PTR_DEVICE,
-                                                     _devptr(stream)))
+        _capi.check(_capi.lib.nvk_block_index_update(self.handle, int(layer), int(num_seqs), _address(block_tables_dev), int(max_blocks),
+                                                     _address(starts_dev), _address(ctx_lens_dev), int(max_new), _capi.PTR_DEVICE,
+                                                     _address(stream)))
 
 
 def sparse_decode(index: BlockIndex, layer: int, q, block_tables, ctx_lens, top_blocks: int, first_blocks: int = 1,
@@ -89,7 +89,7 @@ def sparse_decode_device(index: BlockIndex, layer: int, num_seqs: int, n_heads: 
                          ctx_lens_dev, max_ctx: int, top_blocks: int, first_blocks: int, last_blocks: int, out_dev, selected_dev=None,
                          stream=None) -> None:
     """Asynchronous layer-call on device pointers; selected_dev (int32, may be None) receives the blocks read."""
-    _capi.check(_capi.lib.nvk_sparse_decode_device(index.handle, int(layer), int(num_seqs), int(n_heads), _devptr(q_dev),
-                                                   _devptr(block_tables_dev), int(max_blocks), _devptr(ctx_lens_dev), int(max_ctx),
-                                                   int(top_blocks), int(first_blocks), int(last_blocks), _devptr(out_dev),
-                                                   _devptr(selected_dev), _devptr(stream)))
+    _capi.check(_capi.lib.nvk_sparse_decode_device(index.handle, int(layer), int(num_seqs), int(n_heads), _address(q_dev),
+                                                   _address(block_tables_dev), int(max_blocks), _address(ctx_lens_dev), int(max_ctx),
+                                                   int(top_blocks), int(first_blocks), int(last_blocks), _address(out_dev),
+                                                   _address(selected_dev), _address(stream)))
