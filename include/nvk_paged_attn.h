@@ -441,8 +441,8 @@ int nvk_pool_norm_rope_append(nvk_pool *pool, int layer, const nvk_rope *rope, i
 /* --------------------------------------------------------- the 4-bit paged KV cache --
  * The reference's cache (include/core/model.hpp:94-97) in 17/32 byte a value instead of 4: each value is
  * sign * {0, .5, 1, 1.5, 2, 3, 4, 6} * 2^e (e2m1), with one e (a byte) for each 32 channels of a row, the smallest with
- * |values| <= 7 * 2^e; the last group is what is left of the row.  Values go to the nearest, ties to the even code.  A group
- * that holds an infinity or a NaN is stored as NaN.  Block tables, positions and contexts are those of nvk_pool.
+ * |values| <= 7 * 2^e, at most 125; the last group is what is left of the row.  Values go to the nearest, ties to the even code
+ * (above 5 * 2^125, 2.13e38, to 6 * 2^125).  A group that holds an infinity or a NaN is stored as NaN.  Block tables, positions and contexts are those of nvk_pool.
  *   block_size  a multiple of 16;  head_dim  a multiple of 8, at most 256 (stored as 32, 64, 128 or 256 channels)
  * Zero-initialised.  The layout inside a layer is the library's (nvk_mx4_pool_layer_ptr / _layer_bytes: for copies of whole
  * layers between pools of one geometry).

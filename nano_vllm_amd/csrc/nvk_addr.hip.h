@@ -29,6 +29,14 @@ __device__ __forceinline__ int clamp_block(int id, int num_blocks)
     return (int)min((unsigned)id, (unsigned)(num_blocks - 1));
 }
 
+// Four floats to a caller's address, which is aligned to one.
+__device__ __forceinline__ void store_four(float *p, float x, float y, float z, float w)
+{
+    typedef float four __attribute__((ext_vector_type(4)));
+    typedef four  anywhere __attribute__((aligned(4)));
+    *reinterpret_cast<anywhere *>(p) = four{x, y, z, w};
+}
+
 // The rotation of Ops::apply_rope (ops/positional.hpp:26-27, :35-36): four products and two sums, each rounded on
 // its own (hipcc contracts a*b - c*d into an fma by default, and __fmul_rn/__fsub_rn are plain operators in this
 // ROCm: the pragma is what keeps them separate).  cs = (cos, sin).

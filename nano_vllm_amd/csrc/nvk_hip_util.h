@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
 #include <cstring>
 
 #include "nvk_device_scope.h"
@@ -17,6 +18,13 @@
     } while (0)
 
 namespace nvk {
+
+// Tokens that a block table, a context may hold: an int has room for a tile, a chunk's rounding or a step more.
+constexpr long long kMostTokens = 0x7fff0000LL;
+// Whether a launch of `groups` workgroups of `threads` is one: the threads of a grid are counted in 32 bits.
+inline bool grid_fits(long long groups, int threads) { return groups >= 0 && groups <= 0xffffffffLL / threads; }
+
+inline bool for_floats(const void *p) { return ((uintptr_t)p & 3) == 0; } // aligned to one
 
 inline bool stream_is_capturing(hipStream_t stream)
 {

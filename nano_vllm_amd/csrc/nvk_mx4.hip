@@ -13,6 +13,7 @@
 #include <cmath>
 #include <new>
 
+#include "nvk_addr.hip.h"
 #include "nvk_chunk_join.hip.h"
 #include "nvk_hip_util.h"
 #include "nvk_mx4.hip.h"
@@ -34,13 +35,13 @@ struct Mx4AttnArgs
     const int   *row_offsets; // [num_seqs + 1] or null: row s belongs to sequence s
     const int   *tables, *ctx_lens;
     int          num_seqs, max_blocks, n_heads, group, total_rows;
-    int          col_blocks;   // workgroups along a sequence's (row, head) columns
+    int          col_blocks;   // prefill: workgroups along a sequence's (row, head) columns
     int          chunk_tokens; // tokens a workgroup takes (a multiple of 32)
     int          chunks;       // chunks along the longest context
     float        scale_log2e;  // log2(e) / sqrt(head_dim)
     float       *ws_o, *ws_ml; // partial results where chunks > 1: [rows * heads][chunks][head_dim], [..][2]
     int          whole_lines;  // the decode kernel ran
-    int         *arrivals;     // decode: one for each (sequence, column block, kv-head), or null: the join kernel follows
+    int         *arrivals;     // decode: one for each (sequence, kv-head), or null: the join kernel follows
 };
 
 // The three bf16 numbers whose sum is x, packed for two values at a time.  Truncation: each residual is exact.
@@ -484,7 +485,7 @@ __device__ __forceinline__ int mx4_rows(const Mx4AttnArgs &a, int seq, int &row0
 
 // ---- few columns: the waves of a workgroup share the tokens --------------------------------------------------------------
 // Bound by the codes it reads while everything beside the loads hides behind them; what does not is the vector work of a
-// step.  WAVES waves take steps of 32 tokens in turn and join through LDS.
+// step.  The waves take steps of 32 tokens in turn and join through LDS.
 template <int KK, bool PACK>
 __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2) nvk_mx4_decode_kernel(const Mx4AttnArgs a)
 {
@@ -492,24 +493,22 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
     constexpr int HDP = 32 * KK, COLS = Wave::COLS, W = kDecodeWaves;
     const int     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    // Workgroup -> (sequence, column block, chunk, kv-head).  Consecutive workgroups go to the eight XCDs in turn: the kv-heads
+    // Workgroup -> (sequence, chunk, kv-head); a sequence's columns are one tile.  Consecutive workgroups go to the eight XCDs in turn: the kv-heads
     // of one piece of context are put side by side on one XCD, which then reads whole blocks of the cache.
     const unsigned xcd = blockIdx.x % 8u, rest = blockIdx.x / 8u;
     const int      kvh = (int)(rest % (unsigned)a.mx.n_kv_heads);
-    unsigned       unit = rest / (unsigned)a.mx.n_kv_heads * 8u + xcd;
-    const int      chunk = (int)(unit % (unsigned)a.chunks);
-    unit /= (unsigned)a.chunks;
-    const int cb = (int)(unit % (unsigned)a.col_blocks), seq = (int)(unit / (unsigned)a.col_blocks);
+    const unsigned unit = rest / (unsigned)a.mx.n_kv_heads * 8u + xcd;
+    const int      chunk = (int)(unit % (unsigned)a.chunks), seq = (int)(unit / (unsigned)a.chunks);
     if (seq >= a.num_seqs)
         return;
     int       row0;
-    const int rows = mx4_rows(a, seq, row0), columns = rows * a.group, col0 = cb * COLS;
-    if (rows <= 0 || col0 >= columns)
+    const int rows = mx4_rows(a, seq, row0), columns = rows * a.group;
+    if (rows <= 0)
         return;
     const int ctx = mx4_context(a, seq);
     const int begin = chunk * a.chunk_tokens;
     Wave      w;
-    w.start(a, row0, rows, ctx, kvh, col0);
+    w.start(a, row0, rows, ctx, kvh, 0);
     // the chunks that some column sees; the first one writes rows that see nothing
     const int parts = max(min((w.most + a.chunk_tokens - 1) / a.chunk_tokens, a.chunks), 1);
     if (chunk >= parts)
@@ -593,19 +592,18 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
                 s_o[wave][w.lcol][(4 * w.g + i) * 2 * KK + ct] = w.acc[0][ct][i] * alpha;
     __syncthreads();
     for (int e = threadIdx.x; e < COLS * (HDP / 4); e += 64 * W) {
-        const int c16 = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
-        const int col = col0 + c16;
+        const int col = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
         if (col >= columns || c >= a.mx.head_dim)
             continue;
         float Mc = -INFINITY, L = 0.f;
 #pragma unroll
         for (int x = 0; x < W; x++)
-            Mc = fmaxf(Mc, s_m[x][c16]);
+            Mc = fmaxf(Mc, s_m[x][col]);
         f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < W; x++) {
-            L += s_m[x][c16] == -INFINITY ? 0.f : s_l[x][c16] * __builtin_amdgcn_exp2f(s_m[x][c16] - Mc);
-            o += *reinterpret_cast<const f32x4 *>(&s_o[x][c16][c]);
+            L += s_m[x][col] == -INFINITY ? 0.f : s_l[x][col] * __builtin_amdgcn_exp2f(s_m[x][col] - Mc);
+            o += *reinterpret_cast<const f32x4 *>(&s_o[x][col][c]);
         }
         const int64_t line = (int64_t)(row0 + col / a.group) * a.n_heads + kvh * a.group + col % a.group;
         if (parts > 1) {
@@ -618,19 +616,19 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
         }
         else {
             o *= L == 0.f ? 0.f : 1.f / L;
-            *reinterpret_cast<f32x4 *>(a.out + line * a.mx.head_dim + c) = o;
+            store_four(a.out + line * a.mx.head_dim + c, o[0], o[1], o[2], o[3]);
         }
     }
-    if (parts == 1 || !a.arrivals || !arrived_last(a.arrivals + ((int64_t)seq * a.col_blocks + cb) * a.mx.n_kv_heads + kvh, parts))
+    if (parts == 1 || !a.arrivals || !arrived_last(a.arrivals + (int64_t)seq * a.mx.n_kv_heads + kvh, parts))
         return;
     for (int e = threadIdx.x; e < COLS * (HDP / 4); e += 64 * W) {
-        const int col = col0 + e / (HDP / 4), c = (e % (HDP / 4)) * 4;
+        const int col = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
         if (col >= columns || c >= a.mx.head_dim)
             continue;
         const int64_t line = (int64_t)(row0 + col / a.group) * a.n_heads + kvh * a.group + col % a.group;
         // (a row of a short context was not seen by the later chunks of a longer one: they hold nothing for it)
-        *reinterpret_cast<float4 *>(a.out + line * a.mx.head_dim + c) =
-            join_few(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, parts, a.mx.head_dim);
+        const float4 o = join_few(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, parts, a.mx.head_dim);
+        store_four(a.out + line * a.mx.head_dim + c, o.x, o.y, o.z, o.w);
     }
 }
 
@@ -827,8 +825,7 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     // Waves that share the tokens while one wave holds a sequence's columns; else waves that share the columns.
     s.prefill = (long long)max_rows * group > 16;
     s.pack    = (long long)max_rows * group <= 4;
-    const int cols = s.prefill ? 16 * prefill_cols(pool->kk) * kPrefillWaves : 16;
-    s.col_blocks = ceil_div((long long)max_rows * group, cols);
+    s.col_blocks = s.prefill ? ceil_div((long long)max_rows * group, 16 * prefill_cols(pool->kk) * kPrefillWaves) : 1;
     const long long tasks = (long long)num_seqs * pool->n_kv_heads * s.col_blocks;
     // Cut the context while everything still runs at once (workgroups of four waves: so many fit a CU), into chunks of 64
     // tokens at least; not into more than can be joined inside unless those were long.  (One sequence of 777 tokens: 8.05 us
@@ -872,8 +869,8 @@ int check_attention(const nvk_mx4_pool *pool, int layer, int num_seqs, int n_hea
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: negative size", who);
     if (n_heads <= 0 || n_heads % pool->n_kv_heads != 0)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: n_heads %d is no multiple of n_kv_heads %d", who, n_heads, pool->n_kv_heads);
-    if ((long long)max_blocks * pool->block_size > 0x7fffffffLL || (long long)max_rows * n_heads > 0x3fffffffLL
-        || max_ctx > 0x7fffff00)
+    if ((long long)max_blocks * pool->block_size > nvk::kMostTokens || (long long)max_rows * n_heads > 0x3fffffffLL
+        || max_ctx > nvk::kMostTokens)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: more than 2^31 tokens in a table, or 2^30 columns in a sequence", who);
     return NVK_OK;
 }
@@ -885,7 +882,7 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
     const Mx4Shape  s = mx4_shape(pool, num_seqs, n_heads, total_rows, max_rows, max_ctx);
     const long long units = (long long)num_seqs * s.col_blocks * s.chunks;
     const long long blocks = (s.prefill ? units : (units + 7) / 8 * 8) * pool->n_kv_heads; // (decode: whole rounds of the XCDs)
-    if (blocks > 0x7fffffffLL || (long long)total_rows * n_heads > 0x7fffffffLL)
+    if (!nvk::grid_fits(blocks, 64 * kDecodeWaves) || (s.chunks > 1 && !nvk::grid_fits((long long)total_rows * n_heads, nvk::kJoinThreads)))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %lld workgroups", who, blocks);
     int rc = reserve(pool, s, st, who);
     if (rc != NVK_OK)
@@ -945,6 +942,8 @@ int attention_host(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, con
         max_rows = std::max(max_rows, n), max_ctx = std::max(max_ctx, ctx_lens[s]);
     }
     offsets[num_seqs] = (int)total;
+    if (rc == NVK_OK)
+        rc = check_attention(pool, layer, num_seqs, n_heads, (int)total, max_rows, max_blocks, max_ctx, who);
     if (rc != NVK_OK || total == 0) {
         delete[] offsets;
         return rc;
@@ -1103,6 +1102,8 @@ int nvk_mx4_decode_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_hea
         return NVK_OK;
     if (!q_dev || !block_tables_dev || !ctx_lens_dev || !out_dev)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: null pointer", who);
+    if (!nvk::for_floats(q_dev) || !nvk::for_floats(out_dev))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: q or out is not aligned to its type", who);
     NVK_SCOPE(pool->device);
     return enqueue_attention(pool, layer, num_seqs, n_heads, num_seqs, q_dev, nullptr, 1, block_tables_dev, max_blocks, ctx_lens_dev,
                              max_ctx, out_dev, stream ? (hipStream_t)stream : pool->stream, who);
@@ -1120,6 +1121,8 @@ int nvk_mx4_prefill_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_he
         return NVK_OK;
     if (!q_dev || !row_offsets_dev || !block_tables_dev || !ctx_lens_dev || !out_dev)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: null pointer", who);
+    if (!nvk::for_floats(q_dev) || !nvk::for_floats(out_dev))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: q or out is not aligned to its type", who);
     NVK_SCOPE(pool->device);
     return enqueue_attention(pool, layer, num_seqs, n_heads, total_rows, q_dev, row_offsets_dev, max_rows, block_tables_dev,
                              max_blocks, ctx_lens_dev, max_ctx, out_dev, stream ? (hipStream_t)stream : pool->stream, who);

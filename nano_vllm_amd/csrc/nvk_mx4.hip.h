@@ -68,7 +68,8 @@ __device__ __forceinline__ float mx4_value(unsigned code, unsigned scale_byte)
 
 // The shared exponent of a group whose largest magnitude is `amax`: the smallest e with amax <= 7 * 2^e, as byte e + 127.
 // 7 and not 6: up to 7 the largest code, 6, is off by at most one unit of 2^e, which is what rounding between 4 and 6 costs
-// anyway; beyond 7 clipping would cost more than the next exponent.
+// anyway; beyond 7 clipping would cost more than the next exponent.  At most 125: 6 * 2^125 is the largest level below 2^128,
+// and a value that is finite stays so (a stale infinity behind a context would reach its rows as 0 * infinity).
 __device__ __forceinline__ int mx4_scale_byte(double amax)
 {
     const unsigned long long bits = (unsigned long long)__double_as_longlong(amax);
@@ -77,7 +78,7 @@ __device__ __forceinline__ int mx4_scale_byte(double amax)
         return 255;
     const bool over = (bits & 0xfffffffffffffULL) > 0xc000000000000ULL; // 1.f > 1.75
     const int  e    = ex - 2 + (over ? 1 : 0);
-    return min(max(e, -126), 127) + 127; // (amax 0 or below the range: the smallest exponent)
+    return min(max(e, -126), 125) + 127; // (amax 0 or below the range: the smallest exponent)
 }
 
 // Nearest code, ties to the even code; x already divided by the group's scale (a power of two: exact).

@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel
     __shared__ double s_row[MX4 ? kRotaryWaves : 1][MX4 ? kRotaryBatch : 1];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = blockIdx.x * kRotaryWaves + wave; // (rows * parts fits: checked on the host)
+    const int id = blockIdx.x * kRotaryWaves + wave;
     const int row = id / parts, part = id - row * parts;
     if (row >= rows)
         return;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel
                 double     ya = x[u][j].x, yb = x[u][j].y;
                 if (weight && there)
                     ya = ya * by * (double)weight[ia[j]], yb = yb * by * (double)weight[ib[j]];
-                if (kind != 1) {
+                if (kind != 1 && lw + j * W < turned) { // (others keep what they hold: no 0 * infinity)
                     const double na = ya * cs[j] - yb * sn[j];
                     yb              = ya * sn[j] + yb * cs[j];
                     ya              = na;
@@ -319,8 +319,8 @@ __global__ void __launch_bounds__(256)
         k.z = mx4_value((kw >> (16 * h + 8)) & 15u, ks), k.w = mx4_value((kw >> (16 * h + 12)) & 15u, ks);
         v.x = mx4_value((vw >> (16 * h)) & 15u, vs), v.y = mx4_value((vw >> (16 * h + 4)) & 15u, vs);
         v.z = mx4_value((vw >> (16 * h + 8)) & 15u, vs), v.w = mx4_value((vw >> (16 * h + 12)) & 15u, vs);
-        *reinterpret_cast<float4 *>(k_out + at + 4 * h) = k;
-        *reinterpret_cast<float4 *>(v_out + at + 4 * h) = v;
+        store_four(k_out + at + 4 * h, k.x, k.y, k.z, k.w);
+        store_four(v_out + at + 4 * h, v.x, v.y, v.z, v.w);
     }
 }
 
@@ -381,8 +381,6 @@ int check_rows(int rows, const int *row_seqs, const int *positions, const int *t
     return NVK_OK;
 }
 
-bool aligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
-
 // The part that the two caches share: checks, staging of host arrays, launch.
 template <bool MX4>
 int norm_rope_append(RotaryArgs a, int device, hipStream_t own_stream, const nvk_rope *rope, int rows,
@@ -394,20 +392,24 @@ int norm_rope_append(RotaryArgs a, int device, hipStream_t own_stream, const nvk
     if (rows < 0 || a.num_seqs < 0 || (a.k && a.max_blocks <= 0) || a.n_heads <= 0 || !(a.eps >= 0.0))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: bad arguments (rows %d, num_seqs %d, max_blocks %d, n_heads %d)", who, rows,
                          a.num_seqs, a.max_blocks, a.n_heads);
+    if ((long long)a.n_heads * hd > 0x7fffffffLL)
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: n_heads %d", who, a.n_heads);
     if (hd % 2 != 0 || hd > nvk::kRotaryMaxHead)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: head_dim %d (even, at most %d)", who, hd, nvk::kRotaryMaxHead);
-    if (a.k && (long long)a.max_blocks * bs > 0x7fffffffLL)
+    if (a.k && (long long)a.max_blocks * bs > nvk::kMostTokens)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: a table of %d blocks of %d tokens passes 2^31 tokens", who, a.max_blocks, bs);
     if (rope && (rope->head_dim != hd || rope->device != device))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: the rotary table is for head_dim %d on device %d, the pool has %d on %d", who,
                          rope->head_dim, rope->device, hd, device);
     if (rows == 0)
         return NVK_OK;
+    if (!nvk::grid_fits((rows + (long long)nvk::kRotaryWaves - 1) / nvk::kRotaryWaves, 64 * nvk::kRotaryWaves))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %d rows", who, rows);
     if ((!a.q && !a.k) || (a.q != nullptr) != (a.q_out != nullptr) || (a.k != nullptr) != (a.v != nullptr))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: q and q_out, k_rows and v_rows come in pairs, at least one of them", who);
     if (!a.positions || (a.k && !a.tables))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: positions or block_tables missing", who);
-    if (!aligned(a.q, 4) || !aligned(a.q_out, 4) || !aligned(a.k, 4) || !aligned(a.v, 4))
+    if (!nvk::for_floats(a.q) || !nvk::for_floats(a.q_out) || !nvk::for_floats(a.k) || !nvk::for_floats(a.v))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: rows are not aligned to their type", who);
 
     NVK_SCOPE(device);
@@ -598,15 +600,17 @@ int nvk_mx4_pool_read_rows(nvk_mx4_pool *pool, int layer, int rows, const int *r
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: layer %d outside [0,%d)", who, layer, pool->n_layers);
     if (ptr_kind != NVK_PTR_HOST && ptr_kind != NVK_PTR_DEVICE)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: ptr_kind %d", who, ptr_kind);
-    if (rows < 0 || num_seqs < 0 || max_blocks <= 0 || (long long)max_blocks * pool->block_size > 0x7fffffffLL
+    if (rows < 0 || num_seqs < 0 || max_blocks <= 0 || (long long)max_blocks * pool->block_size > nvk::kMostTokens
         || (rows > 0 && (!positions || !block_tables || !k_out || !v_out)))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: bad arguments", who);
     if (rows == 0)
         return NVK_OK;
+    if (!nvk::for_floats(k_out) || !nvk::for_floats(v_out))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: rows are not aligned to their type", who);
     NVK_SCOPE(pool->device);
     hipStream_t st = (ptr_kind == NVK_PTR_DEVICE && stream) ? (hipStream_t)stream : pool->stream;
     const long long threads = (long long)rows * pool->n_kv_heads * (pool->head_dim / 8);
-    if (threads > 0x7fffffffLL * 256)
+    if (!nvk::grid_fits((threads + 255) / 256, 256))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %d rows", who, rows);
     const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
     if (ptr_kind == NVK_PTR_DEVICE) {

@@ -15,6 +15,7 @@
 #include <cmath>
 #include <new>
 
+#include "nvk_addr.hip.h"
 #include "nvk_chunk_join.hip.h"
 #include "nvk_hip_util.h"
 
@@ -602,8 +603,8 @@ template <int NV, int HG, bool SELECT> __global__ void __launch_bounds__(64 * kS
     for (int e = threadIdx.x; e < heads * (hd / 4); e += 64 * kSparseWaves) {
         const int64_t line = (int64_t)seq * a.n_heads + head0 + e / (hd / 4);
         const int     c = e % (hd / 4) * 4;
-        *reinterpret_cast<float4 *>(a.out + line * hd + c) =
-            join_few(a.ws_o + line * a.chunks * hd + c, a.ws_ml + line * a.chunks * 2, parts, hd);
+        const float4  x = join_few(a.ws_o + line * a.chunks * hd + c, a.ws_ml + line * a.chunks * 2, parts, hd);
+        store_four(a.out + line * hd + c, x.x, x.y, x.z, x.w);
     }
 }
 
@@ -749,7 +750,7 @@ int enqueue_update(nvk_block_index *x, int layer, int num_seqs, const int *table
     a.tables = tables, a.max_blocks = max_blocks, a.starts = starts, a.ctx_lens = ctx_lens, a.num_seqs = num_seqs;
     // max_new tokens lie in at most this many blocks
     const long long slots = std::min((long long)max_blocks, ceil_div((long long)max_new + x->block_size - 1, x->block_size));
-    if (slots * num_seqs > 0x7fffffffLL)
+    if (!nvk::grid_fits(slots * num_seqs, 256))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %lld blocks", who, slots * num_seqs);
     hipLaunchKernelGGL(nvk::nvk_index_update_kernel, dim3((unsigned)(slots * num_seqs)), dim3(256), 0, st, a, (int)slots);
     NVK_HIP_TRY(hipGetLastError());
@@ -762,7 +763,8 @@ int check_sparse(const nvk_block_index *x, int layer, int num_seqs, int n_heads,
     const int rc = check_index(x, layer, who);
     if (rc != NVK_OK)
         return rc;
-    if (num_seqs < 0 || max_blocks <= 0 || max_ctx < 0 || (long long)max_blocks * x->block_size > 0x7fffffffLL)
+    if (num_seqs < 0 || max_blocks <= 0 || max_ctx < 0 || (long long)max_blocks * x->block_size > nvk::kMostTokens
+        || max_ctx > nvk::kMostTokens)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: bad sizes (num_seqs %d, max_blocks %d, max_ctx %d)", who, num_seqs, max_blocks, max_ctx);
     if (n_heads <= 0 || n_heads % x->n_kv_heads != 0)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: n_heads %d is no multiple of n_kv_heads %d", who, n_heads, x->n_kv_heads);
@@ -777,9 +779,13 @@ int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, con
                    const int *ctx_lens, int max_ctx, int top, int first, int last, float *out, int *selected, hipStream_t st,
                    const char *who)
 {
+    if (!selected) // (a list of its own is no wider than the longest context)
+        top = std::min(top, std::max((int)ceil_div(max_ctx, x->block_size), 1));
     const SparseShape s = sparse_shape(x, num_seqs, n_heads, max_ctx, top);
     const long long   lines = (long long)num_seqs * x->n_kv_heads;
-    if (lines * s.score_slots > 0x7fffffffLL || (long long)num_seqs * n_heads > 0x7fffffffLL || lines * s.head_sets * s.chunks > 0x7fffffffLL)
+    const bool        joins = s.chunks > 1 && !s.inside;
+    if (!nvk::grid_fits(lines * s.score_slots, 64 * nvk::kSparseWaves) || !nvk::grid_fits(lines * s.head_sets * s.chunks, 64 * nvk::kSparseWaves)
+        || (!s.select_inside && !nvk::grid_fits(lines, nvk::kSelectThreads)) || (joins && !nvk::grid_fits((long long)num_seqs * n_heads, nvk::kJoinThreads)))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: too many workgroups", who);
     int rc = reserve(x, s, st, who);
     if (rc != NVK_OK)
@@ -806,7 +812,7 @@ int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, con
     default: launch_heads<8>(a, s, score, st); break;
     }
     NVK_HIP_TRY(hipGetLastError());
-    if (s.chunks > 1 && !s.inside) {
+    if (joins) {
         hipLaunchKernelGGL(nvk::nvk_sparse_join_kernel, dim3((unsigned)(num_seqs * n_heads)), dim3(nvk::kJoinThreads), 0, st, a);
         NVK_HIP_TRY(hipGetLastError());
     }
@@ -902,7 +908,7 @@ int nvk_block_index_update(nvk_block_index *index, int layer, int num_seqs, cons
         return rc;
     if (ptr_kind != NVK_PTR_HOST && ptr_kind != NVK_PTR_DEVICE)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: ptr_kind %d", who, ptr_kind);
-    if (num_seqs < 0 || max_blocks <= 0 || max_new < 0 || (long long)max_blocks * index->block_size > 0x7fffffffLL)
+    if (num_seqs < 0 || max_blocks <= 0 || max_new < 0 || (long long)max_blocks * index->block_size > nvk::kMostTokens)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: bad sizes (num_seqs %d, max_blocks %d, max_new %d)", who, num_seqs, max_blocks, max_new);
     if (num_seqs == 0 || (max_new == 0 && ptr_kind == NVK_PTR_DEVICE))
         return NVK_OK;
@@ -948,6 +954,8 @@ int nvk_sparse_decode_device(nvk_block_index *index, int layer, int num_seqs, in
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: null pointer", who);
     if ((uintptr_t)q_dev % 16 != 0)
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: q is not 16-byte aligned", who);
+    if (!nvk::for_floats(out_dev))
+        return nvk::fail(NVK_ERR_INVALID_ARG, "%s: out is not aligned to its type", who);
     NVK_SCOPE(index->device);
     hipStream_t st = nullptr;
     rc             = pool_stream(index, stream, &st);

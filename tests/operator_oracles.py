@@ -50,7 +50,7 @@ def round4(x):
         top = a.max(-1, keepdims=True)
         man, ex = np.frexp(top)  # top = man * 2^ex, man in [0.5, 1)
         e = np.where(man <= 0.875, ex - 3, ex - 2)
-        e = np.where(top == 0, -126, np.clip(e, -126, 127))
+        e = np.where(top == 0, -126, np.clip(e, -126, 125))
         z = np.ldexp(a, -e)
         code = ((z > 0.25).astype(int) + (z >= 0.75) + (z > 1.25) + (z >= 1.75) + (z > 2.5) + (z >= 3.5) + (z > 5.0))
         val = np.ldexp(LEVELS[code], np.broadcast_to(e, code.shape)) * np.where(p < 0, -1.0, 1.0)

@@ -296,3 +296,144 @@ def test_generation_together():
             qr = nv.norm_rope_append(pool, 0, rope, q[t:t + 1], k[t:t + 1], v[t:t + 1], tabs, [t], None, wq, wk)
             got[t:t + 1] = nv.mx4_decode(pool, 0, qr, tabs, [t + 1])
     assert (np.abs(got - want) <= bound).all(), np.abs(got - want).max()
+
+
+@pytest.mark.parametrize("geom", [(2, 2, 128, 16), (4, 2, 64, 32), (6, 2, 48, 16), (1, 1, 256, 16), (8, 2, 128, 16)], ids=lambda g: "x".join(map(str, g)))
+@pytest.mark.parametrize("most", [2, 4])
+def test_prefill_of_a_few_rows(geom, most):
+    """Chunks of up to 16 columns, rows behind short and long contexts beside each other (whole and cut into pieces)."""
+    H, KV, hd, bs = geom
+    rows, ctx = [1, most, 0, 2, most], [1, most, 9, 700, 2001]
+    pool, tabs, held = filled(ctx, bs, KV, hd, seed=hd + H)
+    q = np.random.default_rng(most).normal(size=(sum(rows), H, hd)).astype(np.float32)
+    with pool:
+        got = nv.mx4_prefill(pool, 1, q, tabs, rows, ctx)
+    at = 0
+    for s, n in enumerate(rows):
+        want, bound = oo.attention(q[at:at + n], *held[s], [ctx[s] - n + i + 1 for i in range(n)])
+        err = np.abs(got[at:at + n] - want)
+        assert (err <= bound).all(), f"sequence {s}: {err.max():.3e}"
+        at += n
+
+
+def test_more_pieces_than_one_workgroup_joins():
+    """Contexts of about 100 pieces beside contexts of one and of none, decode and two rows each."""
+    ctx = [9300, 40, 8200, 0, 1000]
+    pool, tabs, held = filled(ctx, 16, 1, 32, seed=33)
+    with pool:
+        check_decode(pool, tabs, held, ctx, 4, 34)
+        rows = [2, 2, 1, 0, 2]
+        q = np.random.default_rng(35).normal(size=(sum(rows), 4, 32)).astype(np.float32)
+        got = nv.mx4_prefill(pool, 1, q, tabs, rows, ctx)
+    at = 0
+    for s, n in enumerate(rows):
+        want, bound = oo.attention(q[at:at + n], *held[s], [ctx[s] - n + i + 1 for i in range(n)])
+        assert (np.abs(got[at:at + n] - want) <= bound).all()
+        at += n
+
+
+def test_stale_values_of_any_size_are_not_seen():
+    """Behind the context the last page holds the largest fp32 numbers: stored as finite ones, and none reaches a row."""
+    bs, hd, n = 32, 64, 96
+    rng = np.random.default_rng(5)
+    big = np.float32(3.4028234e38)
+    tabs = np.array([[0, 1, 2]], np.int32)
+    with nv.Mx4KVPool(1, 3, bs, 1, hd) as pool:
+        k, v = (rng.normal(size=(n, 1, hd)).astype(np.float32) for _ in range(2))
+        k[37:], v[37:] = big, -big
+        nv.norm_rope_append(pool, 0, None, None, k, v, tabs, np.arange(n), np.zeros(n, np.int32))
+        kc, vc = pool.read_rows(0, tabs, np.arange(n), np.zeros(n, np.int32))
+        assert (kc[37:] == np.float32(6 * 2.0 ** 125)).all() and (vc[37:] == np.float32(-6 * 2.0 ** 125)).all()
+        q = rng.normal(size=(17, 2, hd)).astype(np.float32)
+        for c in (1, 31, 33, 37):
+            got = nv.mx4_decode(pool, 0, q[:1], tabs, [c])
+            want, bound = oo.attention(q[:1], oo.round4(k[:c]), oo.round4(v[:c]), [c])
+            assert (np.abs(got - want) <= bound).all()
+        got = nv.mx4_prefill(pool, 0, q, tabs, [17], [37])
+        want, bound = oo.attention(q, oo.round4(k[:37]), oo.round4(v[:37]), np.arange(21, 38))
+        assert (np.abs(got - want) <= bound).all()
+
+
+def test_operands_at_any_float():
+    """q, results and rows that start 4 bytes behind a line: whole contexts, joined pieces, many rows; addresses that are refused."""
+    KV, hd, bs, H = 2, 128, 16, 8
+    ctx, rows = [700, 3, 90], [1, 2, 30]
+    pool, tabs, held = filled(ctx, bs, KV, hd, seed=36)
+    rng = np.random.default_rng(37)
+    q = rng.normal(size=(33, H, hd)).astype(np.float32)
+    shifted = lambda x: DeviceArray(np.concatenate([np.zeros(1, x.dtype), x.reshape(-1)]))  # noqa: E731
+    dq, do, dk, dv = shifted(q), shifted(np.zeros_like(q)), shifted(np.zeros((5, KV, hd), np.float32)), shifted(np.zeros((5, KV, hd), np.float32))
+    dt, dc, dof, dp = (DeviceArray(x) for x in (tabs, np.array(ctx, np.int32), np.array([0, 1, 3, 33], np.int32), np.arange(5, dtype=np.int32)))
+    ds = DeviceArray(np.zeros(5, np.int32))
+    p = lambda x: x.data_ptr() + 4  # noqa: E731
+    back = lambda x, shape: x.numpy()[1:1 + int(np.prod(shape))].reshape(shape)  # noqa: E731
+    with pool:
+        for n in (1, 3):  # one sequence: pieces joined inside
+            nv.mx4_decode_device(pool, 1, n, H, p(dq), dt, tabs.shape[1], dc, max(ctx), p(do))
+            pool.synchronize()
+            assert (back(do, (n, H, hd)) == nv.mx4_decode(pool, 1, q[:n], tabs[:n], ctx[:n])).all()
+        nv.mx4_prefill_device(pool, 1, 3, H, 33, p(dq), dof, 30, dt, tabs.shape[1], dc, max(ctx), p(do))
+        pool.synchronize()
+        assert (back(do, (33, H, hd)) == nv.mx4_prefill(pool, 1, q, tabs, rows, ctx)).all()
+        pool.read_rows_device(1, 5, ds, dp, dt, 3, tabs.shape[1], p(dk), p(dv))
+        pool.synchronize()
+        assert (back(dk, (5, KV, hd)) == held[0][0][:5]).all() and (back(dv, (5, KV, hd)) == held[0][1][:5]).all()
+        for a, b in ((p(dq) + 1, p(do)), (p(dq), p(do) + 2)):
+            with pytest.raises(nv.NvkError):
+                nv.mx4_decode_device(pool, 1, 3, H, a, dt, tabs.shape[1], dc, max(ctx), b)
+            with pytest.raises(nv.NvkError):
+                nv.mx4_prefill_device(pool, 1, 3, H, 33, a, dof, 30, dt, tabs.shape[1], dc, max(ctx), b)
+            with pytest.raises(nv.NvkError):
+                pool.read_rows_device(1, 5, ds, dp, dt, 3, tabs.shape[1], a, b)
+        with pytest.raises(nv.NvkError):
+            nv.mx4_decode_device(pool, 1, 3, H, dq, dt, tabs.shape[1], dc, 2 ** 31 - 1, do)
+
+
+def test_a_layer_of_more_than_32_bits():
+    """Blocks that lie beyond 4 GiB of a layer hold and answer what the first ones do."""
+    KV, hd, bs, H, n = 8, 128, 16, 16, 75
+    blocks = 260_000  # 17408 bytes each
+    rng = np.random.default_rng(38)
+    k, v = (rng.normal(size=(n, KV, hd)).astype(np.float32) for _ in range(2))
+    q = rng.normal(size=(n, H, hd)).astype(np.float32)
+    low = np.array([[3, 0, 4, 1, 2]], np.int32)
+    high = blocks - 1 - low
+    got = []
+    with nv.Mx4KVPool(1, blocks, bs, KV, hd) as pool:
+        assert pool.layer_bytes > 2 ** 32
+        for tabs in (low, high):
+            nv.norm_rope_append(pool, 0, None, None, k, v, tabs, np.arange(n), np.zeros(n, np.int32))
+            got.append((pool.read_rows(0, tabs, np.arange(n), np.zeros(n, np.int32)), nv.mx4_decode(pool, 0, q[:1], tabs, [n]),
+                        nv.mx4_prefill(pool, 0, q, tabs, [n], [n])))
+    (r0, d0, p0), (r1, d1, p1) = got
+    assert (r0[0] == oo.round4(k)).all() and (r1[0] == r0[0]).all() and (r1[1] == r0[1]).all()
+    assert (d0 == d1).all() and (p0 == p1).all()
+
+
+def test_two_pools_at_once_and_shared_blocks():
+    """Calls on two pools, each on a stream of its own, overlap; sequences of one batch share their first blocks."""
+    KV, hd, bs, H, n = 1, 128, 16, 4, 3
+    rng = np.random.default_rng(39)
+    streams = [Stream(), Stream()]
+    sets = []
+    for i in range(2):
+        k, v = (rng.normal(size=(2600, KV, hd)).astype(np.float32) for _ in range(2))
+        base, blocks = oo.tables_for([2600], bs, seed=i)
+        tabs, ctx = np.repeat(base, n, 0), np.array([2600, 1333, 16 * 50], np.int32)
+        pool = nv.Mx4KVPool(1, blocks, bs, KV, hd)
+        nv.norm_rope_append(pool, 0, None, None, k, v, base, np.arange(2600), np.zeros(2600, np.int32))
+        q = rng.normal(size=(n, H, hd)).astype(np.float32)
+        want = nv.mx4_decode(pool, 0, q, tabs, ctx)
+        for s in range(n):
+            w, bound = oo.attention(q[s:s + 1], oo.round4(k), oo.round4(v), [ctx[s]])
+            assert (np.abs(want[s] - w[0]) <= bound[0]).all()
+        d = [DeviceArray(x) for x in (q, tabs, ctx, np.zeros_like(q))]
+        sets.append((pool, d, want, tabs))
+    for turn in range(20):
+        for (pool, d, _, tabs), st in zip(sets, streams):
+            nv.mx4_decode_device(pool, 0, n, H, d[0], d[1], tabs.shape[1], d[2], 2600, d[3], st)
+    for (pool, d, want, _), st in zip(sets, streams):
+        st.synchronize()
+        assert (d[3].numpy() == want).all()
+        pool.close()
+        st.close()

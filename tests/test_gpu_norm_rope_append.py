@@ -254,3 +254,72 @@ def test_captured_and_on_another_stream(cache):
                 check(k, kw, np.abs(kw).max(-1, keepdims=True), "k")
                 assert (v == host["v"]).all()
     st.close()
+
+
+@pytest.mark.parametrize("layout", [nv.ROPE_HALF, nv.ROPE_INTERLEAVED])
+@pytest.mark.parametrize("turned", [0, 32])
+def test_channels_that_do_not_turn_keep_their_values(layout, turned):
+    """Infinities, NaN and signed zeros beside each other: nothing of a channel reaches its neighbour."""
+    H, KV, hd, bs, n = 3, 2, 64, 16, 20
+    rng = np.random.default_rng(12)
+    q, k, v = (rng.normal(size=(n, h, hd)).astype(np.float32) for h in (H, KV, KV))
+    for x in (q, k):
+        x[:, :, 33], x[:, :, 36], x[:, :, 38], x[:, :, 41] = np.inf, -np.inf, np.nan, -0.0
+        x[:, :, 40] = -1.0
+    tabs, blocks = oo.tables_for([n], bs)
+    rope = nv.RotaryTable(hd, turned, layout) if turned else None
+    pos, seqs = np.arange(n, dtype=np.int32), np.zeros(n, np.int32)
+    with make_pool("fp32", blocks, bs, KV, hd) as pool:
+        got = nv.norm_rope_append(pool, 0, rope, q, k, v, tabs, pos, seqs)
+        kc, vc = cached_rows(pool, "fp32", 0, tabs, seqs, pos)
+    for a, b in ((got, q), (kc, k), (vc, v)):
+        a, b = a[..., turned:], b[..., turned:]
+        assert np.array_equal(a, b, equal_nan=True) and np.array_equal(np.signbit(a[~np.isnan(a)]), np.signbit(b[~np.isnan(b)]))
+        assert np.isfinite(got[..., :turned]).all()
+
+
+@pytest.mark.parametrize("cache", ["fp32", "mx4"])
+def test_rows_at_any_float(cache):
+    """Rows, weights and results that start 4 bytes behind a line, device form; sizes and addresses that are refused."""
+    H, KV, hd, bs, n = 5, 2, 128, 16, 37
+    rng = np.random.default_rng(13)
+    q, k, v = (rng.normal(size=(n, h, hd)).astype(np.float32) for h in (H, KV, KV))
+    wq, wk = (rng.normal(1, 0.2, hd).astype(np.float32) for _ in range(2))
+    tabs, blocks = oo.tables_for([n], bs)
+    pos, seqs = np.arange(n, dtype=np.int32), np.zeros(n, np.int32)
+    rope = nv.RotaryTable(hd, layout=nv.ROPE_HALF)
+    shifted = lambda x: DeviceArray(np.concatenate([np.zeros(1, x.dtype), x.reshape(-1)]))  # noqa: E731
+    d = {name: shifted(x) for name, x in (("q", q), ("o", np.zeros_like(q)), ("k", k), ("v", v), ("wq", wq), ("wk", wk))}
+    at = {name: x.data_ptr() + 4 for name, x in d.items()}
+    i = [DeviceArray(x) for x in (seqs, pos, tabs)]
+    with make_pool(cache, blocks, bs, KV, hd) as pool:
+        want = nv.norm_rope_append(pool, 0, rope, q, k, v, tabs, pos, seqs, wq, wk, EPS)
+
+        def call(rows=n, heads=H, **kw):
+            a = {**at, **kw}
+            nv.norm_rope_append_device(pool, 1, rope, rows, heads, a["q"], a["o"], a["k"], a["v"], a["wq"], a["wk"], EPS, *i, 1, tabs.shape[1])
+
+        call()
+        pool.synchronize()
+        assert (d["o"].numpy()[1:].reshape(q.shape) == want).all()
+        rows0, rows1 = (cached_rows(pool, cache, layer, tabs, seqs, pos) for layer in (0, 1))
+        assert (rows0[0] == rows1[0]).all() and (rows0[1] == rows1[1]).all()
+        for kw in (dict(q=at["q"] + 1), dict(o=at["o"] + 2), dict(k=at["k"] + 3), dict(v=at["v"] + 1), dict(rows=2 ** 31 - 1), dict(rows=-1),
+                   dict(heads=2 ** 31 - 1)):
+            with pytest.raises(nv.NvkError):
+                call(**kw)
+
+
+def test_far_positions():
+    """Positions of a million: the angle's fraction is kept (the two sides' products differ by 2^20 * 2^-52 * pi < 1e-9 of a turn)."""
+    H, hd, n = 2, 64, 50
+    rng = np.random.default_rng(14)
+    q = rng.normal(size=(n, H, hd)).astype(np.float32)
+    pos = (2 ** 20 - rng.integers(0, 5000, n)).astype(np.int32)
+    freq, m = oo.frequencies(hd, 10000.0)
+    want = oo.norm_rope(q, None, EPS, pos, freq, m, True)
+    d, dp = DeviceArray(q), DeviceArray(pos)
+    with make_pool("fp32", 1, 16, 1, hd) as pool:
+        nv.norm_rope_append_device(pool, 0, nv.RotaryTable(hd, layout=nv.ROPE_HALF), n, H, d, d, None, None, None, None, EPS, None, dp, None, 0, 0)
+        pool.synchronize()
+    assert (np.abs(d.numpy() - want) <= oo.U * np.abs(want) + 2e-9 * np.abs(want).max(-1, keepdims=True)).all()

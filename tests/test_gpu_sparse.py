@@ -232,3 +232,46 @@ def test_decode_loop_together_and_captured():
                     want, bound = oo.attention(qr[s:s + 1, j * g:(j + 1) * g], kr[s][tok, j:j + 1], v[s][tok, j:j + 1], [len(tok)])
                     assert (np.abs(got[s, j * g:(j + 1) * g] - want[0]) <= bound[0]).all()
     st.close()
+
+
+def test_a_pool_and_an_index_of_more_than_32_bits():
+    """Blocks whose keys and whose bounds lie beyond 2^31 floats of a layer answer what the first ones do."""
+    KV, hd, bs, H, n = 8, 128, 4, 16, 41
+    blocks = 1_060_000  # 4096 floats of keys, 2048 of bounds each
+    rng = np.random.default_rng(60)
+    k, v = (rng.normal(size=(n, KV, hd)).astype(np.float32) for _ in range(2))
+    q = rng.normal(size=(1, H, hd)).astype(np.float32)
+    low = np.random.default_rng(61).permutation(11).astype(np.int32)[None]
+    high = (blocks - 1 - low).astype(np.int32)
+    got = []
+    with nv.PagedKVPool(1, blocks, bs, KV, hd) as pool, nv.BlockIndex(pool) as index:
+        for tabs in (low, high):
+            nv.norm_rope_append(pool, 0, None, None, k, v, tabs, np.arange(n), np.zeros(n, np.int32))
+            index.update(0, tabs, [0], [n])
+            got.append(nv.sparse_decode(index, 0, q, tabs, [n], 5, 1, 1))
+    assert (got[0][0] == got[1][0]).all() and (got[0][1] == got[1][1]).all()
+    score = oo.block_scores(q[0], k, n, bs, KV)
+    for j in range(KV):
+        assert got[0][1][0, j].tolist() == oo.choose(score[j], 11, 5, 1, 1)
+
+
+def test_without_a_list_and_at_any_float():
+    """The list left out (also with top_blocks far above the blocks there are), a result 4 bytes behind a line, other streams,
+    and what is refused."""
+    KV, hd, bs, H = 2, 32, 4, 4
+    ctx = [9001, 37, 0]
+    pool, tabs, held = filled(ctx, bs, KV, hd, seed=62)
+    q = np.random.default_rng(63).normal(size=(3, H, hd)).astype(np.float32)
+    st = Stream()
+    with pool, nv.BlockIndex(pool) as index:
+        index.update(1, tabs, [0] * 3, ctx)
+        dq, dt, dc, do = (DeviceArray(x) for x in (q, tabs, np.array(ctx, np.int32), np.zeros(3 * H * hd + 1, np.float32)))
+        for top, n in ((64, 3), (700, 3), (5000, 3), (2 ** 31 - 1, 3), (4, 1)):
+            want, _ = nv.sparse_decode(index, 1, q[:n], tabs[:n], ctx[:n], min(top, 5000))
+            nv.sparse_decode_device(index, 1, n, H, dq, dt, tabs.shape[1], dc, max(ctx), top, 1, 1, do.data_ptr() + 4, None, st)
+            st.synchronize()
+            assert (do.numpy()[1:1 + n * H * hd].reshape(n, H, hd) == want).all(), top
+        for kw in (dict(out=do.data_ptr() + 2), dict(ctx=2 ** 31 - 1)):
+            with pytest.raises(nv.NvkError):
+                nv.sparse_decode_device(index, 1, 3, H, dq, dt, tabs.shape[1], dc, kw.get("ctx", max(ctx)), 9, 1, 1, kw.get("out", do.data_ptr()))
+    st.close()
