@@ -425,7 +425,7 @@ int nvk_rope_frequencies(const nvk_rope *rope, double *freq, int cap, double *fa
  *   q_weight, k_weight [head_dim]: y = x / sqrt(mean(x^2) + eps) * weight before the rotation; NULL = no norm
  *   rope        NULL = no rotation
  *   row_seqs    [rows] table row of each token row; NULL = row r belongs to sequence r
- *   positions   [rows] position of each row's token; negative = a row of padding: nothing of it is read or written
+ *   positions   [rows] position of each row's token; negative = a row of padding: nothing of it is written
  *   block_tables [num_seqs, max_blocks]
  * Either q and q_out or k_rows and v_rows may be NULL (append only; rotate only: then positions alone matter).
  * All sums, angles and products are held in 64 bits and rounded once, to fp32 or to the cache's 4 bits.

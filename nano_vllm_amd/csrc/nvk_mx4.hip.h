@@ -66,33 +66,38 @@ __device__ __forceinline__ float mx4_value(unsigned code, unsigned scale_byte)
     return scale_byte == 255u ? __uint_as_float(0x7fc00000u) : s;
 }
 
-// The shared exponent of a group whose largest magnitude is `amax`: the smallest e with amax <= 7 * 2^e, as byte e + 127.
+// y in the 24 bits of a float, cut and not rounded, the last bit set where anything was cut off: above, at or below any number of
+// few bits exactly where y is, so that what is decided on it is decided on y.  (Below 2^-126 the conversion rounds.  From 2^128 on
+// y is an infinity, as it is in an fp32 cache.)
+__device__ __forceinline__ float mx4_cut(double y)
+{
+    const unsigned long long bits = (unsigned long long)__double_as_longlong(y);
+    const float f = (float)__longlong_as_double((long long)(bits & ~0x1fffffffULL));
+    return __uint_as_float(__float_as_uint(f) | (((unsigned)bits & 0x1fffffffu) != 0u ? 1u : 0u));
+}
+
+// The scale byte of a group from the largest of its values' bits without their signs: the smallest e with amax <= 7 * 2^e, as e + 127;
+// 255 where the group holds an infinity or a NaN.
 // 7 and not 6: up to 7 the largest code, 6, is off by at most one unit of 2^e, which is what rounding between 4 and 6 costs
 // anyway; beyond 7 clipping would cost more than the next exponent.  At most 125: 6 * 2^125 is the largest level below 2^128,
 // and a value that is finite stays so (a stale infinity behind a context would reach its rows as 0 * infinity).
-__device__ __forceinline__ int mx4_scale_byte(double amax)
+__device__ __forceinline__ unsigned mx4_scale_byte(unsigned amax)
 {
-    const unsigned long long bits = (unsigned long long)__double_as_longlong(amax);
-    const int                ex   = (int)((bits >> 52) & 0x7ffu) - 1023; // amax = 1.f * 2^ex
-    if (ex == 1024)
-        return 255;
-    const bool over = (bits & 0xfffffffffffffULL) > 0xc000000000000ULL; // 1.f > 1.75
-    const int  e    = ex - 2 + (over ? 1 : 0);
-    return min(max(e, -126), 125) + 127; // (amax 0 or below the range: the smallest exponent)
+    const int e = (int)(amax >> 23) - 129 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0); // over 1.75 * 2^ex
+    return amax >= 0x7f800000u ? 255u : (unsigned)(min(max(e, -126), 125) + 127); // (0 or below the range: the smallest exponent)
 }
 
-// Nearest code, ties to the even code; x already divided by the group's scale (a power of two: exact).
-// Counting thresholds that lie below |x| does the rounding: a tie counts exactly where the upper code is the even one.  All
-// thresholds have an empty lower half, so the comparison is made on the upper half and whether anything is left below it.
-__device__ __forceinline__ unsigned mx4_code(double x)
+// The codes of eight values under a scale byte up to 252: to the nearest, ties to the even code, 6 at most.  The conversion does
+// just that, checked on every tie and its neighbours under every exponent.
+__device__ __forceinline__ unsigned mx4_codes(const float (&x)[8], unsigned scale_byte)
 {
-    const unsigned long long bits = (unsigned long long)__double_as_longlong(x);
-    const unsigned a = (unsigned)(bits >> 32) << 1 | ((unsigned)bits != 0u); // (the sign is shifted out)
-    constexpr unsigned q1 = 2u * 0x3fd00000u, q3 = 2u * 0x3fe80000u, q5 = 2u * 0x3ff40000u, q7 = 2u * 0x3ffc0000u, // .25 .75 1.25 1.75
-        h5 = 2u * 0x40040000u, h7 = 2u * 0x400c0000u, five = 2u * 0x40140000u;                                      // 2.5 3.5 5
-    const unsigned mag = (unsigned)(a > q1) + (unsigned)(a >= q3) + (unsigned)(a > q5) + (unsigned)(a >= q7) + (unsigned)(a > h5)
-                         + (unsigned)(a >= h7) + (unsigned)(a > five);
-    return mag | (unsigned)(bits >> 60 & 8u);
+    const float scale = __uint_as_float(scale_byte << 23);
+    unsigned    word = 0;
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[0], x[1], scale, 0);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[2], x[3], scale, 1);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[4], x[5], scale, 2);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[6], x[7], scale, 3);
+    return word;
 }
 
 } // namespace nvk

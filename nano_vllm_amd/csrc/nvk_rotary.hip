@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "nvk_addr.hip.h"
@@ -44,7 +45,7 @@ struct RotaryArgs
     const float  *q, *k, *v;   // [rows, heads, head_dim]; q or (k and v) may be null
     float        *q_out;
     const float  *q_weight, *k_weight; // [head_dim] or null
-    double        eps;
+    double        eps, inv_head_dim;
     const double *freq; // [rotary_dim / 2], in half turns per position; or null
     double        factor;
     int           rotary_dim, half_layout;
@@ -106,38 +107,38 @@ __global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel
     constexpr int U = PPL == 2 ? 2 : 4; // head rows per lane at a time
     constexpr int R = 64 / W;           // head rows side by side in a wave
     constexpr int HB = U * R;           // head rows per batch
-    __shared__ double s_row[MX4 ? kRotaryWaves : 1][MX4 ? kRotaryBatch : 1];
+    __shared__ __attribute__((aligned(16))) float s_row[MX4 ? kRotaryWaves : 1][MX4 ? kRotaryBatch : 4];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int id = blockIdx.x * kRotaryWaves + wave;
     const int row = id / parts, part = id - row * parts;
     if (row >= rows)
         return;
+    // everything that does not hang on the row's place is on its way before the place is known
     const int pos = a.positions[row];
     const int seq = a.row_seqs ? a.row_seqs[row] : row;
-    const int bs = a.mx.block_size;
-    // rows of padding, and rows that have no place in their table, are left alone
-    if (pos < 0 || (a.k && (seq < 0 || seq >= a.num_seqs || pos / bs >= a.max_blocks)))
-        return;
-    const int  hd = a.mx.head_dim, pairs = hd >> 1, kv = a.mx.n_kv_heads;
-    const int  block = a.k ? a.tables[(int64_t)seq * a.max_blocks + pos / bs] : 0;
-    const int  offset = pos % bs;
-    const bool keep = a.k && block >= 0 && block < a.mx.num_blocks;
-    const int  lane = threadIdx.x & 63;
-    const int  sub = lane / W, lw = lane % W; // which of the wave's head rows, and the lane's place in it
-    int        ia[PPL], ib[PPL];
+    const int bs = a.mx.block_size, hd = a.mx.head_dim, pairs = hd >> 1, kv = a.mx.n_kv_heads;
+    const int lane = threadIdx.x & 63;
+    const int sub = lane / W, lw = lane % W; // which of the wave's head rows, and the lane's place in it
+    int       ia[PPL], ib[PPL];
 #pragma unroll
     for (int j = 0; j < PPL; j++)
         pair_channels(a, lw + j * W, ia[j], ib[j]);
+    const int turned = a.freq ? a.rotary_dim >> 1 : 0;
+    double    freq[PPL];
+#pragma unroll
+    for (int j = 0; j < PPL; j++)
+        freq[j] = lw + j * W < turned ? a.freq[lw + j * W] : 0.0;
 
     // batches: keys, values, queries; this wave's are part, part + parts, ..
     const int kb = a.k ? (kv + HB - 1) / HB : 0, qb = a.q ? (a.n_heads + HB - 1) / HB : 0;
     const int batches = 2 * kb + qb;
     auto      kind_of = [&](int t) { return t < kb ? 0 : t < 2 * kb ? 1 : 2; }; // key, value, query
-    auto      fetch = [&](int t, float2 (&x)[U][PPL]) {
+    auto      fetch = [&](int t, float2 (&x)[U][PPL], float2 (&w)[PPL]) {
         const int    kind = kind_of(t);
         const int    head0 = (t - kind * kb) * HB, heads = kind == 2 ? a.n_heads : kv;
         const float *src = (kind == 0 ? a.k : kind == 1 ? a.v : a.q) + (int64_t)row * heads * hd;
+        const float *weight = kind == 0 ? a.k_weight : kind == 1 ? nullptr : a.q_weight;
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
@@ -147,38 +148,39 @@ __global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel
                 if (head < heads && lw + j * W < pairs)
                     x[u][j] = make_float2(src[head * hd + ia[j]], src[head * hd + ib[j]]);
             }
+#pragma unroll
+        for (int j = 0; j < PPL; j++) {
+            w[j] = make_float2(1.f, 1.f);
+            if (weight && lw + j * W < pairs)
+                w[j] = make_float2(weight[ia[j]], weight[ib[j]]);
+        }
     };
-    float2 next[U][PPL];
+    float2 next[U][PPL], next_w[PPL];
     int    t = part;
     if (t < batches)
-        fetch(t, next);
+        fetch(t, next, next_w);
 
-    const int turned = a.freq ? a.rotary_dim >> 1 : 0;
-    double    cs[PPL], sn[PPL];
+    // rows of padding, and rows that have no place in their table, are left alone
+    if (pos < 0 || (a.k && (seq < 0 || seq >= a.num_seqs || pos / bs >= a.max_blocks)))
+        return;
+    const int  block = a.k ? a.tables[(int64_t)seq * a.max_blocks + pos / bs] : 0;
+    const int  offset = pos % bs;
+    const bool keep = a.k && block >= 0 && block < a.mx.num_blocks;
+    double     cs[PPL], sn[PPL];
 #pragma unroll
     for (int j = 0; j < PPL; j++) {
         cs[j] = 1.0, sn[j] = 0.0;
         if (lw + j * W < turned) {
-            sincospi((double)pos * a.freq[lw + j * W], &sn[j], &cs[j]);
+            sincospi((double)pos * freq[j], &sn[j], &cs[j]);
             cs[j] *= a.factor, sn[j] *= a.factor;
         }
     }
 
-    for (; t < batches; t += parts) {
-        const int    kind = kind_of(t);
-        const int    head0 = (t - kind * kb) * HB, heads = kind == 2 ? a.n_heads : kv;
-        const float *weight = kind == 0 ? a.k_weight : kind == 1 ? nullptr : a.q_weight;
-        float2       x[U][PPL];
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int j = 0; j < PPL; j++)
-                x[u][j] = next[u][j];
-        if (t + parts < batches)
-            fetch(t + parts, next);
-        if (kind < 2 && !keep)
-            continue;
-
+    // one batch of keys, values or queries
+    auto work = [&](auto k_, int t, const float2 (&x)[U][PPL], const float2 (&wt)[PPL]) {
+        constexpr int kind = decltype(k_)::value;
+        const int     head0 = (t - kind * kb) * HB, heads = kind == 2 ? a.n_heads : kv;
+        const bool    weight = kind == 0 ? a.k_weight != nullptr : kind == 2 && a.q_weight != nullptr;
         double scale = 1.0; // of head row u: in lane u of every quad
         if (weight) {
             double ss[U];
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel
 #pragma unroll
             for (int u = 1; u < U; u++)
                 mine = (lane & 3) == u ? ss[u] : mine;
-            scale = rsqrt(mine / hd + a.eps);
+            scale = rsqrt(fma(mine, a.inv_head_dim, a.eps));
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -202,20 +204,25 @@ __global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel
             const double by = u == 0 ? across<0x00>(scale) : u == 1 ? across<0x55>(scale) : u == 2 ? across<0xAA>(scale) : across<0xFF>(scale);
 #pragma unroll
             for (int j = 0; j < PPL; j++) {
-                const bool there = head < heads && lw + j * W < pairs;
-                double     ya = x[u][j].x, yb = x[u][j].y;
-                if (weight && there)
-                    ya = ya * by * (double)weight[ia[j]], yb = yb * by * (double)weight[ib[j]];
-                if (kind != 1 && lw + j * W < turned) { // (others keep what they hold: no 0 * infinity)
-                    const double na = ya * cs[j] - yb * sn[j];
-                    yb              = ya * sn[j] + yb * cs[j];
-                    ya              = na;
+                const bool there = head < heads && lw + j * W < pairs, turns = kind != 1 && lw + j * W < turned;
+                float      xa = x[u][j].x, xb = x[u][j].y;
+                if (weight || turns) { // (others keep what they hold: no 0 * infinity)
+                    double ya = xa, yb = xb;
+                    if (weight)
+                        ya = ya * by * (double)wt[j].x, yb = yb * by * (double)wt[j].y;
+                    if (turns) {
+                        const double na = ya * cs[j] - yb * sn[j];
+                        yb              = ya * sn[j] + yb * cs[j];
+                        ya              = na;
+                    }
+                    const bool cut = MX4 && kind == 0;
+                    xa = cut ? mx4_cut(ya) : (float)ya, xb = cut ? mx4_cut(yb) : (float)yb;
                 }
                 if (!there)
                     continue;
                 if (MX4 && kind < 2) {
-                    s_row[wave][(u * R + sub) * hd + ia[j]] = ya;
-                    s_row[wave][(u * R + sub) * hd + ib[j]] = yb;
+                    s_row[wave][(u * R + sub) * hd + ia[j]] = xa;
+                    s_row[wave][(u * R + sub) * hd + ib[j]] = xb;
                 }
                 else {
                     float *dst;
@@ -223,63 +230,75 @@ __global__ void __launch_bounds__(64 * kRotaryWaves) nvk_norm_rope_append_kernel
                         dst = a.q_out + ((int64_t)row * heads + head) * hd;
                     else
                         dst = (kind == 0 ? a.k_slab : a.v_slab) + row_float_index(block, offset, head, bs, kv, hd);
-                    dst[ia[j]] = (float)ya, dst[ib[j]] = (float)yb;
+                    dst[ia[j]] = xa, dst[ib[j]] = xb;
                 }
             }
         }
-        if constexpr (MX4) {
-            if (kind < 2) { // (the wave's own part of LDS: written and read by the same wave, in order)
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                const int  octets = hd >> 3; // dwords of codes per head row
-                const int  mine = lane / octets, c0 = (lane % octets) * 8, head = head0 + mine;
-                const bool there = mine < HB && head < heads;
-                double     y[8], amax = 0.0;
-                bool       finite = true;
+        if constexpr (MX4 && kind < 2) { // (the wave's own part of LDS: written and read by the same wave, in order)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int  octets = hd >> 3; // dwords of codes per head row
+            const int  mine = lane / octets, c0 = (lane % octets) * 8, head = head0 + mine;
+            const bool there = mine < HB && head < heads;
+            float      y[8];
+            unsigned   amax = 0; // as bits: an infinity or a NaN is larger than any number
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    y[i] = there ? s_row[wave][mine * hd + c0 + i] : 0.0;
-                    amax = fmax(amax, fabs(y[i]));
-                    finite = finite && fabs(y[i]) < INFINITY;
-                }
-                // the group of 32 channels is four lanes, or what is left of the row (rows of 48 or 56 channels are 6 or 7
-                // lanes: partners go by the place in the row, and each lane asks all of them)
-                const int    group = c0 / 32;
-                const double amax_own = amax;
-                const int    bad_own = finite ? 0 : 1;
-                int          bad = bad_own;
+            for (int i = 0; i < 8; i++) {
+                y[i] = there ? s_row[wave][mine * hd + c0 + i] : 0.f;
+                amax = max(amax, __float_as_uint(y[i]) & 0x7fffffffu);
+            }
+            // the group of 32 channels is four lanes, or what is left of the row
+            const int group = c0 / 32;
+            if (octets % 4 == 0) {
+                amax = max(amax, (unsigned)__builtin_amdgcn_update_dpp(0, (int)amax, 0xB1, 0xF, 0xF, true));
+                amax = max(amax, (unsigned)__builtin_amdgcn_update_dpp(0, (int)amax, 0x4E, 0xF, 0xF, true));
+            }
+            else { // (rows of 48 or 56 channels are 6 or 7 lanes: partners go by the place in the row, each lane asks all of them)
+                const unsigned own = amax;
 #pragma unroll
                 for (int o = 1; o <= 3; o++) {
                     const int pc = (((c0 >> 3) & 3) ^ o) + 4 * group;
-                    const int from = pc < octets ? mine * octets + pc : lane;
-                    amax = fmax(amax, __shfl(amax_own, from));
-                    bad |= __shfl(bad_own, from);
+                    amax = max(amax, (unsigned)__shfl((int)own, pc < octets ? mine * octets + pc : lane));
                 }
-                if (there) {
-                    const unsigned sb = bad ? 255u : (unsigned)mx4_scale_byte(amax);
-                    const double   inv = __longlong_as_double((long long)(1023 - ((int)sb - 127)) << 52);
-                    unsigned       word = 0;
-                    if (!bad)
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            word |= mx4_code(y[i] * inv) << (4 * i);
-                    const int      kk = a.mx.kk, tok = offset % kMx4Tile;
-                    unsigned char *tile = a.mx.tile(block, offset, head);
-                    if (kind == 0)
-                        *reinterpret_cast<unsigned *>(tile + tok * 16 * kk + c0 / 2) = word;
-                    else if (kk >= 4)
-                        *reinterpret_cast<unsigned *>(tile + mx4_v_at(kk) + mx4_v_byte(tok, c0, kk)) = word;
-                    else
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            tile[mx4_v_at(kk) + mx4_v_byte(tok, c0 + 2 * i, kk)] = (unsigned char)(word >> (8 * i));
-                    if (c0 % 32 == 0)
-                        tile[(kind == 0 ? mx4_ks_at(kk) : mx4_vs_at(kk)) + group * kMx4Tile + tok] = (unsigned char)sb;
-                }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
             }
+            if (there) {
+                const unsigned sb = mx4_scale_byte(amax), word = sb == 255u ? 0u : mx4_codes(y, sb);
+                const int      kk = a.mx.kk, tok = offset % kMx4Tile;
+                unsigned char *tile = a.mx.tile(block, offset, head);
+                if (kind == 0)
+                    *reinterpret_cast<unsigned *>(tile + tok * 16 * kk + c0 / 2) = word;
+                else if (kk >= 4)
+                    *reinterpret_cast<unsigned *>(tile + mx4_v_at(kk) + mx4_v_byte(tok, c0, kk)) = word;
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        tile[mx4_v_at(kk) + mx4_v_byte(tok, c0 + 2 * i, kk)] = (unsigned char)(word >> (8 * i));
+                if (c0 % 32 == 0)
+                    tile[(kind == 0 ? mx4_ks_at(kk) : mx4_vs_at(kk)) + group * kMx4Tile + tok] = (unsigned char)sb;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
+    };
+    for (; t < batches; t += parts) {
+        float2 x[U][PPL], wt[PPL];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < PPL; j++)
+                x[u][j] = next[u][j];
+#pragma unroll
+        for (int j = 0; j < PPL; j++)
+            wt[j] = next_w[j];
+        if (t + parts < batches)
+            fetch(t + parts, next, next_w);
+        const int kind = kind_of(t);
+        if (kind == 2)
+            work(std::integral_constant<int, 2>(), t, x, wt);
+        else if (keep && kind == 0)
+            work(std::integral_constant<int, 0>(), t, x, wt);
+        else if (keep)
+            work(std::integral_constant<int, 1>(), t, x, wt);
     }
 }
 
@@ -338,8 +357,8 @@ template <bool MX4> void launch_rotary(const RotaryArgs &a, int rows, hipStream_
     const int w = pairs <= 16 ? 16 : pairs <= 32 ? 32 : 64;
     const int hb = pairs > 64 ? 2 : 4 * (64 / w);
     const int batches = (a.k ? 2 * ((a.mx.n_kv_heads + hb - 1) / hb) : 0) + (a.q ? (a.n_heads + hb - 1) / hb : 0);
-    // Few rows: a row's batches are spread over several waves, one each at most, while there are
-    // no more than sixteen waves for every CU.
+    // Few rows: a row's batches are spread over several waves, one each at most, while there are no more than sixteen waves for
+    // every CU.  (3001 rows of three batches: 10.6 us a wave a row, 12.9 two, 13.9 three; 256 rows of twelve: 7.9 us.)
     const int  parts = (int)std::max(1LL, std::min((long long)batches, 16LL * kCus / rows));
     const dim3 grid((unsigned)(((long long)rows * parts + nvk::kRotaryWaves - 1) / nvk::kRotaryWaves)), block(64 * nvk::kRotaryWaves);
     if (pairs > 64)
@@ -414,6 +433,7 @@ int norm_rope_append(RotaryArgs a, int device, hipStream_t own_stream, const nvk
 
     NVK_SCOPE(device);
     hipStream_t st = (ptr_kind == NVK_PTR_DEVICE && stream) ? (hipStream_t)stream : own_stream;
+    a.inv_head_dim = 1.0 / hd;
     a.freq = rope ? rope->freq_dev : nullptr;
     a.factor = rope ? rope->factor : 1.0;
     a.rotary_dim = rope ? rope->rotary_dim : 0;
