@@ -158,8 +158,11 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
         return;
     const int  hd = a.head_dim;
     float     *score = a.scores + ((int64_t)seq * a.n_kv_heads + kvh) * a.max_nb;
-    // (a wave's blocks are at most 64: a lane keeps the place of one)
-    const int entry = min(max(a.tables[(int64_t)seq * a.max_blocks + min(begin + lane, end - 1)], 0), a.num_blocks - 1);
+    // (a wave's blocks are at most 128: a lane keeps the place of two)
+    int entry[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        entry[i] = min(max(a.tables[(int64_t)seq * a.max_blocks + min(begin + 64 * i + lane, end - 1)], 0), a.num_blocks - 1);
     for (int h0 = 0; h0 < a.group; h0 += HG) {
         double w[HG][NV][4];
 #pragma unroll
@@ -179,7 +182,8 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
         constexpr int RING = NV < 8 ? 3 : 2; // groups of four blocks: one in work, the others on their way
         float4        x[RING][NV];
         auto   fetch = [&](float4 (&to)[NV], int b0) {
-            const int    pb = __shfl(entry, min(b0 + sub, end - 1) - begin);
+            const int    at = min(b0 + sub, end - 1) - begin, lo = __shfl(entry[0], at & 63), hi = __shfl(entry[1], at & 63);
+            const int    pb = at < 64 ? lo : hi;
             const float *src = a.bounds + ((int64_t)pb * a.n_kv_heads + kvh) * 2 * hd;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
@@ -349,36 +353,61 @@ __global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const 
 }
 
 // The same by the 256 threads of an attention workgroup, for nb <= kHeldBlocks: picks of the selection, ascending, the ones
-// numbered [begin, begin + count) into `mine`; all of them also to `all` where that is not null.
-__device__ __forceinline__ void select_blocks(const SparseArgs &a, const float *score, int nb, int begin, int count, int *mine, int *all)
+// numbered [begin, begin + count) into `mine`, their table entries into `phys`; all of them also to `all` where that is not null.
+__device__ __forceinline__ void select_blocks(const SparseArgs &a, const float *score, const int *table, int nb, int begin, int count, int *mine,
+                                              int *phys, int *all)
 {
     __shared__ __attribute__((aligned(16))) int s_count[4][256];
     __shared__ int s_wave[kSparseWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    unsigned  key[kHeldKeys]; // of blocks 8 tid ..
+    const int per = (nb + 64 * kSparseWaves - 1) / (64 * kSparseWaves), b0 = per * tid; // a thread's blocks: b0 .. b0 + per - 1
+    unsigned  key[kHeldKeys];
 #pragma unroll
     for (int i = 0; i < kHeldKeys; i++)
-        key[i] = kHeldKeys * tid + i < nb ? block_key(a, score, kHeldKeys * tid + i, nb) : 0u;
+        key[i] = i < per && b0 + i < nb ? block_key(a, score, b0 + i, nb) : 0u;
+    int entry[kHeldKeys]; // (the entries of all blocks, while the keys are counted, rather than those of the picks behind it)
+#pragma unroll
+    for (int i = 0; i < kHeldKeys; i++)
+        entry[i] = i < per && b0 + i < nb ? table[b0 + i] : 0;
 #pragma unroll
     for (int i = 0; i < 4; i++)
         s_count[i][tid] = 0;
     __syncthreads();
     unsigned edge = 0;
     int      ties = a.top;
+    // The upper bytes of scores are mostly one or two: counted by the wave, one addition for each.
 #pragma unroll
-    for (int pass = 0; pass < 4; pass++) {
+    for (int i = 0; i < kHeldKeys; i++)
+        if (i < per) {
+            unsigned long long left = __ballot(b0 + i < nb);
+            while (left) {
+                const unsigned           top = (unsigned)__builtin_amdgcn_readlane((int)key[i], __ffsll(left) - 1) >> 24;
+                const unsigned long long same = __ballot((key[i] >> 24) == top) & left;
+                if (lane == 0)
+                    atomicAdd(&s_count[0][top], __popcll(same));
+                left &= ~same & (left - 1); // (the first one is among the same)
+            }
+        }
+    __syncthreads();
+    next_byte(s_count[0], 24, edge, ties);
+#pragma unroll
+    for (int pass = 1; pass < 4; pass++) {
         const int shift = 24 - 8 * pass;
 #pragma unroll
         for (int i = 0; i < kHeldKeys; i++)
-            if (kHeldKeys * tid + i < nb && (pass == 0 || (key[i] >> (shift + 8)) == (edge >> (shift + 8))))
+            if (i < per && b0 + i < nb && (key[i] >> (shift + 8)) == (edge >> (shift + 8)))
                 atomicAdd(&s_count[pass][(key[i] >> shift) & 255u], 1);
         __syncthreads();
         next_byte(s_count[pass], shift, edge, ties);
+        if (s_count[pass][(edge >> shift) & 255u] == ties) { // all of the edge's bin is read: the bytes below do not matter
+            ties = nb;
+            break;
+        }
     }
     int above = 0, even = 0; // up to 2048 of each: one number holds both
 #pragma unroll
     for (int i = 0; i < kHeldKeys; i++) {
-        const bool there = kHeldKeys * tid + i < nb;
+        const bool there = i < per && b0 + i < nb;
         above += there && key[i] > edge, even += there && key[i] == edge;
     }
     const int own = above | even << 16, upto = scan_wave(own);
@@ -392,12 +421,12 @@ __device__ __forceinline__ void select_blocks(const SparseArgs &a, const float *
     int pa = before & 0xffff, pe = before >> 16;
 #pragma unroll
     for (int i = 0; i < kHeldKeys; i++) {
-        const int  b = kHeldKeys * tid + i;
-        const bool hi = b < nb && key[i] > edge, level = b < nb && key[i] == edge;
+        const int  b = b0 + i;
+        const bool there = i < per && b < nb, hi = there && key[i] > edge, level = there && key[i] == edge;
         if (hi || (level && pe < ties)) {
             const int at = pa + min(pe, ties);
             if (at >= begin && at < begin + count)
-                mine[at - begin] = b;
+                mine[at - begin] = b, phys[at - begin] = entry[i];
             if (all)
                 all[at] = b;
         }
@@ -433,10 +462,10 @@ template <int NV, int HG, bool SELECT> __global__ void __launch_bounds__(64 * kS
     if constexpr (SELECT) {
         int *all = chunk == 0 && set == 0 ? chosen : nullptr; // one workgroup tells
         if (nb > a.top)
-            select_blocks(a, a.scores + pair * a.max_nb, nb, begin, count, s_first, all);
+            select_blocks(a, a.scores + pair * a.max_nb, a.tables + (int64_t)seq * a.max_blocks, nb, begin, count, s_first, s_phys, all);
         else {
             if ((int)threadIdx.x < count)
-                s_first[threadIdx.x] = begin + threadIdx.x;
+                s_first[threadIdx.x] = begin + threadIdx.x, s_phys[threadIdx.x] = a.tables[(int64_t)seq * a.max_blocks + begin + threadIdx.x];
             if (all)
                 for (int i = threadIdx.x; i < a.top; i += 64 * kSparseWaves)
                     all[i] = i < nb ? i : -1;
@@ -445,8 +474,9 @@ template <int NV, int HG, bool SELECT> __global__ void __launch_bounds__(64 * kS
     }
     if ((int)threadIdx.x < count) {
         const int b = SELECT ? s_first[threadIdx.x] : min(max(chosen[begin + threadIdx.x], 0), max(nb - 1, 0));
+        const int entry = SELECT ? s_phys[threadIdx.x] : a.tables[(int64_t)seq * a.max_blocks + b];
         s_first[threadIdx.x] = b * bs;
-        s_phys[threadIdx.x]  = min(max(a.tables[(int64_t)seq * a.max_blocks + b], 0), a.num_blocks - 1);
+        s_phys[threadIdx.x]  = min(max(entry, 0), a.num_blocks - 1);
     }
     __syncthreads();
 
@@ -648,10 +678,11 @@ SparseShape sparse_shape(const nvk_block_index *x, int num_seqs, int n_heads, in
     if (x->head_dim > 128) // registers
         s.hg = std::min(s.hg, 2);
     s.head_sets = (int)ceil_div(group, s.hg);
-    // scores: four blocks a wave at least, 64 at most, in between two workgroups for every CU
+    // scores: four blocks a wave at least, 128 at most, in between two workgroups for every CU: one round of the chip.  (16 sequences
+    // of 2048 blocks, eight kv-heads: 47.5 us with 128 blocks a wave, 53.2 in two rounds of 64.)
     const long long lines = (long long)num_seqs * x->n_kv_heads;
     const long long per = lines * s.max_nb / (2LL * kCus * nvk::kSparseWaves);
-    s.blocks_per_wave = (int)std::min(64LL, std::max(4LL, per / 4 * 4));
+    s.blocks_per_wave = (int)std::min(128LL, std::max(4LL, per / 4 * 4));
     s.score_slots     = (int)std::max(1LL, ceil_div(s.max_nb, (long long)s.blocks_per_wave * nvk::kSparseWaves));
     // attention: the chosen blocks are cut while all workgroups still run at once (two fit a CU), into pieces of eight tokens a
     // wave at least and 64 blocks at most

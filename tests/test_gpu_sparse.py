@@ -275,3 +275,24 @@ def test_without_a_list_and_at_any_float():
             with pytest.raises(nv.NvkError):
                 nv.sparse_decode_device(index, 1, 3, H, dq, dt, tabs.shape[1], dc, kw.get("ctx", max(ctx)), 9, 1, 1, kw.get("out", do.data_ptr()))
     st.close()
+
+
+@pytest.mark.parametrize("blocks", [(256, 257, 9, 500), (1025, 600, 40, 1), (2048, 1500, 2047, 513), (2049, 2048, 300, 41)], ids=str)
+@pytest.mark.parametrize("levels", [0, 3])
+def test_selections_of_every_size(blocks, levels):
+    """One to eight blocks a thread and the kernel for more, beside contexts that are read whole; scores of a few levels (many
+    ties) or all different, some of them negative."""
+    KV, hd, bs, H, top = 2, 4, 2, 4, 40
+    ctx = [b * bs - (i % 2) for i, b in enumerate(blocks)]
+    tabs, n = oo.tables_for(ctx, bs, seed=64)
+    rng = np.random.default_rng(65 + levels)
+    held = []
+    with nv.PagedKVPool(2, n, bs, KV, hd) as pool, nv.BlockIndex(pool) as index:
+        for s, c in enumerate(ctx):
+            k = (rng.integers(-levels, levels + 1, (c, KV, hd)) if levels else rng.normal(size=(c, KV, hd))).astype(np.float32)
+            v = rng.normal(size=(c, KV, hd)).astype(np.float32)
+            nv.norm_rope_append(pool, 1, None, None, k, v, tabs, np.arange(c), np.full(c, s))
+            held.append((k, v))
+        index.update(1, tabs, [0] * len(ctx), ctx)
+        for first, last in ((1, 2), (0, 1), (20, 20)):
+            check(pool, index, tabs, held, ctx, H, top, first, last, seed=66)
