@@ -761,27 +761,31 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 
                 a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = w.l[n];
             }
         }
+        // (a lane holds runs of 2 KK channels: a run, or a half of sixteen, is in the row as a whole)
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int ct = 0; ct < 2 * KK; ct++) {
+            for (int ct = 0; ct < 2 * KK; ct += KK == 1 ? 2 : 4) {
                 const int c = (4 * w.g + i) * 2 * KK + ct;
-                if (c < a.mx.head_dim)
-                    dst[c] = w.acc[n][ct][i] * norm;
+                if (c < a.mx.head_dim) {
+                    if constexpr (KK == 1)
+                        dst[c] = w.acc[n][ct][i] * norm, dst[c + 1] = w.acc[n][ct + 1][i] * norm;
+                    else
+                        store_four(dst + c, w.acc[n][ct][i] * norm, w.acc[n][ct + 1][i] * norm, w.acc[n][ct + 2][i] * norm, w.acc[n][ct + 3][i] * norm);
+                }
             }
     }
 }
 
-// a workgroup per (row, head)
-__global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_kernel(const Mx4AttnArgs a)
+// How many chunks the line of a (row, head) has, 0 where nothing is to be joined.
+__device__ __forceinline__ int mx4_line_chunks(const Mx4AttnArgs &a, int64_t line)
 {
-    const int64_t line = blockIdx.x;
-    const int     row = (int)(line / a.n_heads);
-    int           seq = row, rows = 1, row0 = row;
+    const int row = (int)(line / a.n_heads);
+    int       seq = row, rows = 1, row0 = row;
     if (a.row_offsets) { // the sequence whose rows hold this one: offsets[lo] <= row < offsets[hi]
         int lo = 0, hi = a.num_seqs;
         if (row < a.row_offsets[0] || row >= a.row_offsets[a.num_seqs])
-            return;
+            return 0;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (a.row_offsets[mid] <= row)
@@ -793,10 +797,32 @@ __global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_kernel(const Mx4Att
         rows = mx4_rows(a, seq, row0);
     }
     const int ctx = mx4_context(a, seq), limit = max(ctx - rows + (row - row0) + 1, 0);
-    const int n = min(max((limit + a.chunk_tokens - 1) / a.chunk_tokens, 1), a.chunks);
     if (a.whole_lines && min(max((ctx + a.chunk_tokens - 1) / a.chunk_tokens, 1), a.chunks) == 1)
-        return; // (decode writes a sequence of one chunk straight to `out`)
-    join_chunks(a.ws_o + line * a.chunks * a.mx.head_dim, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim, a.out + line * a.mx.head_dim);
+        return 0; // (decode writes a sequence of one chunk straight to `out`)
+    return min(max((limit + a.chunk_tokens - 1) / a.chunk_tokens, 1), a.chunks);
+}
+
+// Many chunks: a workgroup per line.
+__global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_kernel(const Mx4AttnArgs a)
+{
+    const int64_t line = blockIdx.x;
+    const int     n = mx4_line_chunks(a, line);
+    if (n > 0)
+        join_chunks(a.ws_o + line * a.chunks * a.mx.head_dim, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim, a.out + line * a.mx.head_dim);
+}
+
+// Up to kJoinInside chunks (of many lines: a prefill's): a thread per four channels of a line.
+__global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_few_kernel(const Mx4AttnArgs a, unsigned lines)
+{
+    const unsigned quads = a.mx.head_dim >> 2;
+    const int64_t  id = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x, line = id / quads;
+    if (line >= lines)
+        return;
+    const int n = mx4_line_chunks(a, line), c = (int)(id - line * quads) * 4;
+    if (n > 0) {
+        const float4 o = join_few(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim);
+        store_four(a.out + line * a.mx.head_dim + c, o.x, o.y, o.z, o.w);
+    }
 }
 
 } // namespace nvk
@@ -882,7 +908,9 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
     const Mx4Shape  s = mx4_shape(pool, num_seqs, n_heads, total_rows, max_rows, max_ctx);
     const long long units = (long long)num_seqs * s.col_blocks * s.chunks;
     const long long blocks = (s.prefill ? units : (units + 7) / 8 * 8) * pool->n_kv_heads; // (decode: whole rounds of the XCDs)
-    if (!nvk::grid_fits(blocks, 64 * kDecodeWaves) || (s.chunks > 1 && !nvk::grid_fits((long long)total_rows * n_heads, nvk::kJoinThreads)))
+    const long long lines = (long long)total_rows * n_heads, few = (lines * (pool->head_dim / 4) + nvk::kJoinThreads - 1) / nvk::kJoinThreads;
+    if (!nvk::grid_fits(blocks, 64 * kDecodeWaves) || (s.chunks > 1 && !nvk::grid_fits(lines, nvk::kJoinThreads))
+        || (s.chunks > 1 && !nvk::grid_fits(few, nvk::kJoinThreads)))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %lld workgroups", who, blocks);
     int rc = reserve(pool, s, st, who);
     if (rc != NVK_OK)
@@ -906,7 +934,10 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
     }
     NVK_HIP_TRY(hipGetLastError());
     if (s.chunks > 1 && !s.inside) {
-        hipLaunchKernelGGL(nvk::nvk_mx4_join_kernel, dim3((unsigned)(total_rows * n_heads)), dim3(nvk::kJoinThreads), 0, st, a);
+        if (s.chunks <= nvk::kJoinInside)
+            hipLaunchKernelGGL(nvk::nvk_mx4_join_few_kernel, dim3((unsigned)few), dim3(nvk::kJoinThreads), 0, st, a, (unsigned)lines);
+        else
+            hipLaunchKernelGGL(nvk::nvk_mx4_join_kernel, dim3((unsigned)lines), dim3(nvk::kJoinThreads), 0, st, a);
         NVK_HIP_TRY(hipGetLastError());
     }
     return NVK_OK;
