@@ -608,11 +608,9 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
         const int64_t line = (int64_t)(row0 + col / a.group) * a.n_heads + kvh * a.group + col % a.group;
         if (parts > 1) {
             float *dst = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim + c, *ml = a.ws_ml + (line * a.chunks + chunk) * 2;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                store_through(dst + i, o[i]);
+            store_through(dst, o[0], o[1]), store_through(dst + 2, o[2], o[3]);
             if (c == 0)
-                store_through(ml, Mc), store_through(ml + 1, L);
+                store_through(ml, Mc, L);
         }
         else {
             o *= L == 0.f ? 0.f : 1.f / L;
@@ -627,7 +625,7 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
             continue;
         const int64_t line = (int64_t)(row0 + col / a.group) * a.n_heads + kvh * a.group + col % a.group;
         // (a row of a short context was not seen by the later chunks of a longer one: they hold nothing for it)
-        const float4 o = join_few(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, parts, a.mx.head_dim);
+        const float4 o = join_few<true>(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, parts, a.mx.head_dim);
         store_four(a.out + line * a.mx.head_dim + c, o.x, o.y, o.z, o.w);
     }
 }
@@ -820,7 +818,7 @@ __global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_few_kernel(const Mx
         return;
     const int n = mx4_line_chunks(a, line), c = (int)(id - line * quads) * 4;
     if (n > 0) {
-        const float4 o = join_few(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim);
+        const float4 o = join_few<false>(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim);
         store_four(a.out + line * a.mx.head_dim + c, o.x, o.y, o.z, o.w);
     }
 }
@@ -856,7 +854,11 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     // Cut the context while everything still runs at once (workgroups of four waves: so many fit a CU), into chunks of 64
     // tokens at least; not into more than can be joined inside unless those were long.  (One sequence of 777 tokens: 8.05 us
     // in chunks of 256 tokens, 7.45 of 64; 64 x 2048, two workgroups a CU: 28.1 us uncut, 39.6 in two rounds.)
-    const long long fit = (s.pack && pool->kk <= 4 ? 3LL : 2LL) * pool->num_cus;
+    long long fit = (pool->kk == 8 ? 1LL : s.pack ? 3LL : 2LL) * pool->num_cus;
+    // A prompt's early rows see few of the chunks: half as many again where all rows are new.  (1157 rows: 35.6 us in 3 chunks,
+    // 32.2 in 4, 39.6 in 6; 128 rows behind 8064 tokens: 65.3 in 16, 82.4 in 24.)
+    if (s.prefill)
+        fit += fit * std::min(max_rows, max_ctx) / (2LL * std::max(max_ctx, 1));
     s.chunks = (int)std::max(1LL, std::min(fit / std::max(tasks, 1LL), (long long)max_ctx / 64));
     if (!s.prefill && s.chunks > nvk::kJoinInside && max_ctx <= 512 * nvk::kJoinInside)
         s.chunks = nvk::kJoinInside;

@@ -605,9 +605,9 @@ template <int NV, int HG, bool SELECT> __global__ void __launch_bounds__(64 * kS
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < heads * hd; e += 64 * kSparseWaves) {
-        const int h = e / hd, c = e % hd;
-        float     Mh = -INFINITY, L = 0.f, x = 0.f;
+    for (int e = threadIdx.x; e < heads * (hd / 2); e += 64 * kSparseWaves) {
+        const int h = e / (hd / 2), c = e % (hd / 2) * 2;
+        float     Mh = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
         for (int w = 0; w < kSparseWaves; w++)
             Mh = fmaxf(Mh, s_m[w][h]);
@@ -615,25 +615,25 @@ template <int NV, int HG, bool SELECT> __global__ void __launch_bounds__(64 * kS
         for (int w = 0; w < kSparseWaves; w++) {
             const float f = s_m[w][h] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][h] - Mh);
             L += s_l[w][h] * f;
-            x += s_o[w][h][c] * f;
+            x += s_o[w][h][c] * f, y += s_o[w][h][c + 1] * f;
         }
         const int64_t line = (int64_t)seq * a.n_heads + head0 + h;
         if (parts > 1) {
-            store_through(a.ws_o + (line * a.chunks + chunk) * hd + c, x);
-            if (c == 0) {
-                store_through(a.ws_ml + (line * a.chunks + chunk) * 2, Mh);
-                store_through(a.ws_ml + (line * a.chunks + chunk) * 2 + 1, L);
-            }
+            store_through(a.ws_o + (line * a.chunks + chunk) * hd + c, x, y);
+            if (c == 0)
+                store_through(a.ws_ml + (line * a.chunks + chunk) * 2, Mh, L);
         }
-        else
-            a.out[line * hd + c] = L == 0.f ? x : x / L; // (x is 0 then, or no number)
+        else { // (L 0: x and y are 0 then, or no number)
+            a.out[line * hd + c]     = L == 0.f ? x : x / L;
+            a.out[line * hd + c + 1] = L == 0.f ? y : y / L;
+        }
     }
     if (parts == 1 || !a.arrivals || !arrived_last(a.arrivals + ((int64_t)seq * a.head_sets + set) * a.n_kv_heads + kvh, parts))
         return;
     for (int e = threadIdx.x; e < heads * (hd / 4); e += 64 * kSparseWaves) {
         const int64_t line = (int64_t)seq * a.n_heads + head0 + e / (hd / 4);
         const int     c = e % (hd / 4) * 4;
-        const float4  x = join_few(a.ws_o + line * a.chunks * hd + c, a.ws_ml + line * a.chunks * 2, parts, hd);
+        const float4  x = join_few<true>(a.ws_o + line * a.chunks * hd + c, a.ws_ml + line * a.chunks * 2, parts, hd);
         store_four(a.out + line * hd + c, x.x, x.y, x.z, x.w);
     }
 }
