@@ -493,14 +493,15 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
     constexpr int HDP = 32 * KK, COLS = Wave::COLS, W = kDecodeWaves;
     const int     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    // Workgroup -> (sequence, chunk, kv-head); a sequence's columns are one tile.  Consecutive workgroups go to the eight XCDs in turn: the kv-heads
-    // of one piece of context are put side by side on one XCD, which then reads whole blocks of the cache.
-    const unsigned xcd = blockIdx.x % 8u, rest = blockIdx.x / 8u;
-    const int      kvh = (int)(rest % (unsigned)a.mx.n_kv_heads);
-    const unsigned unit = rest / (unsigned)a.mx.n_kv_heads * 8u + xcd;
+    // Workgroup -> (sequence, chunk, kv-head); a sequence's columns are one tile.  Consecutive workgroups go to the eight XCDs in
+    // turn.  Where the pieces of context come out even over the XCDs, the kv-heads of one are put side by side on one XCD, which
+    // then reads whole blocks of the cache (64 x 2048: 3 % less time); elsewhere that would leave an XCD with more
+    // workgroups than there is room for (42 pieces of 6 kv-heads with 256 channels: 29.9 us, 18.6 in plain order).
+    const unsigned n_kv = (unsigned)a.mx.n_kv_heads, pieces = (unsigned)a.num_seqs * (unsigned)a.chunks, rest = blockIdx.x / 8u;
+    const bool     even = pieces % 8u == 0;
+    const int      kvh = (int)((even ? rest : blockIdx.x) % n_kv);
+    const unsigned unit = even ? rest / n_kv * 8u + blockIdx.x % 8u : blockIdx.x / n_kv;
     const int      chunk = (int)(unit % (unsigned)a.chunks), seq = (int)(unit / (unsigned)a.chunks);
-    if (seq >= a.num_seqs)
-        return;
     int       row0;
     const int rows = mx4_rows(a, seq, row0), columns = rows * a.group;
     if (rows <= 0)
@@ -562,13 +563,13 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
             }
         }
     };
-    Mx4Raw<KK> even[2], odd[2]; // in turn: no copies between the steps
+    Mx4Raw<KK> one[2], two[2]; // in turn: no copies between the steps
     if (steps > 0)
-        fetch(even, 0);
+        fetch(one, 0);
     for (int i = 0; i < steps; i += 2) {
-        step(i, even, odd);
+        step(i, one, two);
         if (i + 1 < steps)
-            step(i + 1, odd, even);
+            step(i + 1, two, one);
     }
     w.finish();
 
@@ -851,15 +852,16 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     s.pack    = (long long)max_rows * group <= 4;
     s.col_blocks = s.prefill ? ceil_div((long long)max_rows * group, 16 * prefill_cols(pool->kk) * kPrefillWaves) : 1;
     const long long tasks = (long long)num_seqs * pool->n_kv_heads * s.col_blocks;
-    // Cut the context while everything still runs at once (workgroups of four waves: so many fit a CU), into chunks of 64
-    // tokens at least; not into more than can be joined inside unless those were long.  (One sequence of 777 tokens: 8.05 us
-    // in chunks of 256 tokens, 7.45 of 64; 64 x 2048, two workgroups a CU: 28.1 us uncut, 39.6 in two rounds.)
+    // Cut the context while everything still runs at once (workgroups of four waves: so many fit a CU), into chunks of 192
+    // tokens at least (a step of the four waves is 128; prefill's waves share the tokens: 64); not into more than can be joined
+    // inside unless those were long.  (In chunks of 64, 128, 192, 256 tokens: 1 x 200 7.4, 6.3, 6.3, 6.2 us, 1 x 1000 8.6, 8.6, 8.3,
+    // 9.0, 230 x 256 9.7, 9.7, 7.0, 7.1; 64 x 2048, two workgroups a CU: 28.1 us uncut, 39.6 in two rounds.)
     long long fit = (pool->kk == 8 ? 1LL : s.pack ? 3LL : 2LL) * pool->num_cus;
     // A prompt's early rows see few of the chunks: half as many again where all rows are new.  (1157 rows: 35.6 us in 3 chunks,
     // 32.2 in 4, 39.6 in 6; 128 rows behind 8064 tokens: 65.3 in 16, 82.4 in 24.)
     if (s.prefill)
         fit += fit * std::min(max_rows, max_ctx) / (2LL * std::max(max_ctx, 1));
-    s.chunks = (int)std::max(1LL, std::min(fit / std::max(tasks, 1LL), (long long)max_ctx / 64));
+    s.chunks = (int)std::max(1LL, std::min(fit / std::max(tasks, 1LL), (long long)max_ctx / (s.prefill ? 64 : 192)));
     if (!s.prefill && s.chunks > nvk::kJoinInside && max_ctx <= 512 * nvk::kJoinInside)
         s.chunks = nvk::kJoinInside;
     s.chunk_tokens = std::max(32, ceil_div(ceil_div(max_ctx, s.chunks), 32) * 32);
@@ -909,7 +911,7 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
 {
     const Mx4Shape  s = mx4_shape(pool, num_seqs, n_heads, total_rows, max_rows, max_ctx);
     const long long units = (long long)num_seqs * s.col_blocks * s.chunks;
-    const long long blocks = (s.prefill ? units : (units + 7) / 8 * 8) * pool->n_kv_heads; // (decode: whole rounds of the XCDs)
+    const long long blocks = units * pool->n_kv_heads;
     const long long lines = (long long)total_rows * n_heads, few = (lines * (pool->head_dim / 4) + nvk::kJoinThreads - 1) / nvk::kJoinThreads;
     if (!nvk::grid_fits(blocks, 64 * kDecodeWaves) || (s.chunks > 1 && !nvk::grid_fits(lines, nvk::kJoinThreads))
         || (s.chunks > 1 && !nvk::grid_fits(few, nvk::kJoinThreads)))
