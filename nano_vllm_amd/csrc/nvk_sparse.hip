@@ -438,7 +438,8 @@ __device__ __forceinline__ void select_blocks(const SparseArgs &a, const float *
 // A wave takes eight tokens a step, eight lanes each: a lane holds NV float4s of the row (lane 8 apart: whole lines per
 // token), dots them with HG query heads, and keeps maximum, sum and output of its own eight-lane group -- nothing
 // crosses the groups before the end.  Bound by the keys and values it reads.
-template <int NV, int HG, bool SELECT> __global__ void __launch_bounds__(64 * kSparseWaves) nvk_sparse_attn_kernel(const SparseArgs a)
+template <int NV, int HG, bool SELECT>
+__global__ void __launch_bounds__(64 * kSparseWaves, NV == 1 ? 4 : NV <= 4 || HG == 1 ? 2 : 1) nvk_sparse_attn_kernel(const SparseArgs a)
 {
     constexpr int kMostBlocks = 64; // of a chunk
     __shared__ int   s_phys[kMostBlocks], s_first[kMostBlocks];
@@ -511,18 +512,16 @@ template <int NV, int HG, bool SELECT> __global__ void __launch_bounds__(64 * kS
         }
         return there;
     };
-    float4 kn[NV], vn[NV];
-    bool   next_there = false;
-    if (wave < steps)
-        next_there = fetch(wave, kn, vn);
-    for (int step = wave; step < steps; step += kSparseWaves) {
-        float4 k[NV], v[NV];
+    constexpr int AHEAD = NV == 1 ? 4 : 1; // steps on their way: of narrow rows more
+    float4        kn[AHEAD][NV], vn[AHEAD][NV];
+    bool          next_there[AHEAD];
 #pragma unroll
-        for (int j = 0; j < NV; j++)
-            k[j] = kn[j], v[j] = vn[j];
-        const bool there = next_there;
-        if (step + kSparseWaves < steps)
-            next_there = fetch(step + kSparseWaves, kn, vn);
+    for (int d = 0; d < AHEAD; d++) {
+        next_there[d] = false;
+        if (wave + d * kSparseWaves < steps)
+            next_there[d] = fetch(wave + d * kSparseWaves, kn[d], vn[d]);
+    }
+    auto work = [&](const float4 (&k)[NV], const float4 (&v)[NV], const bool there) {
         float s[HG];
 #pragma unroll
         for (int h = 0; h < HG; h++) {
@@ -578,7 +577,20 @@ template <int NV, int HG, bool SELECT> __global__ void __launch_bounds__(64 * kS
                 o[h][j].z = fmaf(x, v[j].z, o[h][j].z), o[h][j].w = fmaf(x, v[j].w, o[h][j].w);
             }
         }
-    }
+    };
+    for (int step = wave; step < steps; step += AHEAD * kSparseWaves)
+#pragma unroll
+        for (int d = 0; d < AHEAD; d++)
+            if (d == 0 || step + d * kSparseWaves < steps) {
+                float4 k[NV], v[NV];
+#pragma unroll
+                for (int j = 0; j < NV; j++)
+                    k[j] = kn[d][j], v[j] = vn[d][j];
+                const bool there = next_there[d];
+                if (step + (d + AHEAD) * kSparseWaves < steps)
+                    next_there[d] = fetch(step + (d + AHEAD) * kSparseWaves, kn[d], vn[d]);
+                work(k, v, there);
+            }
 
     // the eight groups of the wave, then the waves
     float M = m;
@@ -684,11 +696,14 @@ SparseShape sparse_shape(const nvk_block_index *x, int num_seqs, int n_heads, in
     const long long per = lines * s.max_nb / (2LL * kCus * nvk::kSparseWaves);
     s.blocks_per_wave = (int)std::min(128LL, std::max(4LL, per / 4 * 4));
     s.score_slots     = (int)std::max(1LL, ceil_div(s.max_nb, (long long)s.blocks_per_wave * nvk::kSparseWaves));
-    // attention: the chosen blocks are cut while all workgroups still run at once (two fit a CU), into pieces of eight tokens a
-    // wave at least and 64 blocks at most
+    // attention: the chosen blocks are cut while all workgroups still run at once (two fit a CU, of narrow rows four, of the widest
+    // one), into pieces of eight tokens a wave at least and 64 blocks at most.  Four would fit with 64 channels too, but each
+    // selects for itself.  (32 channels, 166 and 500 blocks: 34 and 46 us with four, 44 and 51 with two; 64 channels, 500 blocks: 31.7
+    // and 27.6; 256 channels, heads by two: 84 us with one, 97 with two.)
     const int       n = std::max(1, std::min(s.max_nb, top));
     const long long tasks = lines * s.head_sets;
-    const long long fit = std::max(1LL, 2LL * kCus / std::max(tasks, 1LL));
+    const int       per_cu = x->head_dim <= 32 ? 4 : x->head_dim <= 128 || s.hg == 1 ? 2 : 1;
+    const long long fit = std::max(1LL, (long long)per_cu * kCus / std::max(tasks, 1LL));
     const long long least = ceil_div(8LL * nvk::kSparseWaves, x->block_size);
     s.blocks_per_chunk = (int)std::min(64LL, std::max(least, ceil_div(n, fit)));
     // (rather sixteen pieces, which the kernel joins itself, than more short ones)
