@@ -358,8 +358,9 @@ template <bool MX4> void launch_rotary(const RotaryArgs &a, int rows, hipStream_
     const int hb = pairs > 64 ? 2 : 4 * (64 / w);
     const int batches = (a.k ? 2 * ((a.mx.n_kv_heads + hb - 1) / hb) : 0) + (a.q ? (a.n_heads + hb - 1) / hb : 0);
     // Few rows: a row's batches are spread over several waves, one each at most, while there are no more than sixteen waves for
-    // every CU.  (3001 rows of three batches: 10.6 us a wave a row, 12.9 two, 13.9 three; 256 rows of twelve: 7.9 us.)
-    const int  parts = (int)std::max(1LL, std::min((long long)batches, 16LL * kCus / rows));
+    // every CU; up to 32 where three are left to each, which pays for its angles.  (3001 rows of three batches: 10.6 us a wave a
+    // row, 12.9 two, 13.9 three; 256 rows of twelve: 7.9 us; 2111 rows of nine: 20.0 us a wave a row, 16.2 three.)
+    const int  parts = (int)std::max({1LL, std::min((long long)batches, 16LL * kCus / rows), std::min(batches / 3LL, 32LL * kCus / rows)});
     const dim3 grid((unsigned)(((long long)rows * parts + nvk::kRotaryWaves - 1) / nvk::kRotaryWaves)), block(64 * nvk::kRotaryWaves);
     if (pairs > 64)
         hipLaunchKernelGGL((nvk::nvk_norm_rope_append_kernel<64, 2, MX4>), grid, block, 0, st, a, rows, parts);
