@@ -56,7 +56,8 @@ struct SparseArgs
     int         *arrivals; // one for each (sequence, set of heads, kv-head), or null: the join kernel follows
 };
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float  f32x4 __attribute__((ext_vector_type(4)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // rows of keys, values and bounds are read once by a launch: not worth keeping in the caches
 __device__ __forceinline__ float4 load_once(const float *p)
@@ -243,6 +244,93 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
                         fetch(x[(d + RING - 1) % RING], b0 + 4 * (d + RING - 1));
                     take(x[d], b0 + 4 * d);
                 }
+        }
+    }
+}
+
+// The same for groups of more than four heads, on fp64 matrix instructions: heads are the rows, sixteen blocks the columns of a
+// product, so that the bounds are read once for sixteen heads.  The order of a contraction is free: a lane holds four
+// neighbouring bounds of its block, and the weights are laid out to match.  An instruction reads half a line of each block, so the
+// loads go through the caches (past them 4 % more time).  (Whole calls, this kernel and the one above in two passes: 16 x 32768, 8
+// kv-heads of 8 heads and 128 channels 150 and 167 us; 30 x 9000, 4 of 7 and 64 channels 32 and 46; 4 of 5 and 32 channels 25 and 36.)
+template <int NV>
+__global__ void __launch_bounds__(64 * kSparseWaves, NV == 4 ? 1 : 2) nvk_block_score_wide_kernel(const SparseArgs a, int slots)
+{
+    constexpr int J = 4 * NV; // float4s of [lo | hi] per lane
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    unsigned  id = blockIdx.x;
+    const int kvh = (int)(id % (unsigned)a.n_kv_heads);
+    id /= (unsigned)a.n_kv_heads;
+    const int slot = (int)(id % (unsigned)slots), seq = (int)(id / (unsigned)slots);
+    const int ctx = context_of(a, seq), nb = (ctx + a.block_size - 1) / a.block_size;
+    const int begin = (slot * kSparseWaves + wave) * a.blocks_per_wave, end = min(begin + a.blocks_per_wave, nb);
+    if (nb <= a.top || begin >= end) // everything is read: no scores needed
+        return;
+    const int hd = a.head_dim;
+    float    *score = a.scores + ((int64_t)seq * a.n_kv_heads + kvh) * a.max_nb;
+    int       entry[2]; // (a wave's blocks are at most 128)
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        entry[i] = min(max(a.tables[(int64_t)seq * a.max_blocks + min(begin + 64 * i + lane, end - 1)], 0), a.num_blocks - 1);
+    const int tiles = (end - begin + 15) / 16;
+    for (int h0 = 0; h0 < a.group; h0 += 16) {
+        double w[J][4];
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const int c = 16 * j + 4 * g; // place in [lo | hi]
+            float4    x = make_float4(0.f, 0.f, 0.f, 0.f);
+            // (a set that ends beyond the group repeats its last head: the maximum is the same)
+            if (c < 2 * hd)
+                x = *reinterpret_cast<const float4 *>(
+                    a.q + ((int64_t)seq * a.n_heads + kvh * a.group + min(h0 + l16, a.group - 1)) * hd + (c < hd ? c : c - hd));
+            const bool low = c < hd;
+            w[j][0] = low ? fminf(x.x, 0.f) : fmaxf(x.x, 0.f), w[j][1] = low ? fminf(x.y, 0.f) : fmaxf(x.y, 0.f);
+            w[j][2] = low ? fminf(x.z, 0.f) : fmaxf(x.z, 0.f), w[j][3] = low ? fminf(x.w, 0.f) : fmaxf(x.w, 0.f);
+        }
+        auto fetch = [&](float4 (&to)[J], int t) {
+            const int    at = min(16 * t + l16, end - 1 - begin), lo = __shfl(entry[0], at & 63), hi = __shfl(entry[1], at & 63);
+            const float *src = a.bounds + ((int64_t)(at < 64 ? lo : hi) * a.n_kv_heads + kvh) * 2 * hd;
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const int c = 16 * j + 4 * g;
+                to[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c < 2 * hd)
+                    to[j] = *reinterpret_cast<const float4 *>(src + c);
+            }
+        };
+        // (no branch between the products and what reads them: the compiler does not keep the wait for a result across one)
+        auto take = [&](const float4 (&x)[J], int t) {
+            f64x4 s0 = {0.0, 0.0, 0.0, 0.0}, s1 = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                s0 = __builtin_amdgcn_mfma_f64_16x16x4f64(w[j][0], (double)x[j].x, s0, 0, 0, 0);
+                s1 = __builtin_amdgcn_mfma_f64_16x16x4f64(w[j][1], (double)x[j].y, s1, 0, 0, 0);
+                s0 = __builtin_amdgcn_mfma_f64_16x16x4f64(w[j][2], (double)x[j].z, s0, 0, 0, 0);
+                s1 = __builtin_amdgcn_mfma_f64_16x16x4f64(w[j][3], (double)x[j].w, s1, 0, 0, 0);
+            }
+            float best = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float r = (float)(s0[i] + s1[i]);
+                best = fmaxf(best, r != r ? INFINITY : r); // no number: as high as can be
+            }
+            best = fmaxf(best, __shfl_xor(best, 16));
+            best = fmaxf(best, __shfl_xor(best, 32));
+            const int b = begin + 16 * t + l16;
+            if (g == 0 && b < end)
+                score[b] = h0 > 0 ? fmaxf(score[b], best) : best;
+        };
+        float4 one[J], two[J]; // in turn
+        fetch(one, 0);
+        for (int t = 0; t < tiles; t += 2) {
+            if (t + 1 < tiles)
+                fetch(two, t + 1);
+            take(one, t);
+            if (t + 1 < tiles) {
+                if (t + 2 < tiles)
+                    fetch(one, t + 2);
+                take(two, t + 1);
+            }
         }
     }
 }
@@ -674,6 +762,7 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 struct SparseShape
 {
     int    max_nb = 0, blocks_per_wave = 4, score_slots = 1, blocks_per_chunk = 1, chunks = 1, head_sets = 1, hg = 1;
+    bool   wide = false; // scores on matrix instructions
     bool   inside = false, select_inside = false; // the attention kernel joins the chunks itself, selects itself
     size_t score_floats = 0, chosen_ints = 0, part_floats = 0, arrivals = 0;
     size_t floats() const { return score_floats + chosen_ints + part_floats; }
@@ -693,8 +782,9 @@ SparseShape sparse_shape(const nvk_block_index *x, int num_seqs, int n_heads, in
     // scores: four blocks a wave at least, 128 at most, in between two workgroups for every CU: one round of the chip.  (16 sequences
     // of 2048 blocks, eight kv-heads: 47.5 us with 128 blocks a wave, 53.2 in two rounds of 64.)
     const long long lines = (long long)num_seqs * x->n_kv_heads;
-    const long long per = lines * s.max_nb / (2LL * kCus * nvk::kSparseWaves);
-    s.blocks_per_wave = (int)std::min(128LL, std::max(4LL, per / 4 * 4));
+    s.wide = group > 4 && x->head_dim <= 128;
+    const long long per = lines * s.max_nb / ((s.wide && x->head_dim > 64 ? 1LL : 2LL) * kCus * nvk::kSparseWaves), unit = s.wide ? 16 : 4;
+    s.blocks_per_wave = (int)std::min(128LL, std::max(unit, per / unit * unit));
     s.score_slots     = (int)std::max(1LL, ceil_div(s.max_nb, (long long)s.blocks_per_wave * nvk::kSparseWaves));
     // attention: the chosen blocks are cut while all workgroups still run at once (two fit a CU, of narrow rows four, of the widest
     // one), into pieces of eight tokens a wave at least and 64 blocks at most.  Four would fit with 64 channels too, but each
@@ -729,9 +819,12 @@ int reserve(nvk_block_index *x, const SparseShape &s, hipStream_t st, const char
 template <int NV, int HG> void launch_sparse(const SparseArgs &a, const SparseShape &s, bool score, hipStream_t st)
 {
     const unsigned lines = (unsigned)a.num_seqs * (unsigned)a.n_kv_heads;
-    if (score)
-        hipLaunchKernelGGL((nvk::nvk_block_score_kernel<NV, HG>), dim3(lines * (unsigned)s.score_slots), dim3(64 * nvk::kSparseWaves), 0,
-                           st, a, s.score_slots);
+    const dim3 scores(lines * (unsigned)s.score_slots), threads(64 * nvk::kSparseWaves);
+    if constexpr (NV < 8 && HG == 4)
+        if (score && s.wide)
+            hipLaunchKernelGGL((nvk::nvk_block_score_wide_kernel<NV>), scores, threads, 0, st, a, s.score_slots);
+    if (score && !s.wide)
+        hipLaunchKernelGGL((nvk::nvk_block_score_kernel<NV, HG>), scores, threads, 0, st, a, s.score_slots);
     const dim3 grid(lines * (unsigned)s.head_sets * (unsigned)s.chunks), block(64 * nvk::kSparseWaves);
     if (s.select_inside)
         hipLaunchKernelGGL((nvk::nvk_sparse_attn_kernel<NV, HG, true>), grid, block, 0, st, a);

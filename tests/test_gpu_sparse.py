@@ -296,3 +296,25 @@ def test_selections_of_every_size(blocks, levels):
         index.update(1, tabs, [0] * len(ctx), ctx)
         for first, last in ((1, 2), (0, 1), (20, 20)):
             check(pool, index, tabs, held, ctx, H, top, first, last, seed=66)
+
+
+@pytest.mark.parametrize("geom", [(16, 2, 128, 16), (10, 2, 64, 4), (7, 1, 32, 2), (21, 1, 36, 3), (40, 1, 128, 2), (9, 1, 80, 8), (12, 2, 4, 1)],
+                         ids=lambda g: "x".join(map(str, g)))
+def test_large_groups(geom):
+    """Groups of 5 to 40 heads: bounds on matrix instructions, sixteen heads and blocks at a time, more blocks than a wave takes;
+    a block whose keys hold an infinity counts as highest."""
+    H, KV, hd, bs = geom
+    ctx = [700 * bs - 1, 17 * bs, 16 * bs + 1, 0, 131 * bs]
+    pool, tabs, held = filled(ctx, bs, KV, hd, seed=hd + H)
+    with pool, nv.BlockIndex(pool) as index:
+        index.update(1, tabs, [0] * len(ctx), ctx)
+        for top, first, last in ((9, 1, 2), (16, 0, 1)):
+            check(pool, index, tabs, held, ctx, H, top, first, last, seed=top)
+        k = held[0][0][:500 * bs].copy()
+        k[300 * bs, 0, 1] = np.inf
+        k[310 * bs, 0, 2] = np.nan
+        nv.norm_rope_append(pool, 1, None, None, k, held[0][1][:500 * bs], tabs, np.arange(500 * bs), np.zeros(500 * bs, np.int32))
+        index.update(1, tabs[:1], [0], [500 * bs])
+        q = np.abs(np.random.default_rng(1).normal(size=(1, H, hd))).astype(np.float32)
+        _, sel = nv.sparse_decode(index, 1, q, tabs[:1], [500 * bs], 4, 0, 1)
+        assert {300, 310, 499} <= set(sel[0, 0].tolist())
