@@ -46,7 +46,8 @@ struct SparseArgs
     int          num_seqs, max_blocks, n_heads, group, n_kv_heads, head_dim, num_blocks, block_size;
     int          top, first, last;
     float       *scores; // [num_seqs, n_kv_heads, max_nb]
-    int         *chosen; // [num_seqs, n_kv_heads, top]; may be null where the attention kernel selects
+    int         *chosen;   // [num_seqs, n_kv_heads, top]: what the selection kernel makes, of lines with more blocks than `top`
+    int         *selected; // the caller's list of the same shape, of all lines, or null
     int          max_nb; // blocks of the longest context
     int          blocks_per_wave;          // score
     int          blocks_per_chunk, chunks; // attend
@@ -336,9 +337,11 @@ __global__ void __launch_bounds__(64 * kSparseWaves, NV == 4 ? 1 : 2) nvk_block_
 }
 
 // ---- selection --------------------------------------------------------------------------------------------------------
-// The key of the last block that is read is found by four counting passes over the bytes of the keys; read are the blocks above
-// it, and as many of those level with it as are left, lowest first, in ascending order.  Where a workgroup can keep all keys
-// (2048 blocks, eight a thread) every workgroup of the attention kernel selects for itself; beyond that a kernel of its own does.
+// The key of the last block that is read is found by counting passes over the four bytes of the keys; read are the blocks above
+// it, and as many of those level with it as are left, lowest first, in ascending order.  Where the 256 threads of an attention
+// workgroup can keep all keys (2048 blocks, eight each) every one of them selects for itself (1 x 8192: 18.8 us, with a launch for
+// the selection 23.6; 16 x 32768: 104.5 and 108).  Beyond that a kernel of its own does, with keys in registers up to 32768 blocks
+// (1 x 131072: 42.5 us, 57.7 with keys made again for every pass).  Bound by latency: counting in LDS between barriers.
 constexpr int kHeldKeys  = 8;
 constexpr int kHeldBlocks = 64 * kSparseWaves * kHeldKeys;
 
@@ -383,8 +386,95 @@ __device__ __forceinline__ void next_byte(const int *count, int shift, unsigned 
     left = __builtin_amdgcn_readlane(rest, from);
 }
 
+// The selection by a workgroup of WAVES waves that keep KEYS keys a thread: take(at, block, i) for each block that is read, `at` its
+// place in ascending order, i the number among the thread's blocks, which are first .. first + share - 1.
+template <int WAVES, int KEYS> struct HeldSelection
+{
+    int      first, share;
+    unsigned key[KEYS];
+    __device__ __forceinline__ bool there(int i, int nb) const { return i < share && first + i < nb; }
+    __device__ __forceinline__ HeldSelection(const SparseArgs &a, const float *score, int nb)
+    {
+        share = (nb + 64 * WAVES - 1) / (64 * WAVES), first = share * (int)threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < KEYS; i++)
+            key[i] = there(i, nb) ? block_key(a, score, first + i, nb) : 0u;
+    }
+    template <class F> __device__ __forceinline__ void run(int top, int nb, F &&take)
+    {
+        __shared__ __attribute__((aligned(16))) int s_count[4][256];
+        __shared__ int s_wave[2][WAVES];
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        for (int i = tid; i < 4 * 256; i += 64 * WAVES)
+            s_count[i >> 8][i & 255] = 0;
+        __syncthreads();
+        unsigned edge = 0;
+        int      ties = top;
+        // The upper bytes of scores are mostly one or two: counted by the wave, one addition for each.
+#pragma unroll
+        for (int i = 0; i < KEYS; i++)
+            if (i < share) {
+                unsigned long long left = __ballot(first + i < nb);
+                while (left) {
+                    const unsigned           top_byte = (unsigned)__builtin_amdgcn_readlane((int)key[i], __ffsll(left) - 1) >> 24;
+                    const unsigned long long same = __ballot((key[i] >> 24) == top_byte) & left;
+                    if (lane == 0)
+                        atomicAdd(&s_count[0][top_byte], __popcll(same));
+                    left &= ~same & (left - 1); // (the first one is among the same)
+                }
+            }
+        __syncthreads();
+        next_byte(s_count[0], 24, edge, ties);
+#pragma unroll
+        for (int pass = 1; pass < 4; pass++) {
+            const int shift = 24 - 8 * pass;
+#pragma unroll
+            for (int i = 0; i < KEYS; i++)
+                if (there(i, nb) && (key[i] >> (shift + 8)) == (edge >> (shift + 8)))
+                    atomicAdd(&s_count[pass][(key[i] >> shift) & 255u], 1);
+            __syncthreads();
+            next_byte(s_count[pass], shift, edge, ties);
+            if (s_count[pass][(edge >> shift) & 255u] == ties) { // all of the edge's bin is read: the bytes below do not matter
+                ties = nb;
+                break;
+            }
+        }
+        int above = 0, even = 0;
+#pragma unroll
+        for (int i = 0; i < KEYS; i++)
+            above += there(i, nb) && key[i] > edge, even += there(i, nb) && key[i] == edge;
+        int pa = scan_wave(above), pe = scan_wave(even);
+        if (lane == 63)
+            s_wave[0][wave] = pa, s_wave[1][wave] = pe;
+        __syncthreads();
+        pa -= above, pe -= even;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++)
+            pa += w < wave ? s_wave[0][w] : 0, pe += w < wave ? s_wave[1][w] : 0;
+#pragma unroll
+        for (int i = 0; i < KEYS; i++) {
+            const bool hi = there(i, nb) && key[i] > edge, level = there(i, nb) && key[i] == edge;
+            if (hi || (level && pe < ties))
+                take(pa + min(pe, ties), first + i, i);
+            pa += hi, pe += level;
+        }
+    }
+};
+
 constexpr int kSelectThreads = 1024;
 
+// a workgroup per (sequence, kv-head)
+template <int KEYS> __global__ void __launch_bounds__(kSelectThreads) nvk_block_select_held_kernel(const SparseArgs a)
+{
+    const int line = blockIdx.x, ctx = context_of(a, line / a.n_kv_heads), nb = (ctx + a.block_size - 1) / a.block_size;
+    if (nb <= a.top)
+        return;
+    int *chosen = a.chosen + (int64_t)line * a.top;
+    HeldSelection<kSelectThreads / 64, KEYS> held(a, a.scores + (int64_t)line * a.max_nb, nb);
+    held.run(a.top, nb, [&](int at, int b, int) { chosen[at] = b; });
+}
+
+// the same for any number of blocks, whose keys are made again for every pass
 __global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const SparseArgs a)
 {
     constexpr int W = kSelectThreads / 64;
@@ -395,11 +485,8 @@ __global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const 
     const int    ctx = context_of(a, seq), nb = (ctx + a.block_size - 1) / a.block_size;
     int         *chosen = a.chosen + (int64_t)line * a.top;
     const float *score = a.scores + (int64_t)line * a.max_nb;
-    if (nb <= a.top) {
-        for (int i = tid; i < a.top; i += kSelectThreads)
-            chosen[i] = i < nb ? i : -1;
+    if (nb <= a.top)
         return;
-    }
     s_count[tid >> 8][tid & 255] = 0;
     __syncthreads();
     unsigned edge = 0;
@@ -440,88 +527,6 @@ __global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const 
     }
 }
 
-// The same by the 256 threads of an attention workgroup, for nb <= kHeldBlocks: picks of the selection, ascending, the ones
-// numbered [begin, begin + count) into `mine`, their table entries into `phys`; all of them also to `all` where that is not null.
-__device__ __forceinline__ void select_blocks(const SparseArgs &a, const float *score, const int *table, int nb, int begin, int count, int *mine,
-                                              int *phys, int *all)
-{
-    __shared__ __attribute__((aligned(16))) int s_count[4][256];
-    __shared__ int s_wave[kSparseWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (nb + 64 * kSparseWaves - 1) / (64 * kSparseWaves), b0 = per * tid; // a thread's blocks: b0 .. b0 + per - 1
-    unsigned  key[kHeldKeys];
-#pragma unroll
-    for (int i = 0; i < kHeldKeys; i++)
-        key[i] = i < per && b0 + i < nb ? block_key(a, score, b0 + i, nb) : 0u;
-    int entry[kHeldKeys]; // (the entries of all blocks, while the keys are counted, rather than those of the picks behind it)
-#pragma unroll
-    for (int i = 0; i < kHeldKeys; i++)
-        entry[i] = i < per && b0 + i < nb ? table[b0 + i] : 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        s_count[i][tid] = 0;
-    __syncthreads();
-    unsigned edge = 0;
-    int      ties = a.top;
-    // The upper bytes of scores are mostly one or two: counted by the wave, one addition for each.
-#pragma unroll
-    for (int i = 0; i < kHeldKeys; i++)
-        if (i < per) {
-            unsigned long long left = __ballot(b0 + i < nb);
-            while (left) {
-                const unsigned           top = (unsigned)__builtin_amdgcn_readlane((int)key[i], __ffsll(left) - 1) >> 24;
-                const unsigned long long same = __ballot((key[i] >> 24) == top) & left;
-                if (lane == 0)
-                    atomicAdd(&s_count[0][top], __popcll(same));
-                left &= ~same & (left - 1); // (the first one is among the same)
-            }
-        }
-    __syncthreads();
-    next_byte(s_count[0], 24, edge, ties);
-#pragma unroll
-    for (int pass = 1; pass < 4; pass++) {
-        const int shift = 24 - 8 * pass;
-#pragma unroll
-        for (int i = 0; i < kHeldKeys; i++)
-            if (i < per && b0 + i < nb && (key[i] >> (shift + 8)) == (edge >> (shift + 8)))
-                atomicAdd(&s_count[pass][(key[i] >> shift) & 255u], 1);
-        __syncthreads();
-        next_byte(s_count[pass], shift, edge, ties);
-        if (s_count[pass][(edge >> shift) & 255u] == ties) { // all of the edge's bin is read: the bytes below do not matter
-            ties = nb;
-            break;
-        }
-    }
-    int above = 0, even = 0; // up to 2048 of each: one number holds both
-#pragma unroll
-    for (int i = 0; i < kHeldKeys; i++) {
-        const bool there = i < per && b0 + i < nb;
-        above += there && key[i] > edge, even += there && key[i] == edge;
-    }
-    const int own = above | even << 16, upto = scan_wave(own);
-    if (lane == 63)
-        s_wave[wave] = upto;
-    __syncthreads();
-    int before = upto - own;
-#pragma unroll
-    for (int w = 0; w < kSparseWaves; w++)
-        before += w < wave ? s_wave[w] : 0;
-    int pa = before & 0xffff, pe = before >> 16;
-#pragma unroll
-    for (int i = 0; i < kHeldKeys; i++) {
-        const int  b = b0 + i;
-        const bool there = i < per && b < nb, hi = there && key[i] > edge, level = there && key[i] == edge;
-        if (hi || (level && pe < ties)) {
-            const int at = pa + min(pe, ties);
-            if (at >= begin && at < begin + count)
-                mine[at - begin] = b, phys[at - begin] = entry[i];
-            if (all)
-                all[at] = b;
-        }
-        pa += hi, pe += level;
-    }
-}
-
 // ---- attention over the chosen blocks -----------------------------------------------------------------------------------
 // A wave takes eight tokens a step, eight lanes each: a lane holds NV float4s of the row (lane 8 apart: whole lines per
 // token), dots them with HG query heads, and keeps maximum, sum and output of its own eight-lane group -- nothing
@@ -547,26 +552,35 @@ __global__ void __launch_bounds__(64 * kSparseWaves, NV == 1 ? 4 : NV <= 4 || HG
     if (chunk >= parts)
         return;
     const int64_t pair = (int64_t)seq * a.n_kv_heads + kvh;
-    int          *chosen = a.chosen ? a.chosen + pair * a.top : nullptr;
-    if constexpr (SELECT) {
-        int *all = chunk == 0 && set == 0 ? chosen : nullptr; // one workgroup tells
-        if (nb > a.top)
-            select_blocks(a, a.scores + pair * a.max_nb, a.tables + (int64_t)seq * a.max_blocks, nb, begin, count, s_first, s_phys, all);
-        else {
-            if ((int)threadIdx.x < count)
-                s_first[threadIdx.x] = begin + threadIdx.x, s_phys[threadIdx.x] = a.tables[(int64_t)seq * a.max_blocks + begin + threadIdx.x];
-            if (all)
-                for (int i = threadIdx.x; i < a.top; i += 64 * kSparseWaves)
-                    all[i] = i < nb ? i : -1;
-        }
-        __syncthreads();
+    const int    *table = a.tables + (int64_t)seq * a.max_blocks;
+    int          *selected = a.selected && chunk == 0 && set == 0 ? a.selected + pair * a.top : nullptr; // one workgroup tells
+    if (nb <= a.top) { // everything is read
+        if ((int)threadIdx.x < count)
+            s_first[threadIdx.x] = begin + threadIdx.x, s_phys[threadIdx.x] = table[begin + threadIdx.x];
+        if (selected)
+            for (int i = threadIdx.x; i < a.top; i += 64 * kSparseWaves)
+                selected[i] = i < nb ? i : -1;
     }
-    if ((int)threadIdx.x < count) {
-        const int b = SELECT ? s_first[threadIdx.x] : min(max(chosen[begin + threadIdx.x], 0), max(nb - 1, 0));
-        const int entry = SELECT ? s_phys[threadIdx.x] : a.tables[(int64_t)seq * a.max_blocks + b];
-        s_first[threadIdx.x] = b * bs;
-        s_phys[threadIdx.x]  = min(max(entry, 0), a.num_blocks - 1);
+    else if constexpr (SELECT) {
+        HeldSelection<kSparseWaves, kHeldKeys> held(a, a.scores + pair * a.max_nb, nb);
+        int entry[kHeldKeys]; // (of all the thread's blocks, while the keys are counted, rather than of the picks behind it)
+#pragma unroll
+        for (int i = 0; i < kHeldKeys; i++)
+            entry[i] = held.there(i, nb) ? table[held.first + i] : 0;
+        held.run(a.top, nb, [&](int at, int b, int i) {
+            if (at >= begin && at < begin + count)
+                s_first[at - begin] = b, s_phys[at - begin] = entry[i];
+            if (selected)
+                selected[at] = b;
+        });
     }
+    else if ((int)threadIdx.x < count) { // (the list is the selection kernel's)
+        const int b = min(max(a.chosen[pair * a.top + begin + threadIdx.x], 0), nb - 1);
+        s_first[threadIdx.x] = b, s_phys[threadIdx.x] = table[b];
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < count)
+        s_first[threadIdx.x] *= bs, s_phys[threadIdx.x] = min(max(s_phys[threadIdx.x], 0), a.num_blocks - 1);
     __syncthreads();
 
     const int head0 = kvh * a.group + set * HG, heads = min(HG, a.group - set * HG);
@@ -803,7 +817,7 @@ SparseShape sparse_shape(const nvk_block_index *x, int num_seqs, int n_heads, in
     s.chunks           = (int)ceil_div(n, s.blocks_per_chunk);
     s.score_floats     = s.max_nb > top ? to_line((size_t)lines * s.max_nb) : 0;
     s.select_inside    = s.max_nb <= nvk::kHeldBlocks;
-    s.chosen_ints      = s.select_inside ? 0 : to_line((size_t)lines * top);
+    s.chosen_ints      = s.select_inside || s.max_nb <= top ? 0 : to_line((size_t)lines * top);
     s.inside           = s.chunks > 1 && s.chunks <= nvk::kJoinInside;
     s.arrivals         = s.inside ? (size_t)tasks : 0;
     s.part_floats      = s.chunks > 1 ? (size_t)num_seqs * n_heads * s.chunks * (x->head_dim + 2) : 0;
@@ -829,7 +843,15 @@ template <int NV, int HG> void launch_sparse(const SparseArgs &a, const SparseSh
     if (s.select_inside)
         hipLaunchKernelGGL((nvk::nvk_sparse_attn_kernel<NV, HG, true>), grid, block, 0, st, a);
     else {
-        hipLaunchKernelGGL(nvk::nvk_block_select_kernel, dim3(lines), dim3(nvk::kSelectThreads), 0, st, a);
+        if (score) { // (4 x 4096 blocks: 56.5 us with 16 keys a thread, 63.0 with 32; 18750 blocks: 43.3 with 32, 79.4 with none)
+            const dim3 all(nvk::kSelectThreads);
+            if (s.max_nb <= 16 * nvk::kSelectThreads)
+                hipLaunchKernelGGL(nvk::nvk_block_select_held_kernel<16>, dim3(lines), all, 0, st, a);
+            else if (s.max_nb <= 32 * nvk::kSelectThreads)
+                hipLaunchKernelGGL(nvk::nvk_block_select_held_kernel<32>, dim3(lines), all, 0, st, a);
+            else
+                hipLaunchKernelGGL(nvk::nvk_block_select_kernel, dim3(lines), all, 0, st, a);
+        }
         hipLaunchKernelGGL((nvk::nvk_sparse_attn_kernel<NV, HG, false>), grid, block, 0, st, a);
     }
 }
@@ -938,7 +960,7 @@ int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, con
     a.max_nb = s.max_nb, a.blocks_per_wave = s.blocks_per_wave, a.blocks_per_chunk = s.blocks_per_chunk, a.chunks = s.chunks;
     a.head_sets = s.head_sets, a.scale_log2e = (float)(1.4426950408889634 / std::sqrt((double)x->head_dim));
     a.scores = x->ws;
-    a.chosen = selected || s.select_inside ? selected : (int *)(x->ws + s.score_floats);
+    a.selected = selected, a.chosen = selected ? selected : (int *)(x->ws + s.score_floats);
     a.ws_o   = x->ws + s.score_floats + s.chosen_ints;
     a.ws_ml  = a.ws_o + (size_t)num_seqs * n_heads * s.chunks * x->head_dim;
     a.arrivals = s.inside ? x->arrivals : nullptr;

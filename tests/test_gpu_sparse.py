@@ -318,3 +318,22 @@ def test_large_groups(geom):
         q = np.abs(np.random.default_rng(1).normal(size=(1, H, hd))).astype(np.float32)
         _, sel = nv.sparse_decode(index, 1, q, tabs[:1], [500 * bs], 4, 0, 1)
         assert {300, 310, 499} <= set(sel[0, 0].tolist())
+
+
+@pytest.mark.parametrize("blocks", [(2049, 5000, 30), (16385, 2100, 41), (32768, 16000, 40), (32769, 32768, 39)], ids=str)
+@pytest.mark.parametrize("levels", [0, 2])
+def test_selections_of_long_contexts(blocks, levels):
+    """Up to 32 blocks a thread of the selection kernel, and the one for more; scores of a few levels or all different."""
+    KV, hd, bs, H, top = 1, 4, 1, 2, 40
+    tabs, n = oo.tables_for(blocks, bs, seed=67)
+    rng = np.random.default_rng(68 + levels)
+    held = []
+    with nv.PagedKVPool(2, n, bs, KV, hd) as pool, nv.BlockIndex(pool) as index:
+        for s, c in enumerate(blocks):
+            k = (rng.integers(-levels, levels + 1, (c, KV, hd)) if levels else rng.normal(size=(c, KV, hd))).astype(np.float32)
+            v = rng.normal(size=(c, KV, hd)).astype(np.float32)
+            nv.norm_rope_append(pool, 1, None, None, k, v, tabs, np.arange(c), np.full(c, s))
+            held.append((k, v))
+        index.update(1, tabs, [0] * len(blocks), blocks)
+        for first, last in ((1, 2), (0, 1)):
+            check(pool, index, tabs, held, blocks, H, top, first, last, seed=69)
