@@ -337,3 +337,29 @@ def test_selections_of_long_contexts(blocks, levels):
         index.update(1, tabs, [0] * len(blocks), blocks)
         for first, last in ((1, 2), (0, 1)):
             check(pool, index, tabs, held, blocks, H, top, first, last, seed=69)
+
+
+@pytest.mark.parametrize("geom", [(3, 96, 64), (1, 4, 33), (16, 128, 5), (9, 256, 16), (2, 260 - 4, 7)], ids=lambda g: "x".join(map(str, g)))
+@pytest.mark.parametrize("many", [False, True])
+def test_bounds_of_rows_of_any_width(geom, many):
+    """Few long blocks and many short ones: rows that end inside a workgroup's run of channels, blocks that are full, begun and
+    untouched; a NaN in a key stays in its channel."""
+    KV, hd, bs = geom
+    ctx = [7 * bs + 1, 3 * bs, 1, 0, 2 * bs - 1] + ([bs + 1] * 300 if many else [])
+    rng = np.random.default_rng(70)
+    tabs, blocks = oo.tables_for(ctx, bs, seed=70)
+    want = np.zeros((blocks, KV, 2, hd), np.float32)
+    with nv.PagedKVPool(1, blocks, bs, KV, hd) as pool, nv.BlockIndex(pool) as index:
+        rows, seqs, pos = [], [], []
+        for s, n in enumerate(ctx):
+            k = rng.normal(size=(n, KV, hd)).astype(np.float32)
+            if s == 1:
+                k[bs, KV - 1, hd - 1] = np.nan
+            for b in range((n + bs - 1) // bs):
+                part = k[b * bs:min(n, (b + 1) * bs)]
+                want[tabs[s, b], :, 0], want[tabs[s, b], :, 1] = part.min(0), part.max(0)
+            rows.append(k), seqs.append(np.full(n, s)), pos.append(np.arange(n))
+        k = np.concatenate(rows)
+        nv.norm_rope_append(pool, 0, None, None, k, k, tabs, np.concatenate(pos), np.concatenate(seqs))
+        index.update(0, tabs, [0] * len(ctx), ctx)
+        assert np.array_equal(bounds_of(index, 0), want, equal_nan=True)
