@@ -485,7 +485,11 @@ __device__ __forceinline__ int mx4_rows(const Mx4AttnArgs &a, int seq, int &row0
 
 // ---- few columns: the waves of a workgroup share the tokens --------------------------------------------------------------
 // Bound by the codes it reads while everything beside the loads hides behind them; what does not is the vector work of a
-// step.  The waves take steps of 32 tokens in turn and join through LDS.
+// step.  The waves take steps of 32 tokens in turn and join through LDS.  Of 128 channels, groups of four heads, eight kv-heads: 64 x
+// 2048 tokens 28.5 us (144 MB, 5.1 TB/s), 16 x 32768 98.5 us (574 MB, 5.8 TB/s; its loads alone, with nothing done to them, 91).  PACK
+// takes 16 products a step instead of 48 and 158 registers instead of 198, so that three workgroups fit a CU and not two: 16 x 32768
+// 115 us without, 105 with it, 102 in one round of three a CU.  Tried and no faster: two or three steps on their way (30.8 and 31.2
+// for the 28.4 of 64 x 2048), workgroups of three, six or twelve waves (45, 37 and 36 us).
 template <int KK, bool PACK>
 __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2) nvk_mx4_decode_kernel(const Mx4AttnArgs a)
 {
@@ -634,7 +638,10 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
 // ---- many columns: the waves of a workgroup share the operands -------------------------------------------------------------
 // Bound by the matrix instructions (48 for a tile of columns, a step and 128 channels) once the codes are turned into operands
 // only once: the four waves of a workgroup convert a quarter of a step's K and V each into LDS, a step ahead, and read all
-// of it as 16-byte operands.  One barrier a step: a buffer is written while the other is read.
+// of it as 16-byte operands.  One barrier a step: a buffer is written while the other is read.  Three chunks of up to 1500 rows
+// behind up to 4000 tokens, 32 heads of 128 channels: 440 us for 497 GFLOP of products, 1130 TFLOP/s, where a large library
+// product of bf16 reaches 1180 (each wave converting for itself: 684 us; one tile of columns a wave instead of two 2 % more).
+// With 64 channels and fewer the vector work of the softmax, which stays the same, is what bounds it.
 template <int KK, int NC>
 __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 : 2) nvk_mx4_prefill_kernel(const Mx4AttnArgs a)
 {
@@ -810,7 +817,8 @@ __global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_kernel(const Mx4Att
         join_chunks(a.ws_o + line * a.chunks * a.mx.head_dim, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim, a.out + line * a.mx.head_dim);
 }
 
-// Up to kJoinInside chunks (of many lines: a prefill's): a thread per four channels of a line.
+// Up to kJoinInside chunks (of many lines: a prefill's): a thread per four channels of a line.  (4088 rows of 8 heads of 80 channels, two
+// chunks: 9.4 us, a workgroup per line 45.6.)
 __global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_few_kernel(const Mx4AttnArgs a, unsigned lines)
 {
     const unsigned quads = a.mx.head_dim >> 2;
@@ -847,7 +855,8 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
 {
     Mx4Shape  s;
     const int group = n_heads / pool->n_kv_heads;
-    // Waves that share the tokens while one wave holds a sequence's columns; else waves that share the columns.
+    // Waves that share the tokens while one wave holds a sequence's columns; else waves that share the columns.  (Up to 16 columns a
+    // wave of the latter would be all that works.)
     s.prefill = (long long)max_rows * group > 16;
     s.pack    = (long long)max_rows * group <= 4;
     s.col_blocks = s.prefill ? ceil_div((long long)max_rows * group, 16 * prefill_cols(pool->kk) * kPrefillWaves) : 1;

