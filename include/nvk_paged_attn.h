@@ -460,7 +460,8 @@ long long nvk_mx4_pool_layer_bytes(const nvk_mx4_pool *pool);
 int       nvk_mx4_pool_layer_ptr(const nvk_mx4_pool *pool, int layer, void **base_dev);
 int       nvk_mx4_pool_stream(const nvk_mx4_pool *pool, void **stream);
 int       nvk_mx4_pool_synchronize(nvk_mx4_pool *pool);
-/* total_rows, max_rows: query rows in all and of one sequence (decode: num_seqs and 1) */
+/* total_rows, max_rows: query rows in all and of one sequence (decode: num_seqs and 1).  No call with as many heads and no more
+ * sequences, rows and tokens grows the workspace afterwards. */
 int       nvk_mx4_pool_reserve_workspace(nvk_mx4_pool *pool, int num_seqs, int n_heads, int total_rows, int max_rows, int max_ctx);
 long long nvk_mx4_pool_workspace_generation(const nvk_mx4_pool *pool);
 /* nvk_pool_norm_rope_append into the 4-bit cache (rope, weights NULL: a plain append) */
@@ -516,7 +517,9 @@ int nvk_mx4_prefill_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_he
  * asynchronous on `stream` (NULL = the pool's), max_ctx >= every ctx_lens[s], q 16-byte aligned; table entries outside the pool are
  * clamped for reading and skipped by an update.  Scores, lists and partial results live in one workspace of the index: decode
  * calls on an index must be ordered with respect to each other; a call that would have to grow it under stream capture is refused
- * (nvk_block_index_reserve_workspace).  The index must be destroyed before its pool; destroying waits for the device. */
+ * (nvk_block_index_reserve_workspace:
+ * no call with as many heads and no more sequences, tokens and blocks grows it afterwards).  Two tables may share blocks that
+ * hold the same tokens of both.  The index must be destroyed before its pool; destroying waits for the device. */
 typedef struct nvk_block_index nvk_block_index;
 int       nvk_block_index_create(nvk_pool *pool, nvk_block_index **out_index);
 int       nvk_block_index_destroy(nvk_block_index *index);

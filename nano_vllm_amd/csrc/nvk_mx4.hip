@@ -881,10 +881,21 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     return s;
 }
 
-int reserve(nvk_mx4_pool *pool, const Mx4Shape &s, hipStream_t st, const char *who)
+int reserve(nvk_mx4_pool *pool, size_t floats, size_t arrivals, hipStream_t st, const char *who)
 {
-    const int rc = nvk::grow_workspace(&pool->ws, &pool->ws_floats, &pool->ws_generation, s.ws_floats, st, who);
-    return rc != NVK_OK ? rc : nvk::grow_counters(&pool->arrivals, &pool->arrivals_cap, &pool->ws_generation, s.arrivals, st, who);
+    const int rc = nvk::grow_workspace(&pool->ws, &pool->ws_floats, &pool->ws_generation, floats, st, who);
+    return rc != NVK_OK ? rc : nvk::grow_counters(&pool->arrivals, &pool->arrivals_cap, &pool->ws_generation, arrivals, st, who);
+}
+
+// What no call of up to this shape passes, fewer sequences (which are cut into more chunks) among them: as mx4_shape cuts, lines times
+// chunks are at most the workgroups that fit the chip, half as many again for prompts, times the columns of one.
+size_t most_floats(const nvk_mx4_pool *pool, int n_heads, int total_rows, int max_rows, int max_ctx)
+{
+    const long long columns = (long long)max_rows * (n_heads / pool->n_kv_heads), lines = (long long)total_rows * n_heads;
+    long long       most = std::max(3 * std::min(columns, 4LL), 2 * std::min(columns, 16LL));
+    if (columns > 16)
+        most = std::max(most, 3 * std::min(columns, 16LL * prefill_cols(pool->kk) * kPrefillWaves));
+    return (size_t)std::min(most * pool->num_cus, lines * (max_ctx / 64)) * (size_t)(pool->head_dim + 2);
 }
 
 template <int KK> void launch_attn(const Mx4AttnArgs &a, const Mx4Shape &s, unsigned blocks, hipStream_t st)
@@ -925,7 +936,7 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
     if (!nvk::grid_fits(blocks, 64 * kDecodeWaves) || (s.chunks > 1 && !nvk::grid_fits(lines, nvk::kJoinThreads))
         || (s.chunks > 1 && !nvk::grid_fits(few, nvk::kJoinThreads)))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: %lld workgroups", who, blocks);
-    int rc = reserve(pool, s, st, who);
+    int rc = reserve(pool, s.ws_floats, s.arrivals, st, who);
     if (rc != NVK_OK)
         return rc;
     Mx4AttnArgs a{};
@@ -1130,8 +1141,7 @@ int nvk_mx4_pool_reserve_workspace(nvk_mx4_pool *pool, int num_seqs, int n_heads
     if (rc != NVK_OK)
         return rc;
     NVK_SCOPE(pool->device);
-    const Mx4Shape s = mx4_shape(pool, num_seqs, n_heads, total_rows, std::max(max_rows, 1), max_ctx);
-    return reserve(pool, s, pool->stream, who);
+    return reserve(pool, most_floats(pool, n_heads, total_rows, max_rows, max_ctx), 3 * (size_t)pool->num_cus, pool->stream, who);
 }
 
 int nvk_mx4_decode_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, const float *q_dev,

@@ -847,10 +847,20 @@ SparseShape sparse_shape(const nvk_block_index *x, int num_seqs, int n_heads, in
     return s;
 }
 
-int reserve(nvk_block_index *x, const SparseShape &s, hipStream_t st, const char *who)
+int reserve(nvk_block_index *x, size_t floats, size_t arrivals, hipStream_t st, const char *who)
 {
-    const int rc = nvk::grow_workspace(&x->ws, &x->ws_floats, &x->ws_generation, s.floats(), st, who);
-    return rc != NVK_OK ? rc : nvk::grow_counters(&x->arrivals, &x->arrivals_cap, &x->ws_generation, s.arrivals, st, who);
+    const int rc = nvk::grow_workspace(&x->ws, &x->ws_floats, &x->ws_generation, floats, st, who);
+    return rc != NVK_OK ? rc : nvk::grow_counters(&x->arrivals, &x->arrivals_cap, &x->ws_generation, arrivals, st, who);
+}
+
+// What no call of up to this shape passes, fewer sequences (which are cut into more chunks) and fewer blocks among them: as
+// sparse_shape cuts, lines times chunks are at most the workgroups that fit the chip times the heads of one, or chunks are 64 blocks.
+size_t most_floats(const nvk_block_index *x, int num_seqs, int n_heads, int max_ctx, int top)
+{
+    const SparseShape s = sparse_shape(x, num_seqs, n_heads, max_ctx, top);
+    const size_t      lines = (size_t)num_seqs * x->n_kv_heads;
+    const long long   parts = std::max(4LL * kCus * s.hg, (long long)num_seqs * n_heads * ceil_div(std::min(s.max_nb, top), 64));
+    return to_line(lines * s.max_nb) + to_line(lines * std::min(s.max_nb, top)) + (size_t)parts * (x->head_dim + 2);
 }
 
 template <int NV, int HG> void launch_sparse(const SparseArgs &a, const SparseShape &s, bool score, hipStream_t st)
@@ -976,7 +986,7 @@ int enqueue_sparse(nvk_block_index *x, int layer, int num_seqs, int n_heads, con
     if (!nvk::grid_fits(lines * s.score_slots, 64 * nvk::kSparseWaves) || !nvk::grid_fits(lines * s.head_sets * s.chunks, 64 * nvk::kSparseWaves)
         || (!s.select_inside && !nvk::grid_fits(lines, nvk::kSelectThreads)) || (joins && !nvk::grid_fits((long long)num_seqs * n_heads, nvk::kJoinThreads)))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: too many workgroups", who);
-    int rc = reserve(x, s, st, who);
+    int rc = reserve(x, s.floats(), s.arrivals, st, who);
     if (rc != NVK_OK)
         return rc;
     SparseArgs a{};
@@ -1085,7 +1095,8 @@ int nvk_block_index_reserve_workspace(nvk_block_index *index, int num_seqs, int 
     const int   rs = pool_stream(index, nullptr, &st);
     if (rs != NVK_OK)
         return rs;
-    return reserve(index, sparse_shape(index, num_seqs, n_heads, max_ctx, top_blocks), st, who);
+    const size_t tasks = (size_t)num_seqs * n_heads; // (no more workgroups meet than there are heads)
+    return reserve(index, most_floats(index, num_seqs, n_heads, max_ctx, top_blocks), std::max(tasks, 4 * (size_t)kCus), st, who);
 }
 
 int nvk_block_index_update(nvk_block_index *index, int layer, int num_seqs, const int *block_tables, int max_blocks,

@@ -437,3 +437,24 @@ def test_two_pools_at_once_and_shared_blocks():
         assert (d[3].numpy() == want).all()
         pool.close()
         st.close()
+
+
+def test_a_reservation_holds_for_every_smaller_call():
+    """Fewer sequences are cut into more pieces: after one reservation nothing up to that shape moves the workspace."""
+    for KV, group, hd in ((1, 4, 32), (2, 7, 64), (2, 1, 256), (1, 20, 128)):
+        H = KV * group
+        for seqs, rows, ctx in ((64, 1, 3000), (40, 6, 9000), (6, 500, 2000)):
+            with nv.Mx4KVPool(1, 600, 16, KV, hd) as pool:
+                pool.reserve_workspace(seqs, H, rows, ctx, seqs * rows)
+                gen = pool.workspace_generation
+                tabs = DeviceArray(np.zeros((seqs, 600), np.int32))
+                q, out = (DeviceArray(np.zeros((seqs * rows, H, hd), np.float32)) for _ in range(2))
+                for n in sorted({1, 2, 3, 7, 13, seqs // 2, seqs} & set(range(1, seqs + 1))):
+                    for c in sorted({1, 100, 700, ctx // 2, ctx}):
+                        lens = DeviceArray(np.full(n, 1, np.int32))  # (what counts is the bound given)
+                        nv.mx4_decode_device(pool, 0, n, H, q, tabs, 600, lens, c, out)
+                        for r in sorted({1, 2, 5, rows // 2, rows} & set(range(1, rows + 1))):
+                            off = DeviceArray(np.arange(n + 1, dtype=np.int32))
+                            nv.mx4_prefill_device(pool, 0, n, H, n * r, q, off, r, tabs, 600, lens, c, out)
+                            pool.synchronize()
+                assert pool.workspace_generation == gen, (KV, group, hd, seqs, rows, ctx)

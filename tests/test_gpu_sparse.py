@@ -363,3 +363,23 @@ def test_bounds_of_rows_of_any_width(geom, many):
         nv.norm_rope_append(pool, 0, None, None, k, k, tabs, np.concatenate(pos), np.concatenate(seqs))
         index.update(0, tabs, [0] * len(ctx), ctx)
         assert np.array_equal(bounds_of(index, 0), want, equal_nan=True)
+
+
+def test_a_reservation_holds_for_every_smaller_call():
+    for KV, group, hd, bs in ((1, 4, 32, 16), (2, 7, 64, 4), (2, 3, 256, 16), (1, 20, 128, 1)):
+        H = KV * group
+        for seqs, ctx, top in ((64, 3000, 300), (5, 9000, 4000), (300, 400, 20)):
+            width = (ctx + bs - 1) // bs
+            with nv.PagedKVPool(1, 4, bs, KV, hd) as pool, nv.BlockIndex(pool) as index:
+                index.reserve_workspace(seqs, H, ctx, top)
+                gen = index.workspace_generation
+                tabs = DeviceArray(np.zeros((seqs, width), np.int32))
+                q, out = (DeviceArray(np.zeros((seqs, H, hd), np.float32)) for _ in range(2))
+                for n in sorted({1, 2, 3, 7, 13, seqs // 2, seqs} & set(range(1, seqs + 1))):
+                    lens = DeviceArray(np.full(n, 1, np.int32))  # (what counts is the bound given)
+                    for c in sorted({1, 100, ctx // 2, ctx}):
+                        for t in sorted({1, 5, 16, 65, top // 2, top}):
+                            if t <= top:
+                                nv.sparse_decode_device(index, 0, n, H, q, tabs, width, lens, c, t, 0, 1, out)
+                    pool.synchronize()
+                assert index.workspace_generation == gen, (KV, group, hd, bs, seqs, ctx, top)
