@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
 // Bound by the matrix instructions (48 for a tile of columns, a step and 128 channels) once the codes are turned into operands
 // only once: the four waves of a workgroup convert a quarter of a step's K and V each into LDS, a step ahead, and read all
 // of it as 16-byte operands.  One barrier a step: a buffer is written while the other is read.  Three chunks of up to 1500 rows
-// behind up to 4000 tokens, 32 heads of 128 channels: 440 us for 497 GFLOP of products, 1130 TFLOP/s, where a large library
+// behind up to 4000 tokens, 32 heads of 128 channels: 435 us for 497 GFLOP of products, 1140 TFLOP/s, where a large library
 // product of bf16 reaches 1180 (each wave converting for itself: 684 us; one tile of columns a wave instead of two 2 % more).
 // With 64 channels and fewer the vector work of the softmax, which stays the same, is what bounds it.
 template <int KK, int NC>
@@ -678,16 +678,17 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 
     const Mx4Tiles      tiles(a, seq, kvh, (min(end, ctx) - 1) / kMx4Tile);
     const Mx4Places<KK> places(w.lane);
     const int           tile_j = wave & 1; // (W is even: all K items of a wave lie in one tile)
-    Mx4Raw<KK>          raw[2];
+    constexpr int       AHEAD = KK == 2 ? 2 : 1; // steps whose codes are on their way (64 channels: 5 % less time; 32: 25 % more)
+    Mx4Raw<KK>          ring[AHEAD][2];
     int                 entry = 0; // lane L: tile L of the current 32 steps
-    auto                fetch = [&](int i) {
+    auto                fetch = [&](int i, Mx4Raw<KK> (&raw)[2]) {
         if ((i & 31) == 0)
             entry = tiles.entry((begin >> 4) + 2 * i + w.lane);
 #pragma unroll
         for (int j = 0; j < 2; j++)
             load_tile_part<KK>(raw[j], tiles.at(__builtin_amdgcn_readlane(entry, 2 * (i & 31) + j)), places, j == tile_j, wave < KK);
     };
-    auto convert = [&](int i) {
+    auto convert = [&](int i, const Mx4Raw<KK> (&raw)[2]) {
         unsigned vs[2] = {raw[0].vs, raw[1].vs};
         w.mark(vs, begin + 32 * i);
         const int   buf = i & 1;
@@ -705,17 +706,19 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 
             }
     };
     if (steps > 0) {
-        fetch(0);
-        convert(0);
-        if (steps > 1)
-            fetch(1);
+        fetch(0, ring[0]);
+        convert(0, ring[0]);
+#pragma unroll
+        for (int d = 1; d <= AHEAD; d++)
+            if (d < steps)
+                fetch(d, ring[d % AHEAD]);
     }
     __syncthreads();
-    for (int i = 0; i < steps; i++) {
+    auto step = [&](int i, Mx4Raw<KK> (&raw)[2]) { // raw: the codes of step i + 1
         if (i + 1 < steps) {
-            convert(i + 1);
-            if (i + 2 < steps)
-                fetch(i + 2);
+            convert(i + 1, raw);
+            if (i + 1 + AHEAD < steps)
+                fetch(i + 1 + AHEAD, raw);
         }
         const int t0 = begin + 32 * i, buf = i & 1;
         if (t0 < w.most) {
@@ -749,7 +752,12 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 
             }
         }
         __syncthreads();
-    }
+    };
+    for (int i = 0; i < steps; i += AHEAD)
+#pragma unroll
+        for (int d = 0; d < AHEAD; d++)
+            if (d == 0 || i + d < steps)
+                step(i + d, ring[(d + 1) % AHEAD]);
     w.finish();
 
 #pragma unroll
@@ -867,8 +875,9 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     // 9.0, 230 x 256 9.7, 9.7, 7.0, 7.1; 64 x 2048, two workgroups a CU: 28.1 us uncut, 39.6 in two rounds.)
     long long fit = (pool->kk == 8 ? 1LL : s.pack ? 3LL : 2LL) * pool->num_cus;
     // A prompt's early rows see few of the chunks: half as many again where all rows are new.  (1157 rows: 35.6 us in 3 chunks,
-    // 32.2 in 4, 39.6 in 6; 128 rows behind 8064 tokens: 65.3 in 16, 82.4 in 24.)
-    if (s.prefill)
+    // 32.2 in 4, 39.6 in 6; 128 rows behind 8064 tokens: 65.3 in 16, 82.4 in 24.  Not with 256 channels, one workgroup a CU: 700 rows
+    // 80 uncut, 93 in 2.)
+    if (s.prefill && pool->kk <= 4)
         fit += fit * std::min(max_rows, max_ctx) / (2LL * std::max(max_ctx, 1));
     s.chunks = (int)std::max(1LL, std::min(fit / std::max(tasks, 1LL), (long long)max_ctx / (s.prefill ? 64 : 192)));
     if (!s.prefill && s.chunks > nvk::kJoinInside && max_ctx <= 512 * nvk::kJoinInside)
