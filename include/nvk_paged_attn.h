@@ -442,7 +442,8 @@ int nvk_pool_norm_rope_append(nvk_pool *pool, int layer, const nvk_rope *rope, i
  * The reference's cache (include/core/model.hpp:94-97) in 17/32 byte a value instead of 4: each value is
  * sign * {0, .5, 1, 1.5, 2, 3, 4, 6} * 2^e (e2m1), with one e (a byte) for each 32 channels of a row, the smallest with
  * |values| <= 7 * 2^e, at most 125; the last group is what is left of the row.  Values go to the nearest, ties to the even code
- * (above 5 * 2^125, 2.13e38, to 6 * 2^125).  A group that holds an infinity or a NaN is stored as NaN.  Block tables, positions and contexts are those of nvk_pool.
+ * (above 5 * 2^125, 2.13e38, to 6 * 2^125).  A group that holds an infinity or a NaN is stored as NaN.  Block tables, positions
+ * and contexts are those of nvk_pool.
  *   block_size  a multiple of 16;  head_dim  a multiple of 8, at most 256 (stored as 32, 64, 128 or 256 channels)
  * Zero-initialised.  The layout inside a layer is the library's (nvk_mx4_pool_layer_ptr / _layer_bytes: for copies of whole
  * layers between pools of one geometry).
@@ -500,7 +501,7 @@ int nvk_mx4_prefill_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_he
 /* ------------------------------------------------------- block-sparse decode --
  * Decode attention that reads the blocks a cheap score selects, for long contexts; the cache is an nvk_pool (head_dim a
  * multiple of 4, at most 256).  An index beside the pool keeps the least (lo) and the largest (hi) key element of each block,
- * kv-head and channel: [layer][block][kv-head][lo | hi][head_dim] fp32, 1 / (2 block_size) of the pool, zero like a new pool.
+ * kv-head and channel: [layer][block][kv-head][lo | hi][head_dim] fp32, 1 / block_size of the pool, zero like a new pool.
  * For a query head q, q . k <= sum_c max(q_c, 0) hi_c + min(q_c, 0) lo_c for every key k of a block; a block's score for a kv-head
  * is the largest of these over the group's query heads (summed in 64 bits, rounded to fp32; a score that is no number
  * counts as infinite).  For each (sequence, kv-head) a call reads
@@ -516,10 +517,10 @@ int nvk_mx4_prefill_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_he
  * Host-pointer forms (ptr_kind NVK_PTR_HOST, nvk_sparse_decode) validate, stage, run, synchronise; device-pointer forms are
  * asynchronous on `stream` (NULL = the pool's), max_ctx >= every ctx_lens[s], q 16-byte aligned; table entries outside the pool are
  * clamped for reading and skipped by an update.  Scores, lists and partial results live in one workspace of the index: decode
- * calls on an index must be ordered with respect to each other; a call that would have to grow it under stream capture is refused
- * (nvk_block_index_reserve_workspace:
- * no call with as many heads and no more sequences, tokens and blocks grows it afterwards).  Two tables may share blocks that
- * hold the same tokens of both.  The index must be destroyed before its pool; destroying waits for the device. */
+ * calls on an index must be ordered with respect to each other; a call that would have to grow it under stream capture is
+ * refused (after nvk_block_index_reserve_workspace no call with as many heads and no more sequences, tokens and blocks grows
+ * it).  Tables may share blocks that hold the same tokens of each sequence.  The index must be destroyed before its pool;
+ * destroying waits for the device. */
 typedef struct nvk_block_index nvk_block_index;
 int       nvk_block_index_create(nvk_pool *pool, nvk_block_index **out_index);
 int       nvk_block_index_destroy(nvk_block_index *index);
