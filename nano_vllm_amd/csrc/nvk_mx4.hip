@@ -863,8 +863,8 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
 {
     Mx4Shape  s;
     const int group = n_heads / pool->n_kv_heads;
-    // Waves that share the tokens while one wave holds a sequence's columns; else waves that share the columns.  (Up to 16 columns a
-    // wave of the latter would be all that works.)
+    // Waves that share the tokens while one wave holds a sequence's columns; else waves that share the columns, of which one alone
+    // would work on up to 16.
     s.prefill = (long long)max_rows * group > 16;
     s.pack    = (long long)max_rows * group <= 4;
     s.col_blocks = s.prefill ? ceil_div((long long)max_rows * group, 16 * prefill_cols(pool->kk) * kPrefillWaves) : 1;
@@ -938,6 +938,7 @@ int enqueue_attention(nvk_mx4_pool *pool, int layer, int num_seqs, int n_heads, 
                       const int *row_offsets, int max_rows, const int *tables, int max_blocks, const int *ctx_lens, int max_ctx,
                       float *out, hipStream_t st, const char *who)
 {
+    total_rows = (int)std::min((long long)total_rows, (long long)num_seqs * max_rows); // (rows behind these belong to nobody)
     const Mx4Shape  s = mx4_shape(pool, num_seqs, n_heads, total_rows, max_rows, max_ctx);
     const long long units = (long long)num_seqs * s.col_blocks * s.chunks;
     const long long blocks = units * pool->n_kv_heads;

@@ -458,3 +458,24 @@ def test_a_reservation_holds_for_every_smaller_call():
                             nv.mx4_prefill_device(pool, 0, n, H, n * r, q, off, r, tabs, 600, lens, c, out)
                             pool.synchronize()
                 assert pool.workspace_generation == gen, (KV, group, hd, seqs, rows, ctx)
+
+
+def test_a_padded_batch_of_rows():
+    """Far more rows than the sequences' chunks can hold: they are left as they were and take no workspace."""
+    KV, H, hd, bs = 1, 4, 128, 16
+    ctx, rows = [2500, 900], [3, 5]
+    pool, tabs, held = filled(ctx, bs, KV, hd, seed=41)
+    q = np.random.default_rng(42).normal(size=(4000, H, hd)).astype(np.float32)
+    dq, do, dt, dc, dof = (DeviceArray(x) for x in (q, np.full_like(q, 5), tabs, np.array(ctx, np.int32), np.array([0, 3, 8], np.int32)))
+    with pool:
+        pool.reserve_workspace(2, H, 5, max(ctx), 4000)
+        gen = pool.workspace_generation
+        nv.mx4_prefill_device(pool, 1, 2, H, 4000, dq, dof, 5, dt, tabs.shape[1], dc, max(ctx), do)
+        pool.synchronize()
+        assert pool.workspace_generation == gen
+        got = do.numpy()
+    assert (got[8:] == 5).all()
+    for s, lo, hi in ((0, 0, 3), (1, 3, 8)):
+        n = hi - lo
+        want, bound = oo.attention(q[lo:hi], *held[s], [ctx[s] - n + i + 1 for i in range(n)])
+        assert (np.abs(got[lo:hi] - want) <= bound).all()
