@@ -66,7 +66,7 @@ class PagedKVPool:
     # -- lifetime -----------------------------------------------------------
     def close(self) -> None:
         h = getattr(self, "_h", None)
-        if h:
+        if h and _capi.lib is not None:  # (None: the interpreter is going down)
             _capi.lib.nvk_pool_destroy(h)
             self._h = None
 
