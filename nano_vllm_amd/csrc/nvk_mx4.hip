@@ -202,7 +202,7 @@ __device__ __forceinline__ void load_tile_part(Mx4Raw<KK> &r, const unsigned cha
 }
 
 // ---- what both kernels are made of ------------------------------------------------------------------------------------
-// A wave holds NC tiles of columns, a column being a (row, head of the group) pair of one kv-head, and takes 32 tokens a step:
+// A wave holds a tile of 16 columns, a column being a (row, head of the group) pair of one kv-head, and takes 32 tokens a step:
 //   S^T = K Q^T     A = K [16 tokens x 32 channels], B = Q^T [32 channels x 16 columns] -> lane (g, col): tokens 4g .. 4g+3
 //   O^T = V^T P^T   A = V^T [16 channels x 32 tokens], B = P^T [32 tokens x 16 columns]
 // The order of channels (in S) and of tokens (in O) along a contraction is free, so it is chosen such that the lane that holds
@@ -211,21 +211,21 @@ __device__ __forceinline__ void load_tile_part(Mx4Raw<KK> &r, const unsigned cha
 // PACK: up to four columns, each four times in a tile: the first three copies carry one piece of q and of the probabilities
 // each, whose products then take a third of the instructions and registers, and the copies of a column are added (a quad of
 // lanes).
-template <int KK, int NC, bool PACK> struct Mx4Wave
+template <int KK, bool PACK> struct Mx4Wave
 {
     static constexpr int COLS   = PACK ? 4 : 16; // columns of a tile
     static constexpr int PIECES = PACK ? 1 : 3;
 
     int      lane, g, l16, lcol, piece; // lcol: the lane's column of a tile; PACK: `piece` is which copy of it
-    int      limit[NC], out_row[NC], out_head[NC]; // a column's row sees the tokens below `limit`: all up to its own
-    int      most, least;                          // the largest and the smallest limit of the wave's columns
-    bf16x8   q[NC][KK][PIECES];
-    f32x4    acc[NC][2 * KK]; // [ct][i]: channel (4 g + i) * 2 KK + ct
+    int      limit, out_row, out_head; // the lane's column: its row sees the tokens below `limit`, all up to its own
+    int      most, least;              // the largest and the smallest limit of the wave's columns
+    bf16x8   q[KK][PIECES];
+    f32x4    acc[2 * KK]; // [ct][i]: channel (4 g + i) * 2 KK + ct
     // m: what scores are taken relative to, a score that was the largest once (0 while lim is -inf: no token yet).  It is moved
     // only where a score passes it by more than 8: probabilities up to 2^8 are as exact as those up to 1.
-    float    m[NC], lim[NC], l[NC];
-    unsigned poisoned[NC]; // channel groups in which a token that the column sees holds no number
-    unsigned cut1, cut2;   // PACK: what a probability loses to become the lane's piece (the fourth copy's result is dropped)
+    float    m, lim, l;
+    unsigned poisoned;   // channel groups in which a token that the column sees holds no number
+    unsigned cut1, cut2; // PACK: what a probability loses to become the lane's piece (the fourth copy's result is dropped)
 
     __device__ __forceinline__ void start(const Mx4AttnArgs &a, int row0, int rows, int ctx, int kvh, int col0)
     {
@@ -233,47 +233,44 @@ template <int KK, int NC, bool PACK> struct Mx4Wave
         lcol = PACK ? l16 >> 2 : l16, piece = l16 & 3;
         cut1 = piece > 0 ? 0xffff0000u : 0u, cut2 = piece > 1 ? 0xffff0000u : 0u;
         const int columns = rows * a.group;
-        const int last = min(col0 + COLS * NC - 1, columns - 1) / a.group;
+        const int last = min(col0 + COLS - 1, columns - 1) / a.group;
         most  = col0 < columns ? max(ctx - rows + last + 1, 0) : 0;
         least = col0 < columns ? max(ctx - rows + col0 / a.group + 1, 0) : 0;
+        const int col = col0 + lcol, r = col / a.group;
+        out_row  = col < columns ? row0 + r : -1;
+        out_head = kvh * a.group + col % a.group;
+        limit    = col < columns ? max(ctx - rows + r + 1, 0) : 0;
+        // Q^T: channels g*8*KK + kk*8 .. of the column, in units in which a probability is a power of two
 #pragma unroll
-        for (int n = 0; n < NC; n++) {
-            const int col = col0 + COLS * n + lcol, r = col / a.group;
-            out_row[n]  = col < columns ? row0 + r : -1;
-            out_head[n] = kvh * a.group + col % a.group;
-            limit[n]    = col < columns ? max(ctx - rows + r + 1, 0) : 0;
-            // Q^T: channels g*8*KK + kk*8 .. of the column, in units in which a probability is a power of two
+        for (int kk = 0; kk < KK; kk++) {
+            float     x[8];
+            const int c0 = g * 8 * KK + kk * 8;
 #pragma unroll
-            for (int kk = 0; kk < KK; kk++) {
-                float     x[8];
-                const int c0 = g * 8 * KK + kk * 8;
+            for (int i = 0; i < 8; i++)
+                x[i] = 0.f;
+            if (out_row >= 0 && c0 < a.mx.head_dim) {
+                const float *src = a.q + ((int64_t)out_row * a.n_heads + out_head) * a.mx.head_dim + c0;
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    x[i] = 0.f;
-                if (out_row[n] >= 0 && c0 < a.mx.head_dim) {
-                    const float *src = a.q + ((int64_t)out_row[n] * a.n_heads + out_head[n]) * a.mx.head_dim + c0;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        x[i] = src[i] * a.scale_log2e;
-                }
-                const Pieces three = split8(x);
-                if constexpr (PACK) {
-                    const u32x4 none = {0, 0, 0, 0};
-                    const u32x4 one  = piece == 0   ? __builtin_bit_cast(u32x4, three.p[0])
-                                       : piece == 1 ? __builtin_bit_cast(u32x4, three.p[1])
-                                       : piece == 2 ? __builtin_bit_cast(u32x4, three.p[2]) : none;
-                    q[n][kk][0] = __builtin_bit_cast(bf16x8, one);
-                }
-                else
-#pragma unroll
-                    for (int e = 0; e < 3; e++)
-                        q[n][kk][e] = three.p[e];
+                    x[i] = src[i] * a.scale_log2e;
             }
-            m[n] = 0.f, lim[n] = -INFINITY, l[n] = 0.f, poisoned[n] = 0;
+            const Pieces three = split8(x);
+            if constexpr (PACK) {
+                const u32x4 none = {0, 0, 0, 0};
+                const u32x4 one  = piece == 0   ? __builtin_bit_cast(u32x4, three.p[0])
+                                   : piece == 1 ? __builtin_bit_cast(u32x4, three.p[1])
+                                   : piece == 2 ? __builtin_bit_cast(u32x4, three.p[2]) : none;
+                q[kk][0] = __builtin_bit_cast(bf16x8, one);
+            }
+            else
 #pragma unroll
-            for (int ct = 0; ct < 2 * KK; ct++)
-                acc[n][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int e = 0; e < 3; e++)
+                    q[kk][e] = three.p[e];
         }
+        m = 0.f, lim = -INFINITY, l = 0.f, poisoned = 0;
+#pragma unroll
+        for (int ct = 0; ct < 2 * KK; ct++)
+            acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
     // A group of V that holds no number (scale byte 255): its scale is taken as 0, and the columns that see the token are marked.
@@ -294,23 +291,18 @@ template <int KK, int NC, bool PACK> struct Mx4Wave
                     for (; who; who &= who - 1) { // lane (quad, c16) tells: token 4 quad + b of tile j, group of c16
                         const int from = __ffsll((long long)who) - 1;
                         const int token = t0 + 16 * j + 4 * (from >> 4) + b;
-#pragma unroll
-                        for (int n = 0; n < NC; n++)
-                            if (token < limit[n])
-                                poisoned[n] |= 1u << ((from & 15) * KK / 16);
+                        if (token < limit)
+                            poisoned |= 1u << ((from & 15) * KK / 16);
                     }
                 }
         }
     }
 
     // Where scores start: relative to m.
-    __device__ __forceinline__ f32x4 origin(int n) const
-    {
-        return PACK && piece ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{-m[n], -m[n], -m[n], -m[n]};
-    }
+    __device__ __forceinline__ f32x4 origin() const { return PACK && piece ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{-m, -m, -m, -m}; }
 
-    // Scores of tile n (s[j][i]: token t0 + 16 j + 4 g + i) -> the pieces of its probabilities; maximum, sum and output follow.
-    __device__ __forceinline__ void softmax(int n, const f32x4 (&s)[2], int t0, bf16x8 (&p)[PIECES])
+    // Scores (s[j][i]: token t0 + 16 j + 4 g + i) -> the pieces of its probabilities; maximum, sum and output follow.
+    __device__ __forceinline__ void softmax(const f32x4 (&s)[2], int t0, bf16x8 (&p)[PIECES])
     {
         float t[8], top = -INFINITY;
 #pragma unroll
@@ -322,23 +314,23 @@ template <int KK, int NC, bool PACK> struct Mx4Wave
         if (t0 + 32 > least) {
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (t0 + 16 * (e >> 2) + 4 * g + (e & 3) >= limit[n])
+                if (t0 + 16 * (e >> 2) + 4 * g + (e & 3) >= limit)
                     t[e] = -INFINITY;
         }
 #pragma unroll
         for (int e = 0; e < 8; e++)
             top = fmaxf(top, t[e]);
         top = max_of_g(top);
-        if (__any(top > lim[n])) {
-            const bool  over = top > lim[n];
+        if (__any(top > lim)) {
+            const bool  over = top > lim;
             const float up = over ? top : 0.f;
-            const float alpha = lim[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-up);
-            m[n] += up;
-            lim[n] = over ? 8.f : lim[n];
-            l[n] *= alpha;
+            const float alpha = lim == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-up);
+            m += up;
+            lim = over ? 8.f : lim;
+            l *= alpha;
 #pragma unroll
             for (int ct = 0; ct < 2 * KK; ct++)
-                acc[n][ct] *= alpha;
+                acc[ct] *= alpha;
 #pragma unroll
             for (int e = 0; e < 8; e++)
                 t[e] -= up;
@@ -349,7 +341,7 @@ template <int KK, int NC, bool PACK> struct Mx4Wave
             t[e] = __builtin_amdgcn_exp2f(t[e]);
             sum += t[e];
         }
-        l[n] += sum;
+        l += sum;
         if constexpr (PACK) { // the lane's own piece: what as many truncations leave
             union
             {
@@ -379,26 +371,21 @@ template <int KK, int NC, bool PACK> struct Mx4Wave
     {
         if constexpr (PACK) // the three copies of a column
 #pragma unroll
-            for (int n = 0; n < NC; n++)
+            for (int ct = 0; ct < 2 * KK; ct++)
 #pragma unroll
-                for (int ct = 0; ct < 2 * KK; ct++)
+                for (int i = 0; i < 4; i++)
+                    acc[ct][i] = sum_of_quad(piece == 3 ? 0.f : acc[ct][i]);
+        if (lim == -INFINITY)
+            m = -INFINITY;
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (poisoned)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        acc[n][ct][i] = sum_of_quad(piece == 3 ? 0.f : acc[n][ct][i]);
+            for (int ct = 0; ct < 2 * KK; ct++)
 #pragma unroll
-        for (int n = 0; n < NC; n++) {
-            if (lim[n] == -INFINITY)
-                m[n] = -INFINITY;
-            l[n] += __shfl_xor(l[n], 16);
-            l[n] += __shfl_xor(l[n], 32);
-            if (poisoned[n])
-#pragma unroll
-                for (int ct = 0; ct < 2 * KK; ct++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if ((poisoned[n] >> (((4 * g + i) * 2 * KK + ct) / 32)) & 1u)
-                            acc[n][ct][i] = __uint_as_float(0x7fc00000u);
-        }
+                for (int i = 0; i < 4; i++)
+                    if ((poisoned >> (((4 * g + i) * 2 * KK + ct) / 32)) & 1u)
+                        acc[ct][i] = __uint_as_float(0x7fc00000u);
     }
 };
 
@@ -493,7 +480,7 @@ __device__ __forceinline__ int mx4_rows(const Mx4AttnArgs &a, int seq, int &row0
 template <int KK, bool PACK>
 __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2) nvk_mx4_decode_kernel(const Mx4AttnArgs a)
 {
-    using Wave = Mx4Wave<KK, 1, PACK>;
+    using Wave = Mx4Wave<KK, PACK>;
     constexpr int HDP = 32 * KK, COLS = Wave::COLS, W = kDecodeWaves;
     const int     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -546,24 +533,24 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
             for (int kk = 0; kk < KK; kk++)
                 k[j][kk] = k_operand(raw[j].k[kk], scale_at(raw[j].ks[KK == 8 ? kk / 4 : 0], 0));
         // the large pieces of q first: the sums of the small ones then round at the size of what is left
-        f32x4 s[2] = {w.origin(0), w.origin(0)};
+        f32x4 s[2] = {w.origin(), w.origin()};
 #pragma unroll
         for (int e = 0; e < Wave::PIECES; e++)
 #pragma unroll
             for (int kk = 0; kk < KK; kk++)
 #pragma unroll
                 for (int j = 0; j < 2; j++)
-                    s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[j][kk], w.q[0][kk][e], s[j], 0, 0, 0);
+                    s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[j][kk], w.q[kk][e], s[j], 0, 0, 0);
         bf16x8 p[Wave::PIECES];
-        w.softmax(0, s, t0, p);
+        w.softmax(s, t0, p);
 #pragma unroll
         for (int b = 0; b < KK; b++) {
             bf16x8 even, odd;
             v_operands<KK>(raw[0].v, raw[1].v, vs, b, even, odd);
 #pragma unroll
             for (int e = Wave::PIECES - 1; e >= 0; e--) {
-                w.acc[0][2 * b]     = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p[e], w.acc[0][2 * b], 0, 0, 0);
-                w.acc[0][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p[e], w.acc[0][2 * b + 1], 0, 0, 0);
+                w.acc[2 * b]     = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p[e], w.acc[2 * b], 0, 0, 0);
+                w.acc[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p[e], w.acc[2 * b + 1], 0, 0, 0);
             }
         }
     };
@@ -582,19 +569,19 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
     __shared__ __attribute__((aligned(16))) float s_o[W][COLS][HDP + 4];
     const bool writes = !PACK || w.piece == 0;
     if (w.g == 0 && writes)
-        s_m[wave][w.lcol] = w.m[0], s_l[wave][w.lcol] = w.l[0];
+        s_m[wave][w.lcol] = w.m, s_l[wave][w.lcol] = w.l;
     __syncthreads();
     float M = -INFINITY;
 #pragma unroll
     for (int x = 0; x < W; x++)
         M = fmaxf(M, s_m[x][w.lcol]);
-    const float alpha = w.m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m[0] - M);
+    const float alpha = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - M);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int ct = 0; ct < 2 * KK; ct++)
             if (writes)
-                s_o[wave][w.lcol][(4 * w.g + i) * 2 * KK + ct] = w.acc[0][ct][i] * alpha;
+                s_o[wave][w.lcol][(4 * w.g + i) * 2 * KK + ct] = w.acc[ct][i] * alpha;
     __syncthreads();
     for (int e = threadIdx.x; e < COLS * (HDP / 4); e += 64 * W) {
         const int col = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
@@ -639,14 +626,14 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
 // Bound by the matrix instructions (48 for a tile of columns, a step and 128 channels) once the codes are turned into operands
 // only once: the four waves of a workgroup convert a quarter of a step's K and V each into LDS, a step ahead, and read all
 // of it as 16-byte operands.  One barrier a step: a buffer is written while the other is read.  Three chunks of up to 1500 rows
-// behind up to 4000 tokens, 32 heads of 128 channels: 435 us for 497 GFLOP of products, 1140 TFLOP/s, where a large library
-// product of bf16 reaches 1180 (each wave converting for itself: 684 us; one tile of columns a wave instead of two 2 % more).
+// behind up to 4000 tokens, 32 heads of 128 channels: 433 us for 497 GFLOP of products, 1150 TFLOP/s, where a large library
+// product of bf16 reaches 1180 (each wave converting for itself: 684 us).  Two tiles of columns a wave halve the operands read but leave
+// room for two workgroups a CU and not three: as fast there, and 34 us instead of 26 for a prompt of 512 tokens, 135 instead of 100 for 2048.
 // With 64 channels and fewer the vector work of the softmax, which stays the same, is what bounds it.
-template <int KK, int NC>
-__global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 : 2) nvk_mx4_prefill_kernel(const Mx4AttnArgs a)
+template <int KK> __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : 3) nvk_mx4_prefill_kernel(const Mx4AttnArgs a)
 {
-    using Wave = Mx4Wave<KK, NC, false>;
-    constexpr int COLS = Wave::COLS * NC, W = kPrefillWaves;
+    using Wave = Mx4Wave<KK, false>;
+    constexpr int COLS = Wave::COLS, W = kPrefillWaves;
     __shared__ __attribute__((aligned(16))) bf16x8 s_k[2][2 * KK][64], s_v[2][2 * KK][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -678,7 +665,7 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 
     const Mx4Tiles      tiles(a, seq, kvh, (min(end, ctx) - 1) / kMx4Tile);
     const Mx4Places<KK> places(w.lane);
     const int           tile_j = wave & 1; // (W is even: all K items of a wave lie in one tile)
-    constexpr int       AHEAD = KK == 2 ? 2 : 1; // steps whose codes are on their way (64 channels: 5 % less time; 32: 25 % more)
+    constexpr int       AHEAD = KK == 2 ? 2 : 1; // steps whose codes are on their way (two: 64 channels 3 % less time, 32 and 128 a sixth more and beyond)
     Mx4Raw<KK>          ring[AHEAD][2];
     int                 entry = 0; // lane L: tile L of the current 32 steps
     auto                fetch = [&](int i, Mx4Raw<KK> (&raw)[2]) {
@@ -722,33 +709,22 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 
         }
         const int t0 = begin + 32 * i, buf = i & 1;
         if (t0 < w.most) {
-            f32x4 s[NC][2];
-#pragma unroll
-            for (int n = 0; n < NC; n++)
-                s[n][0] = w.origin(n), s[n][1] = w.origin(n);
+            f32x4 s[2] = {w.origin(), w.origin()};
 #pragma unroll
             for (int e = 0; e < 3; e++)
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const bf16x8 k = s_k[buf][kk * 2 + j][w.lane];
-#pragma unroll
-                        for (int n = 0; n < NC; n++)
-                            s[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, w.q[n][kk][e], s[n][j], 0, 0, 0);
-                    }
-            bf16x8 p[NC][3];
-#pragma unroll
-            for (int n = 0; n < NC; n++)
-                w.softmax(n, s[n], t0, p[n]);
+                    for (int j = 0; j < 2; j++)
+                        s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(s_k[buf][kk * 2 + j][w.lane], w.q[kk][e], s[j], 0, 0, 0);
+            bf16x8 p[3];
+            w.softmax(s, t0, p);
 #pragma unroll
             for (int ct = 0; ct < 2 * KK; ct++) {
                 const bf16x8 v = s_v[buf][ct][w.lane];
 #pragma unroll
-                for (int n = 0; n < NC; n++)
-#pragma unroll
-                    for (int e = 2; e >= 0; e--)
-                        w.acc[n][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n][e], w.acc[n][ct], 0, 0, 0);
+                for (int e = 2; e >= 0; e--)
+                    w.acc[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[e], w.acc[ct], 0, 0, 0);
             }
         }
         __syncthreads();
@@ -760,35 +736,32 @@ __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : NC == 1 ? 3 
                 step(i + d, ring[(d + 1) % AHEAD]);
     w.finish();
 
+    if (w.out_row < 0)
+        return;
+    const int64_t line = (int64_t)w.out_row * a.n_heads + w.out_head;
+    float        *dst = a.out + line * a.mx.head_dim;
+    float         norm = w.l == 0.f ? 0.f : 1.f / w.l;
+    if (a.chunks > 1) {
+        dst  = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim;
+        norm = 1.f;
+        if (w.g == 0) {
+            a.ws_ml[(line * a.chunks + chunk) * 2]     = w.m;
+            a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = w.l;
+        }
+    }
+    // (a lane holds runs of 2 KK channels: a run, or a half of sixteen, is in the row as a whole)
 #pragma unroll
-    for (int n = 0; n < NC; n++) {
-        if (w.out_row[n] < 0)
-            continue;
-        const int64_t line = (int64_t)w.out_row[n] * a.n_heads + w.out_head[n];
-        float        *dst = a.out + line * a.mx.head_dim;
-        float         norm = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
-        if (a.chunks > 1) {
-            dst  = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim;
-            norm = 1.f;
-            if (w.g == 0) {
-                a.ws_ml[(line * a.chunks + chunk) * 2]     = w.m[n];
-                a.ws_ml[(line * a.chunks + chunk) * 2 + 1] = w.l[n];
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int ct = 0; ct < 2 * KK; ct += KK == 1 ? 2 : 4) {
+            const int c = (4 * w.g + i) * 2 * KK + ct;
+            if (c < a.mx.head_dim) {
+                if constexpr (KK == 1)
+                    dst[c] = w.acc[ct][i] * norm, dst[c + 1] = w.acc[ct + 1][i] * norm;
+                else
+                    store_four(dst + c, w.acc[ct][i] * norm, w.acc[ct + 1][i] * norm, w.acc[ct + 2][i] * norm, w.acc[ct + 3][i] * norm);
             }
         }
-        // (a lane holds runs of 2 KK channels: a run, or a half of sixteen, is in the row as a whole)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int ct = 0; ct < 2 * KK; ct += KK == 1 ? 2 : 4) {
-                const int c = (4 * w.g + i) * 2 * KK + ct;
-                if (c < a.mx.head_dim) {
-                    if constexpr (KK == 1)
-                        dst[c] = w.acc[n][ct][i] * norm, dst[c + 1] = w.acc[n][ct + 1][i] * norm;
-                    else
-                        store_four(dst + c, w.acc[n][ct][i] * norm, w.acc[n][ct + 1][i] * norm, w.acc[n][ct + 2][i] * norm, w.acc[n][ct + 3][i] * norm);
-                }
-            }
-    }
 }
 
 // How many chunks the line of a (row, head) has, 0 where nothing is to be joined.
@@ -847,7 +820,6 @@ namespace {
 using nvk::Mx4AttnArgs;
 
 using nvk::kDecodeWaves, nvk::kPrefillWaves;
-constexpr int prefill_cols(int kk) { return kk == 8 ? 1 : 2; } // columns of a prefill wave: 16 times this (registers)
 
 struct Mx4Shape
 {
@@ -867,19 +839,21 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     // would work on up to 16.
     s.prefill = (long long)max_rows * group > 16;
     s.pack    = (long long)max_rows * group <= 4;
-    s.col_blocks = s.prefill ? ceil_div((long long)max_rows * group, 16 * prefill_cols(pool->kk) * kPrefillWaves) : 1;
+    s.col_blocks = s.prefill ? ceil_div((long long)max_rows * group, 16 * kPrefillWaves) : 1;
     const long long tasks = (long long)num_seqs * pool->n_kv_heads * s.col_blocks;
     // Cut the context while everything still runs at once (workgroups of four waves: so many fit a CU), into chunks of 192
     // tokens at least (a step of the four waves is 128; prefill's waves share the tokens: 64); not into more than can be joined
     // inside unless those were long.  (In chunks of 64, 128, 192, 256 tokens: 1 x 200 7.4, 6.3, 6.3, 6.2 us, 1 x 1000 8.6, 8.6, 8.3,
     // 9.0, 230 x 256 9.7, 9.7, 7.0, 7.1; 64 x 2048, two workgroups a CU: 28.1 us uncut, 39.6 in two rounds.)
-    long long fit = (pool->kk == 8 ? 1LL : s.pack ? 3LL : 2LL) * pool->num_cus;
-    // A prompt's early rows see few of the chunks: half as many again where all rows are new.  (1157 rows: 35.6 us in 3 chunks,
-    // 32.2 in 4, 39.6 in 6; 128 rows behind 8064 tokens: 65.3 in 16, 82.4 in 24.  Not with 256 channels, one workgroup a CU: 700 rows
-    // 80 uncut, 93 in 2.)
-    if (s.prefill && pool->kk <= 4)
-        fit += fit * std::min(max_rows, max_ctx) / (2LL * std::max(max_ctx, 1));
+    // Prompts with narrow heads are cut finer, more workgroups fit.  (1157 rows of 48 channels: 36.8 us uncut, 31.6 in 2, 26.9 in 3.)
+    const long long per_cu = pool->kk == 8 ? 1 : s.prefill ? (pool->kk <= 2 ? 4 : 2) : s.pack ? 3 : 2, fit = per_cu * pool->num_cus;
     s.chunks = (int)std::max(1LL, std::min(fit / std::max(tasks, 1LL), (long long)max_ctx / (s.prefill ? 64 : 192)));
+    // A prompt is cut where that saves more than the join costs: a step of 32 tokens takes about 1 us, the join 4 us and its reads and
+    // writes at 5 TB/s.  (128 rows of 32 heads of 128 channels: 10.4 us uncut, 13.6 in 2; 256: 15.5 and 19.1 in 4; 512: 25.7 and 29.5 in 2;
+    // 512 behind 512: 44.5 and 43.1 in 2.)
+    if (s.prefill && s.chunks > 1
+        && (max_ctx - max_ctx / s.chunks) / 32 < 4 + (long long)total_rows * n_heads * pool->head_dim * s.chunks * 8 / 5000000)
+        s.chunks = 1;
     if (!s.prefill && s.chunks > nvk::kJoinInside && max_ctx <= 512 * nvk::kJoinInside)
         s.chunks = nvk::kJoinInside;
     s.chunk_tokens = std::max(32, ceil_div(ceil_div(max_ctx, s.chunks), 32) * 32);
@@ -897,20 +871,20 @@ int reserve(nvk_mx4_pool *pool, size_t floats, size_t arrivals, hipStream_t st, 
 }
 
 // What no call of up to this shape passes, fewer sequences (which are cut into more chunks) among them: as mx4_shape cuts, lines times
-// chunks are at most the workgroups that fit the chip, half as many again for prompts, times the columns of one.
+// chunks are at most the workgroups that fit the chip times the columns of one.
 size_t most_floats(const nvk_mx4_pool *pool, int n_heads, int total_rows, int max_rows, int max_ctx)
 {
     const long long columns = (long long)max_rows * (n_heads / pool->n_kv_heads), lines = (long long)total_rows * n_heads;
     long long       most = std::max(3 * std::min(columns, 4LL), 2 * std::min(columns, 16LL));
     if (columns > 16)
-        most = std::max(most, 3 * std::min(columns, 16LL * prefill_cols(pool->kk) * kPrefillWaves));
+        most = std::max(most, 4 * std::min(columns, 16LL * kPrefillWaves));
     return (size_t)std::min(most * pool->num_cus, lines * (max_ctx / 64)) * (size_t)(pool->head_dim + 2);
 }
 
 template <int KK> void launch_attn(const Mx4AttnArgs &a, const Mx4Shape &s, unsigned blocks, hipStream_t st)
 {
     if (s.prefill)
-        hipLaunchKernelGGL((nvk::nvk_mx4_prefill_kernel<KK, prefill_cols(KK)>), dim3(blocks), dim3(64 * kPrefillWaves), 0, st, a);
+        hipLaunchKernelGGL(nvk::nvk_mx4_prefill_kernel<KK>, dim3(blocks), dim3(64 * kPrefillWaves), 0, st, a);
     else if (s.pack)
         hipLaunchKernelGGL((nvk::nvk_mx4_decode_kernel<KK, true>), dim3(blocks), dim3(64 * kDecodeWaves), 0, st, a);
     else
