@@ -45,10 +45,10 @@ struct SparseArgs
     const int   *tables, *ctx_lens, *starts; // starts: index update only
     int          num_seqs, max_blocks, n_heads, group, n_kv_heads, head_dim, num_blocks, block_size;
     int          top, first, last;
-    float       *scores; // [num_seqs, n_kv_heads, max_nb]
+    float       *scores;   // [num_seqs, n_kv_heads, max_nb]
     int         *chosen;   // [num_seqs, n_kv_heads, top]: what the selection kernel makes, of lines with more blocks than `top`
     int         *selected; // the caller's list of the same shape, of all lines, or null
-    int          max_nb; // blocks of the longest context
+    int          max_nb;                   // blocks of the longest context
     int          blocks_per_wave;          // score
     int          blocks_per_chunk, chunks; // attend
     int          head_sets;                // attend: workgroups along the group's heads
