@@ -583,6 +583,7 @@ int reserve_hidden_rows(nvk_batch *b, int rows, int dim)
     if ((size_t)rows <= b->h_rows && (size_t)dim <= b->h_dim && qdim <= b->h_qdim)
         return NVK_OK;
     HIP_TRY(hipDeviceSynchronize()); // earlier launches may still use the old ones
+    b->hidden_generation++;          // (now and not with the new ones, which may not come)
     for (float **p : {&b->h_q, &b->h_k, &b->h_v, &b->h_xb})
         if (*p) {
             (void)hipFree(*p);
@@ -595,7 +596,6 @@ int reserve_hidden_rows(nvk_batch *b, int rows, int dim)
     HIP_TRY(hipMalloc((void **)&b->h_v, r * b->row_len * sizeof(float)));
     HIP_TRY(hipMalloc((void **)&b->h_xb, r * d * sizeof(float)));
     b->h_rows = r, b->h_dim = d, b->h_qdim = qdim;
-    b->hidden_generation++;
     return NVK_OK;
 }
 

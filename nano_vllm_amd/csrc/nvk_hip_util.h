@@ -32,52 +32,49 @@ inline bool stream_is_capturing(hipStream_t stream)
     return stream && hipStreamIsCapturing(stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
 }
 
-// A workspace of at least `floats`, freed and allocated again when it has to grow.  Never while `stream` records a graph
+// A buffer of at least `want` elements, freed and allocated again when it has to grow.  Never while `stream` records a graph
 // (the graph would keep the old address; hipMalloc is not capturable): refused, with the remedy in the message.
-inline int grow_workspace(float **ws, size_t *have, long long *generation, size_t floats, hipStream_t stream, const char *who)
+// The generation moves before the old buffer goes, not with the new one: where no memory is left for that, a graph which holds
+// the old address must not be replayed either.
+template <class T>
+inline int grow_buffer(T **buf, size_t *have, long long *generation, size_t want, hipStream_t stream, const char *who)
 {
-    if (floats <= *have)
+    if (want <= *have)
         return NVK_OK;
     if (stream_is_capturing(stream))
         return fail(NVK_ERR_INVALID_ARG,
                     "%s: the workspace would have to grow while the stream is being captured: size it first, outside the "
                     "capture (the reserve_workspace entry point, or one direct call of the same shape)", who);
-    NVK_HIP_TRY(hipDeviceSynchronize()); // launches on any stream may still use the old buffer
-    if (*ws)
-        NVK_HIP_TRY(hipFree(*ws));
-    *ws = nullptr, *have = 0;
-    NVK_HIP_TRY(hipMalloc((void **)ws, floats * sizeof(float)));
-    *have = floats;
+    if (*buf) {
+        NVK_HIP_TRY(hipDeviceSynchronize()); // launches on any stream may still use the old buffer
+        ++*generation;
+        NVK_HIP_TRY(hipFree(*buf));
+        *buf = nullptr, *have = 0;
+    }
+    NVK_HIP_TRY(hipMalloc((void **)buf, want * sizeof(T)));
+    *have = want;
     ++*generation;
     return NVK_OK;
 }
 
-// Counters that every launch finds at zero and leaves at zero, grown like the workspace.
+// Counters that every launch finds at zero and leaves at zero, grown like a workspace.
 inline int grow_counters(int **counters, size_t *have, long long *generation, size_t want, hipStream_t stream, const char *who)
 {
     if (want <= *have)
         return NVK_OK;
     want = want < 4096 ? 4096 : want;
-    int *fresh = nullptr;
-    if (stream_is_capturing(stream))
-        return fail(NVK_ERR_INVALID_ARG,
-                    "%s: the workspace would have to grow while the stream is being captured: size it first, outside the "
-                    "capture (the reserve_workspace entry point, or one direct call of the same shape)", who);
-    NVK_HIP_TRY(hipDeviceSynchronize()); // launches on any stream may still use the old ones
-    if (*counters)
-        NVK_HIP_TRY(hipFree(*counters));
-    *counters = nullptr, *have = 0;
-    NVK_HIP_TRY(hipMalloc((void **)&fresh, want * sizeof(int)));
+    const int rc = grow_buffer(counters, have, generation, want, stream, who);
+    if (rc != NVK_OK)
+        return rc;
     // (the fill may still run when hipMemset returns, and a non-blocking stream does not wait for it)
-    hipError_t e = hipMemset(fresh, 0, want * sizeof(int));
+    hipError_t e = hipMemset(*counters, 0, want * sizeof(int));
     if (e == hipSuccess)
         e = hipDeviceSynchronize();
     if (e != hipSuccess) {
-        (void)hipFree(fresh);
+        (void)hipFree(*counters);
+        *counters = nullptr, *have = 0;
         return fail(NVK_ERR_HIP, "%s: clearing the counters failed: %s", who, hipGetErrorString(e));
     }
-    *counters = fresh, *have = want;
-    ++*generation;
     return NVK_OK;
 }
 

@@ -866,7 +866,7 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
 
 int reserve(nvk_mx4_pool *pool, size_t floats, size_t arrivals, hipStream_t st, const char *who)
 {
-    const int rc = nvk::grow_workspace(&pool->ws, &pool->ws_floats, &pool->ws_generation, floats, st, who);
+    const int rc = nvk::grow_buffer(&pool->ws, &pool->ws_floats, &pool->ws_generation, floats, st, who);
     return rc != NVK_OK ? rc : nvk::grow_counters(&pool->arrivals, &pool->arrivals_cap, &pool->ws_generation, arrivals, st, who);
 }
 

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "nvk_device_scope.h"
+#include "nvk_hip_util.h"
 #include "nvk_internal.h"
 #include "nvk_kernels.hip.h"
 
@@ -226,37 +227,13 @@ int ensure_workspace(nvk_pool *pool, size_t o_floats, size_t ml_floats, size_t a
     int rc = refuse_growth_under_capture(stream, "the split-K workspace");
     if (rc != NVK_OK)
         return rc;
-    HIP_TRY(hipDeviceSynchronize()); // launches on any stream may still use the old buffers
-    if (o_floats > pool->ws_o_floats) {
-        if (pool->ws_o)
-            HIP_TRY(hipFree(pool->ws_o));
-        pool->ws_o = nullptr, pool->ws_o_floats = 0;
-        HIP_TRY(hipMalloc(&pool->ws_o, o_floats * sizeof(float)));
-        pool->ws_o_floats = o_floats;
-        pool->ws_generation++;
-    }
-    if (ml_floats > pool->ws_ml_floats) {
-        if (pool->ws_ml)
-            HIP_TRY(hipFree(pool->ws_ml));
-        pool->ws_ml = nullptr, pool->ws_ml_floats = 0;
-        HIP_TRY(hipMalloc(&pool->ws_ml, ml_floats * sizeof(float)));
-        pool->ws_ml_floats = ml_floats;
-        pool->ws_generation++;
-    }
-    if (arrival_ints > pool->arrivals_cap) {
-        if (pool->arrivals)
-            HIP_TRY(hipFree(pool->arrivals));
-        pool->arrivals = nullptr, pool->arrivals_cap = 0;
-        const size_t want = std::max(arrival_ints, (size_t)4096);
-        HIP_TRY(hipMalloc(&pool->arrivals, want * sizeof(int)));
-        // (hipMemset on the null stream may return before the fill has run, and the pool's stream is non-blocking:
-        // it does not wait for the null stream.  The first launch must find zeros: fill, then wait for the device.)
-        HIP_TRY(hipMemset(pool->arrivals, 0, want * sizeof(int)));
-        HIP_TRY(hipDeviceSynchronize());
-        pool->arrivals_cap = want;
-        pool->ws_generation++;
-    }
-    return NVK_OK;
+    const char *who = "the split-K workspace";
+    rc = nvk::grow_buffer(&pool->ws_o, &pool->ws_o_floats, &pool->ws_generation, o_floats, stream, who);
+    if (rc == NVK_OK)
+        rc = nvk::grow_buffer(&pool->ws_ml, &pool->ws_ml_floats, &pool->ws_generation, ml_floats, stream, who);
+    if (rc == NVK_OK) // (zeros: each launch's arrivals leave them so)
+        rc = nvk::grow_counters(&pool->arrivals, &pool->arrivals_cap, &pool->ws_generation, arrival_ints, stream, who);
+    return rc;
 }
 
 // inv_freq[p] = 1 / powf(theta, 2p / head_dim): the reference's own expression (ops/positional.hpp:16,
@@ -587,7 +564,7 @@ struct nvk_plan
     bool          built = false;
     nvk::WorkItem *items = nullptr;
     int          *counters = nullptr; // [0] = n_items, [1 + s] = chunks of sequence s
-    size_t        cap_items = 0, cap_seqs = 0;
+    size_t        cap_items = 0, cap_counters = 0;
     int           item_bound = 0; // grid.x: at least as many workgroups as items
     long long     generation = 0; // bumped whenever items / counters move (a captured graph holds their addresses)
     // direct indexing (NVK_DECODE_UNIFORM / NVK_DECODE_NO_PLAN): no work list; the kernels read the lengths themselves
@@ -600,36 +577,18 @@ namespace {
 
 int plan_reserve(nvk_plan *plan, size_t items, size_t seqs, hipStream_t stream)
 {
-    if (items > plan->cap_items || seqs > plan->cap_seqs) {
+    if (items > plan->cap_items || seqs + 1 > plan->cap_counters) {
         int rc = refuse_growth_under_capture(stream, "the decode plan");
         if (rc != NVK_OK)
             return rc;
     }
-    if (items > plan->cap_items) {
-        if (plan->items) {
-            HIP_TRY(hipDeviceSynchronize());
-            HIP_TRY(hipFree(plan->items));
-            plan->items     = nullptr;
-            plan->cap_items = 0;
-        }
-        const size_t want = std::max(items, (size_t)1024);
-        HIP_TRY(hipMalloc(&plan->items, want * sizeof(nvk::WorkItem)));
-        plan->cap_items = want;
-        plan->generation++;
-    }
-    if (seqs > plan->cap_seqs) {
-        if (plan->counters) {
-            HIP_TRY(hipDeviceSynchronize());
-            HIP_TRY(hipFree(plan->counters));
-            plan->counters = nullptr;
-            plan->cap_seqs = 0;
-        }
-        const size_t want = std::max(seqs, (size_t)1024);
-        HIP_TRY(hipMalloc(&plan->counters, (want + 1) * sizeof(int)));
-        plan->cap_seqs = want;
-        plan->generation++;
-    }
-    return NVK_OK;
+    const char *who = "the decode plan";
+    int         rc  = NVK_OK;
+    if (items > plan->cap_items)
+        rc = nvk::grow_buffer(&plan->items, &plan->cap_items, &plan->generation, std::max(items, (size_t)1024), stream, who);
+    if (rc == NVK_OK && seqs + 1 > plan->cap_counters)
+        rc = nvk::grow_buffer(&plan->counters, &plan->cap_counters, &plan->generation, std::max(seqs, (size_t)1024) + 1, stream, who);
+    return rc;
 }
 
 // The host half of a plan: launch shape and planning mode for a batch.  Touches no device memory.

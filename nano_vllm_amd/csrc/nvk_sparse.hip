@@ -849,7 +849,7 @@ SparseShape sparse_shape(const nvk_block_index *x, int num_seqs, int n_heads, in
 
 int reserve(nvk_block_index *x, size_t floats, size_t arrivals, hipStream_t st, const char *who)
 {
-    const int rc = nvk::grow_workspace(&x->ws, &x->ws_floats, &x->ws_generation, floats, st, who);
+    const int rc = nvk::grow_buffer(&x->ws, &x->ws_floats, &x->ws_generation, floats, st, who);
     return rc != NVK_OK ? rc : nvk::grow_counters(&x->arrivals, &x->arrivals_cap, &x->ws_generation, arrivals, st, who);
 }
 
