@@ -163,6 +163,9 @@ template <bool SHARED> __global__ void __launch_bounds__(64 * kSparseWaves) nvk_
     *reinterpret_cast<float4 *>(to + a.head_dim) = hi;
 }
 
+// min(q, 0) for the least key element, max(q, 0) for the largest; a NaN stays one (fminf and fmaxf would make it 0)
+__device__ __forceinline__ float weight_of(float q, bool low) { return (low ? q > 0.f : q < 0.f) ? 0.f : q; }
+
 // ---- scores ---------------------------------------------------------------------------------------------------------
 // With w = [min(q, 0) | max(q, 0)] a bound is the dot product of w with a block's [lo | hi], 2 head_dim contiguous floats.  It is
 // summed in 64 bits (every product of two fp32 numbers is exact there) and rounded once: which of two close blocks is
@@ -200,8 +203,8 @@ template <int NV, int HG> __global__ void __launch_bounds__(64 * kSparseWaves) n
                     x = *reinterpret_cast<const float4 *>(
                         a.q + ((int64_t)seq * a.n_heads + kvh * a.group + min(h0 + h, a.group - 1)) * hd + (c < hd ? c : c - hd));
                 const bool low = c < hd;
-                w[h][j][0] = low ? fminf(x.x, 0.f) : fmaxf(x.x, 0.f), w[h][j][1] = low ? fminf(x.y, 0.f) : fmaxf(x.y, 0.f);
-                w[h][j][2] = low ? fminf(x.z, 0.f) : fmaxf(x.z, 0.f), w[h][j][3] = low ? fminf(x.w, 0.f) : fmaxf(x.w, 0.f);
+                w[h][j][0] = weight_of(x.x, low), w[h][j][1] = weight_of(x.y, low);
+                w[h][j][2] = weight_of(x.z, low), w[h][j][3] = weight_of(x.w, low);
             }
         constexpr int RING = NV < 8 ? 3 : 2; // groups of four blocks: one in work, the others on their way
         float4        x[RING][NV];
@@ -307,8 +310,8 @@ __global__ void __launch_bounds__(64 * kSparseWaves, NV == 4 ? 1 : 2) nvk_block_
                 x = *reinterpret_cast<const float4 *>(
                     a.q + ((int64_t)seq * a.n_heads + kvh * a.group + min(h0 + l16, a.group - 1)) * hd + (c < hd ? c : c - hd));
             const bool low = c < hd;
-            w[j][0] = low ? fminf(x.x, 0.f) : fmaxf(x.x, 0.f), w[j][1] = low ? fminf(x.y, 0.f) : fmaxf(x.y, 0.f);
-            w[j][2] = low ? fminf(x.z, 0.f) : fmaxf(x.z, 0.f), w[j][3] = low ? fminf(x.w, 0.f) : fmaxf(x.w, 0.f);
+            w[j][0] = weight_of(x.x, low), w[j][1] = weight_of(x.y, low);
+            w[j][2] = weight_of(x.z, low), w[j][3] = weight_of(x.w, low);
         }
         auto fetch = [&](float4 (&to)[J], int t) {
             const int    at = min(16 * t + l16, end - 1 - begin), lo = __shfl(entry[0], at & 63), hi = __shfl(entry[1], at & 63);
