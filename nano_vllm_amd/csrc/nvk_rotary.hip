@@ -435,6 +435,9 @@ int norm_rope_append(RotaryArgs a, int device, hipStream_t own_stream, const nvk
     if (!nvk::for_floats(a.q) || !nvk::for_floats(a.q_out) || !nvk::for_floats(a.k) || !nvk::for_floats(a.v))
         return nvk::fail(NVK_ERR_INVALID_ARG, "%s: rows are not aligned to their type", who);
 
+    if (!a.k) // (positions alone matter: what else is given may be of any size)
+        a.row_seqs = a.tables = nullptr;
+
     NVK_SCOPE(device);
     hipStream_t st = (ptr_kind == NVK_PTR_DEVICE && stream) ? (hipStream_t)stream : own_stream;
     a.inv_head_dim = 1.0 / hd;
