@@ -17,6 +17,16 @@ HELD_BACK = {
 }
 
 
+def reference_expected(root):
+    """Whether a library built from the reference belongs to this tree: unless the build said that it had no reference to build
+    from (`make ref` leaves oracle/ref_state, beside the folder that can get lost)."""
+    try:
+        with open(os.path.join(root, "oracle", "ref_state")) as fh:
+            return fh.read().strip() != "no reference"
+    except OSError:
+        return True
+
+
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
@@ -31,10 +41,8 @@ def pytest_collection_modifyitems(config, items):
             item.add_marker(pytest.mark.skip(reason=HELD_BACK[item.originalname]))
 
     if nano_vllm_amd.device_count() > 0:
-        # a GPU run gets its tree from the build container, where oracle/_ref/ was built from the reference: the
-        # engine drop-in tests then FAIL rather than skip when that library did not travel (NVK_EXPECT_REF=0 opts out).
-        # Where the build had no reference to build from there is no oracle/_ref/ at all, and they skip.
-        os.environ.setdefault("NVK_EXPECT_REF", "1" if os.path.isdir(os.path.join(ROOT, "oracle", "_ref")) else "0")
+        # the engine drop-in tests FAIL rather than skip when the built library did not travel (NVK_EXPECT_REF=0 opts out)
+        os.environ.setdefault("NVK_EXPECT_REF", "1" if reference_expected(ROOT) else "0")
         return
     skip = pytest.mark.skip(reason="no HIP device visible")
     for item in items:
