@@ -14,7 +14,8 @@ LIB     := nano_vllm_amd/libnvk_paged_attn.so
 # No packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this machine.
 # (A device feature: hipcc's host pass says that it does not know it, which is harmless.)
 HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Iinclude -I$(CSRC) -Wall -Wno-unused-function -fno-gpu-rdc \
-            -Xclang -target-feature -Xclang -packed-fp32-ops
+            -Xclang -target-feature -Xclang -packed-fp32-ops $(EXTRA)
+EXTRA    ?=
 OBJ      := build/obj
 HIP_SRC  := nvk_paged_attn nvk_batch nvk_linear nvk_model nvk_shard nvk_rotary nvk_mx4 nvk_sparse
 CPP_SRC  := nvk_block_manager nvk_tokenizer nvk_model_group
@@ -28,14 +29,15 @@ lib: $(LIB)
 
 # one object per source (make -j builds them side by side; without -fgpu-rdc each carries its own device code)
 $(OBJ)/%.o: $(CSRC)/%.hip $(HEADERS) Makefile
-	@mkdir -p $(OBJ)
+	@mkdir -p $(@D)
 	$(HIPCC) $(HIPFLAGS) -c -o $@ $<
 
 $(OBJ)/%.o: $(CSRC)/%.cpp $(HEADERS) Makefile
-	@mkdir -p $(OBJ)
+	@mkdir -p $(@D)
 	$(HIPCC) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Iinclude -I$(CSRC) -Wall -c -o $@ $<
 
 $(LIB): $(OBJS)
+	@mkdir -p $(@D)
 	$(HIPCC) --offload-arch=$(ARCH) -shared -fPIC -o $@ $(OBJS) -ldl -lpthread
 
 # the reference's command line over the library (tools/nvk_run.cpp): host-only C++ over the C ABI
@@ -44,11 +46,13 @@ cli: $(CLI)
 $(CLI): tools/nvk_run.cpp include/nvk_paged_attn.h $(LIB)
 	g++ -std=c++17 -O2 -Wall -Iinclude -o $@ tools/nvk_run.cpp -Lnano_vllm_amd -lnvk_paged_attn -Wl,-rpath,'$$ORIGIN'
 
-# device assembly + register/occupancy report for the kernels (not needed to run)
-asm:
-	mkdir -p build/asm
-	$(HIPCC) --offload-arch=$(ARCH) -O3 -std=c++17 -Iinclude -I$(CSRC) -save-temps=obj -c \
-	   -Rpass-analysis=kernel-resource-usage -o build/asm/nvk_paged_attn.o $(CSRC)/nvk_paged_attn.hip 2> build/resource_usage.txt
+# device assembly + register/occupancy report for the kernels as they are shipped (not needed to run)
+asm: $(HIP_SRC:%=build/asm/%.o)
+	cat $(HIP_SRC:%=build/asm/%.remarks) > build/resource_usage.txt
+
+build/asm/%.o: $(CSRC)/%.hip $(HEADERS) Makefile
+	@mkdir -p $(@D)
+	$(HIPCC) $(HIPFLAGS) -save-temps=obj -c -Rpass-analysis=kernel-resource-usage -o $@ $< 2> build/asm/$*.remarks
 
 # Host code under AddressSanitizer + UndefinedBehaviorSanitizer (CPU build only; the pool runs no GPU sanitizer):
 # the block allocator, the tokenizer and the CPU checker behind tests/asan_driver.cpp, and the command line
