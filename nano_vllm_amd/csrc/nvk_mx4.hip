@@ -275,8 +275,9 @@ template <int KK, bool PACK> struct Mx4Wave
 
     // A group of V that holds no number (scale byte 255): its scale is taken as 0, and the columns that see the token are marked.
     // (One of K makes its token's scores NaN by itself.)  `vs`: the lane's V scales of the two tiles from token t0 on.
-    // Always before any product of a step: this compiler does not keep the wait between a matrix instruction and the first
-    // read of its result across a branch, so none may stand there.
+    // Before any product of a step: an earlier form of these kernels had its branches behind the score products, with results in
+    // accumulation registers, and a first read one slot behind across a branch; its scores differed from run to run.  Where
+    // a branch stands there now (`softmax`) the compiler pads both ways; a walk over every path of the built kernels checks it.
     __device__ __forceinline__ void mark(unsigned (&vs)[2], int t0)
     {
         if (__any((byte_255(vs[0]) | byte_255(vs[1])) != 0)) {

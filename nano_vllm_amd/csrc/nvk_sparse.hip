@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(64 * kSparseWaves, NV == 4 ? 1 : 2) nvk_block_
                     to[j] = *reinterpret_cast<const float4 *>(src + c);
             }
         };
-        // (no branch between the products and what reads them: the compiler does not keep the wait for a result across one)
+        // (no branch between the products and what reads them: a wait for a result was once seen lost across one)
         auto take = [&](const float4 (&x)[J], int t) {
             f64x4 s0 = {0.0, 0.0, 0.0, 0.0}, s1 = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
