@@ -14,8 +14,10 @@ namespace nvk {
 
 constexpr int kJoinThreads = 256; // a workgroup per line; head_dim <= 256
 
-// `o` [n][hd] and `ml` [n][2] of the line -> out [hd].  A line without a token (every l_c 0) gives zeros.
-__device__ __forceinline__ void join_chunks(const float *__restrict__ o, const float *__restrict__ ml, int n, int hd, float *__restrict__ out)
+// `o` [n][hd] and `ml` [n][2] of the line -> out [hd].  `empty`: a line that sees no token gives zeros (one whose scores are all
+// -infinity is 0 / 0, no number).
+__device__ __forceinline__ void join_chunks(const float *__restrict__ o, const float *__restrict__ ml, int n, int hd, bool empty,
+                                            float *__restrict__ out)
 {
     constexpr int W = kJoinThreads / 64;
     __shared__ float s_o[W][256];
@@ -62,7 +64,7 @@ __device__ __forceinline__ void join_chunks(const float *__restrict__ o, const f
     __syncthreads();
     for (int c = threadIdx.x; c < hd; c += kJoinThreads) {
         const float sum = (s_o[0][c] + s_o[1][c]) + (s_o[2][c] + s_o[3][c]);
-        out[c]          = L == 0.f ? sum : sum / L; // (no token: 0, or no number where one was met)
+        out[c]          = empty ? 0.f : sum / L;
     }
 }
 
@@ -104,7 +106,7 @@ __device__ __forceinline__ bool arrived_last(int *counter, int n)
 
 // Four channels of a line from its n <= kJoinInside chunks, stored hd (o) and 2 (ml) floats apart; THROUGH: by other workgroups
 // of this launch.
-template <bool THROUGH> __device__ __forceinline__ float4 join_few(const float *o, const float *ml, int n, int hd)
+template <bool THROUGH> __device__ __forceinline__ float4 join_few(const float *o, const float *ml, int n, int hd, bool empty)
 {
     float4 y[kJoinInside];
     float2 w[kJoinInside];
@@ -134,9 +136,7 @@ template <bool THROUGH> __device__ __forceinline__ float4 join_few(const float *
             L += w[c].y * f;
             x.x += y[c].x * f, x.y += y[c].y * f, x.z += y[c].z * f, x.w += y[c].w * f;
         }
-    if (L != 0.f)
-        x.x /= L, x.y /= L, x.z /= L, x.w /= L;
-    return x;
+    return empty ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x / L, x.y / L, x.z / L, x.w / L);
 }
 
 } // namespace nvk

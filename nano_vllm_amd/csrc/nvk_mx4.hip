@@ -584,6 +584,8 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
             if (writes)
                 s_o[wave][w.lcol][(4 * w.g + i) * 2 * KK + ct] = w.acc[ct][i] * alpha;
     __syncthreads();
+    // (zeros for a row that sees no token; one whose scores are all -infinity is 0 / 0, no number)
+    auto sees_none = [&](int col) { return ctx - rows + col / a.group + 1 <= 0; };
     for (int e = threadIdx.x; e < COLS * (HDP / 4); e += 64 * W) {
         const int col = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
         if (col >= columns || c >= a.mx.head_dim)
@@ -606,7 +608,7 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
                 store_through(ml, Mc, L);
         }
         else {
-            o *= L == 0.f ? 0.f : 1.f / L;
+            o = sees_none(col) ? f32x4{0.f, 0.f, 0.f, 0.f} : o * (1.f / L);
             store_four(a.out + line * a.mx.head_dim + c, o[0], o[1], o[2], o[3]);
         }
     }
@@ -618,7 +620,8 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
             continue;
         const int64_t line = (int64_t)(row0 + col / a.group) * a.n_heads + kvh * a.group + col % a.group;
         // (a row of a short context was not seen by the later chunks of a longer one: they hold nothing for it)
-        const float4 o = join_few<true>(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, parts, a.mx.head_dim);
+        const float4 o = join_few<true>(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, parts, a.mx.head_dim,
+                                        sees_none(col));
         store_four(a.out + line * a.mx.head_dim + c, o.x, o.y, o.z, o.w);
     }
 }
@@ -741,7 +744,7 @@ template <int KK> __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 
         return;
     const int64_t line = (int64_t)w.out_row * a.n_heads + w.out_head;
     float        *dst = a.out + line * a.mx.head_dim;
-    float         norm = w.l == 0.f ? 0.f : 1.f / w.l;
+    float         norm = w.limit == 0 ? 0.f : 1.f / w.l; // (no token seen: zeros; scores that are all -infinity: 0 / 0)
     if (a.chunks > 1) {
         dst  = a.ws_o + (line * a.chunks + chunk) * a.mx.head_dim;
         norm = 1.f;
@@ -765,8 +768,8 @@ template <int KK> __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 
         }
 }
 
-// How many chunks the line of a (row, head) has, 0 where nothing is to be joined.
-__device__ __forceinline__ int mx4_line_chunks(const Mx4AttnArgs &a, int64_t line)
+// How many chunks the line of a (row, head) has, 0 where nothing is to be joined; `empty`: its row sees no token.
+__device__ __forceinline__ int mx4_line_chunks(const Mx4AttnArgs &a, int64_t line, bool &empty)
 {
     const int row = (int)(line / a.n_heads);
     int       seq = row, rows = 1, row0 = row;
@@ -785,6 +788,7 @@ __device__ __forceinline__ int mx4_line_chunks(const Mx4AttnArgs &a, int64_t lin
         rows = mx4_rows(a, seq, row0);
     }
     const int ctx = mx4_context(a, seq), limit = max(ctx - rows + (row - row0) + 1, 0);
+    empty = limit == 0;
     if (a.whole_lines && min(max((ctx + a.chunk_tokens - 1) / a.chunk_tokens, 1), a.chunks) == 1)
         return 0; // (decode writes a sequence of one chunk straight to `out`)
     return min(max((limit + a.chunk_tokens - 1) / a.chunk_tokens, 1), a.chunks);
@@ -794,9 +798,10 @@ __device__ __forceinline__ int mx4_line_chunks(const Mx4AttnArgs &a, int64_t lin
 __global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_kernel(const Mx4AttnArgs a)
 {
     const int64_t line = blockIdx.x;
-    const int     n = mx4_line_chunks(a, line);
+    bool          empty = true;
+    const int     n = mx4_line_chunks(a, line, empty);
     if (n > 0)
-        join_chunks(a.ws_o + line * a.chunks * a.mx.head_dim, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim, a.out + line * a.mx.head_dim);
+        join_chunks(a.ws_o + line * a.chunks * a.mx.head_dim, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim, empty, a.out + line * a.mx.head_dim);
 }
 
 // Up to kJoinInside chunks (of many lines: a prefill's): a thread per four channels of a line.  (4088 rows of 8 heads of 80 channels, two
@@ -807,9 +812,10 @@ __global__ void __launch_bounds__(kJoinThreads) nvk_mx4_join_few_kernel(const Mx
     const int64_t  id = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x, line = id / quads;
     if (line >= lines)
         return;
-    const int n = mx4_line_chunks(a, line), c = (int)(id - line * quads) * 4;
+    bool      empty = true;
+    const int n = mx4_line_chunks(a, line, empty), c = (int)(id - line * quads) * 4;
     if (n > 0) {
-        const float4 o = join_few<false>(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim);
+        const float4 o = join_few<false>(a.ws_o + line * a.chunks * a.mx.head_dim + c, a.ws_ml + line * a.chunks * 2, n, a.mx.head_dim, empty);
         store_four(a.out + line * a.mx.head_dim + c, o.x, o.y, o.z, o.w);
     }
 }

@@ -763,9 +763,9 @@ __global__ void __launch_bounds__(64 * kSparseWaves, NV == 1 ? 4 : NV <= 4 || HG
             if (c == 0)
                 store_through(a.ws_ml + (line * a.chunks + chunk) * 2, Mh, L);
         }
-        else { // (L 0: x and y are 0 then, or no number)
-            a.out[line * hd + c]     = L == 0.f ? x : x / L;
-            a.out[line * hd + c + 1] = L == 0.f ? y : y / L;
+        else { // (no token: zeros; scores that are all -infinity: 0 / 0)
+            a.out[line * hd + c]     = ctx == 0 ? 0.f : x / L;
+            a.out[line * hd + c + 1] = ctx == 0 ? 0.f : y / L;
         }
     }
     if (parts == 1 || !a.arrivals || !arrived_last(a.arrivals + ((int64_t)seq * a.head_sets + set) * a.n_kv_heads + kvh, parts))
@@ -773,7 +773,7 @@ __global__ void __launch_bounds__(64 * kSparseWaves, NV == 1 ? 4 : NV <= 4 || HG
     for (int e = threadIdx.x; e < heads * (hd / 4); e += 64 * kSparseWaves) {
         const int64_t line = (int64_t)seq * a.n_heads + head0 + e / (hd / 4);
         const int     c = e % (hd / 4) * 4;
-        const float4  x = join_few<true>(a.ws_o + line * a.chunks * hd + c, a.ws_ml + line * a.chunks * 2, parts, hd);
+        const float4  x = join_few<true>(a.ws_o + line * a.chunks * hd + c, a.ws_ml + line * a.chunks * 2, parts, hd, false);
         store_four(a.out + line * hd + c, x.x, x.y, x.z, x.w);
     }
 }
@@ -786,7 +786,7 @@ __global__ void __launch_bounds__(kJoinThreads) nvk_sparse_join_kernel(const Spa
     const int     n = max((min(nb, a.top) + a.blocks_per_chunk - 1) / a.blocks_per_chunk, 1);
     if (n == 1)
         return; // (written straight to `out`)
-    join_chunks(a.ws_o + line * a.chunks * a.head_dim, a.ws_ml + line * a.chunks * 2, n, a.head_dim, a.out + line * a.head_dim);
+    join_chunks(a.ws_o + line * a.chunks * a.head_dim, a.ws_ml + line * a.chunks * 2, n, a.head_dim, false, a.out + line * a.head_dim);
 }
 
 } // namespace nvk

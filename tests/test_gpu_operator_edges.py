@@ -59,3 +59,44 @@ def test_rotation_alone_reads_positions_alone(cache, kind):
                 want[2] = 0  # (the row of padding: left alone here, returned as it came there)
             assert (out == want).all()
     rope.close()
+
+
+@pytest.mark.parametrize("case", [(16, 128, 90, 40), (16, 64, 3000, 40), (2, 32, 6000, 2000), (16, 256, 2000, 300)], ids=str)
+def test_scores_that_are_all_minus_infinity_are_no_answer(case):
+    """Every key holds -inf in a channel where the query is positive: 0 / 0, which is nvk_decode's answer too and not the zeros of an
+    empty context.  Written directly, joined by the attention kernel, joined by a kernel of its own; beside it a context of which one
+    token is left, and an empty one."""
+    bs, hd, n, top = case
+    rng = np.random.default_rng(74)
+    ctx = [n, n, 0]
+    tabs, blocks = oo.tables_for(ctx, bs, seed=75)
+    k, v = (rng.normal(size=(2, n, 1, hd)).astype(np.float32) for _ in range(2))
+    k[:, :, 0, 5] = -np.inf
+    k[1, n - 1, 0, 5] = 0.25
+    q = rng.normal(size=(3, 4, hd)).astype(np.float32)
+    q[:, :, 5] = 1.0
+    with nv.PagedKVPool(1, blocks, bs, 1, hd) as pool, nv.BlockIndex(pool) as index:
+        for s in range(2):
+            nv.norm_rope_append(pool, 0, None, None, k[s], v[s], tabs, np.arange(n), np.full(n, s))
+        index.update(0, tabs, [0, 0, 0], ctx)
+        got, _ = nv.sparse_decode(index, 0, q, tabs, ctx, top, 1, 1)
+        dense = nv.decode(pool, 0, q, np.where(tabs < 0, 0, tabs), ctx)
+    for out in (got, dense):
+        assert np.isnan(out[0]).all() and (out[1] == v[1, n - 1, 0]).all() and (out[2] == 0).all()
+
+
+@pytest.mark.parametrize("hd", [48, 128, 256])
+@pytest.mark.parametrize("n", [40, 1500, 9000])
+def test_scores_of_the_4_bit_cache_that_pass_fp32_are_no_answer(hd, n):
+    """Every score below the least fp32 number: 0 / 0 as above, decode and chunks of a few and of many rows; an empty context beside it."""
+    bs, rows = 16, (1, 3, 70)
+    tabs, blocks = oo.tables_for([n, 0], bs, seed=76)
+    v = np.random.default_rng(77).normal(size=(n, 1, hd)).astype(np.float32)
+    with nv.Mx4KVPool(1, blocks, bs, 1, hd) as pool:
+        nv.norm_rope_append(pool, 0, None, None, np.full((n, 1, hd), -1e38, np.float32), v, tabs, np.arange(n), np.zeros(n, np.int32))
+        q = np.full((80, 4, hd), 3e38, np.float32)
+        one = nv.mx4_decode(pool, 0, q[:2], tabs, [n, 0])
+        assert np.isnan(one[0]).all() and (one[1] == 0).all()
+        for r in rows:
+            if r <= n:
+                assert np.isnan(nv.mx4_prefill(pool, 0, q[:r], tabs, [r, 0], [n, 0])).all(), r
