@@ -163,8 +163,12 @@ template <bool SHARED> __global__ void __launch_bounds__(64 * kSparseWaves) nvk_
     *reinterpret_cast<float4 *>(to + a.head_dim) = hi;
 }
 
-// min(q, 0) for the least key element, max(q, 0) for the largest; a NaN stays one (fminf and fmaxf would make it 0)
-__device__ __forceinline__ float weight_of(float q, bool low) { return (low ? q > 0.f : q < 0.f) ? 0.f : q; }
+// min(q, 0) for the least key element, max(q, 0) for the largest; a NaN stays one (fminf and fmaxf would make it 0; comparisons
+// instead become branches around the loads: 1 x 8192 21.9 us for 18.8)
+__device__ __forceinline__ float weight_of(float q, bool low)
+{
+    return low ? __builtin_elementwise_minimum(q, 0.f) : __builtin_elementwise_maximum(q, 0.f);
+}
 
 // ---- scores ---------------------------------------------------------------------------------------------------------
 // With w = [min(q, 0) | max(q, 0)] a bound is the dot product of w with a block's [lo | hi], 2 head_dim contiguous floats.  It is
