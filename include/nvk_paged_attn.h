@@ -402,7 +402,8 @@ int nvk_bind_pool(nvk_pool *pool, int layer);
  *     NTK       the base becomes theta * factor^(rotary_dim / (rotary_dim - 2)); rotary_dim > 2
  *     YARN      a pair that turns t = original_len * f_i / 2 pi times over original_len keeps the share
  *               clamp((t - 1) / 31, 0, 1) of f_i, the rest is divided by factor; cos and sin are multiplied by
- *               0.1 ln(factor) + 1
+ *               0.1 ln(factor) + 1.  (The ramp is linear in t, with bounds 1 and 32.  Where a checkpoint's code ramps over the
+ *               pair's number i between two rounded numbers instead, pairs on the ramp turn at other angles.)
  *     factor >= 1; original_len > 0 for YARN; both ignored otherwise
  * The table is made on the host in 64 bits and does not change: it may be used from any stream of its device.
  * nvk_rope_destroy waits for the device. */
@@ -477,8 +478,8 @@ int nvk_mx4_pool_read_rows(nvk_mx4_pool *pool, int layer, int rows, const int *r
                            void *stream);
 
 /* Attention over the 4-bit cache: the arithmetic of nvk_decode / nvk_prefill (products exact, sums in fp32) over the
- * values it holds.  A context of 0 tokens gives a zero row.  Codes of tokens that a row does not see never reach it, also
- * where they are NaN.
+ * values it holds.  A context of 0 tokens gives a zero row, one whose scores are all -infinity NaN.  Codes of tokens that a row
+ * does not see never reach it, also where they are NaN.
  *   decode   q, out [num_seqs, n_heads, head_dim]; sequence s attends to ctx_lens[s] tokens
  *   prefill  q, out [total_rows, n_heads, head_dim]; sequence s has rows row_offsets[s] .. row_offsets[s+1] - 1 (an
  *            ascending list of num_seqs + 1, starting at 0), the newest of its ctx_lens[s] tokens, and each sees the tokens up
@@ -507,7 +508,7 @@ int nvk_mx4_prefill_device(nvk_mx4_pool *pool, int layer, int num_seqs, int n_he
  * counts as infinite).  For each (sequence, kv-head) a call reads
  *   the first first_blocks and the last last_blocks (at least 1: the newest block) of the context, and
  *   the best-scored others, equal scores lowest block first, up to top_blocks in all -- or every block, if there are no more.
- * Over those the result is nvk_decode's.  A context of 0 tokens gives a zero row.
+ * Over those the result is nvk_decode's.  A context of 0 tokens gives a zero row, one whose scores are all -infinity NaN.
  *
  * nvk_block_index_update: behind an append (any entry point that writes keys), brings the blocks that hold the tokens
  * [starts[s], ctx_lens[s]) of each sequence up to date, from all their tokens below ctx_lens[s].  The newest block is always

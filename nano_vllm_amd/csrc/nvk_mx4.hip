@@ -633,7 +633,9 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, KK == 8 ? 1 : PACK ? 3 : 2)
 // behind up to 4000 tokens, 32 heads of 128 channels: 433 us for 497 GFLOP of products, 1150 TFLOP/s, where a large library
 // product of bf16 reaches 1180 (each wave converting for itself: 684 us).  Two tiles of columns a wave halve the operands read but leave
 // room for two workgroups a CU and not three: as fast there, and 34 us instead of 26 for a prompt of 512 tokens, 135 instead of 100 for 2048.
-// With 64 channels and fewer the vector work of the softmax, which stays the same, is what bounds it.
+// With 64 channels and fewer neither pipe is full: a step is one chain (operands from LDS, score products, maximum, exponentials,
+// pieces, output products) between barriers.  (1157 rows of 16 heads of 48 channels: waves wait 48 % of their time, the vector pipe is
+// busy 34 % of the kernel's and the matrix pipe 16 %.)
 template <int KK> __global__ void __launch_bounds__(64 * kPrefillWaves, KK == 8 ? 1 : 3) nvk_mx4_prefill_kernel(const Mx4AttnArgs a)
 {
     using Wave = Mx4Wave<KK, false>;
@@ -856,8 +858,11 @@ Mx4Shape mx4_shape(const nvk_mx4_pool *pool, int num_seqs, int n_heads, int tota
     const long long per_cu = pool->kk == 8 ? 1 : s.prefill ? (pool->kk <= 2 ? 4 : 2) : s.pack ? 3 : 2, fit = per_cu * pool->num_cus;
     s.chunks = (int)std::max(1LL, std::min(fit / std::max(tasks, 1LL), (long long)max_ctx / (s.prefill ? 64 : 192)));
     // A prompt is cut where that saves more than the join costs: a step of 32 tokens takes about 1 us, the join 4 us and its reads and
-    // writes at 5 TB/s.  (128 rows of 32 heads of 128 channels: 10.4 us uncut, 13.6 in 2; 256: 15.5 and 19.1 in 4; 512: 25.7 and 29.5 in 2;
-    // 512 behind 512: 44.5 and 43.1 in 2.)
+    // writes at 5 TB/s.  (128 rows of 32 heads of 128 channels: 10.4 us uncut, 13.3 in 2; 256: 15.5 and 20.7 in 4; 512: 25.9 and 32.5 in 2;
+    // 512 behind 1536: 82.7 and 69.5 in 2.  16 heads of 48: 128 rows 7.8 and 10.7, 1157 rows 37.5 and 27.3, 128 behind 896 31.1 and 14.9.)
+    // The step is that of 128 channels.  Narrower ones are shorter, and the widest take about 2 us, so that the rule errs by up to a
+    // fifth where the two sides are close: 512 rows of 32 heads of 64 are cut (23.1 us, uncut 19.1), 256 and 512 of 16 heads of 256
+    // are not (26.6 and 45.7 us, cut 21.5 and 39.4).
     if (s.prefill && s.chunks > 1
         && (max_ctx - max_ctx / s.chunks) / 32 < 4 + (long long)total_rows * n_heads * pool->head_dim * s.chunks * 8 / 5000000)
         s.chunks = 1;
