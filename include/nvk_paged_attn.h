@@ -117,8 +117,7 @@ int nvk_pool_geometry(const nvk_pool *pool, int *out6);
 /* device base addresses of one layer's K and V slabs (for callers that fill
  * the pool with their own kernels, e.g. a fused RoPE+append) */
 int nvk_pool_layer_ptrs(const nvk_pool *pool, int layer, void **k_dev, void **v_dev);
-/* the pool's own HIP stream (hipStream_t; non-blocking).  It changes only when a model that owns the pool had a graph
- * recording invalidated from outside the library and took a fresh one (nvk_model_use_graphs): ask again then. */
+/* the pool's own HIP stream (hipStream_t; non-blocking), the same for the pool's life */
 int nvk_pool_stream(const nvk_pool *pool, void **stream);
 /* Counts the (re)allocations of the split-K workspace: launches recorded in a hipGraph hold its address. */
 long long nvk_pool_workspace_generation(const nvk_pool *pool);
@@ -685,10 +684,9 @@ int nvk_model_add_request(nvk_model *model, int request_id);
 int nvk_model_finish_request(nvk_model *model, int request_id); /* frees its KV blocks */
 int nvk_model_request_len(const nvk_model *model, int request_id);
 int nvk_model_free_blocks(const nvk_model *model);
-/* Pure decode steps replay a hipGraph of their ~12 launches per layer (captured again whenever the batch, the launch
- * shape or a scratch address changes); on by default, results are the same bits either way.  0 switches it off, which an
- * application has to do whose other threads use the null stream or wait for the device meanwhile: such a call is refused while a
- * stream records, and costs the recording and the pool's stream. */
+/* Pure decode steps replay a hipGraph of their ~12 launches per layer (recorded again whenever the batch, the launch
+ * shape or a scratch address changes); on by default, results are the same bits either way.  0 switches it off.  The graph is
+ * built without capturing a stream: what other threads do meanwhile, on the null stream too, neither disturbs it nor is refused. */
 int nvk_model_use_graphs(nvk_model *model, int on);
 /* A step of up to 16 decoding rows (the reference's own case is one: bound by launch latency, not by HBM) carries its norms between
  * the GEMVs instead of running them as kernels: the wo / w_down GEMVs add their product to the residual stream and

@@ -25,6 +25,7 @@
 
 #include "nvk_device_scope.h"
 #include "nvk_internal.h"
+#include "nvk_launch.h"
 
 #define HIP_TRY(expr)                                                                                                  \
     do {                                                                                                               \
@@ -359,8 +360,8 @@ int nvk_batch_begin_step(nvk_batch *b, const int *request_ids, int n, int n_head
             if (n_patches > 0)
                 HIP_TRY(hipMemcpyAsync(b->d_patches, b->h_patches, (size_t)3 * n_patches * sizeof(int),
                                        hipMemcpyHostToDevice, st));
-            hipLaunchKernelGGL(nvk_batch_advance_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, b->d_tables,
-                               b->max_blocks, b->d_pos, b->d_ctx, n, b->d_patches, n_patches);
+            nvk::launch(nvk_batch_advance_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, b->d_tables,
+                        b->max_blocks, b->d_pos, b->d_ctx, n, b->d_patches, n_patches);
             HIP_TRY(hipGetLastError());
             b->patch_steps++;
         }

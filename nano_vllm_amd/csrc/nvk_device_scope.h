@@ -11,15 +11,16 @@
 
 namespace nvk {
 
-// The recording gate.  A model records its decode step as a hipGraph (stream capture, nvk_model_step_chunks).  While a
+// The capture gate.  The library captures a stream of its own into a graph in one place (nvk_decode_bench_graph; a model's steps
+// are recorded without a capture: nvk_launch.h).  While a
 // stream of the process is capturing, ROCm 7.2 refuses work that other threads put on the null stream ("operation would
 // make the legacy stream depend on a capturing blocking stream" -- also for a non-blocking capturing stream, in
-// thread-local capture mode), refuses first-use work such as allocations, and any such call invalidates the recording and
-// leaves the recording stream unusable for good.  So the library keeps its own calls out of each other's way: every
+// thread-local capture mode), refuses first-use work such as allocations, and any such call invalidates the capture and
+// leaves the capturing stream unusable for good.  So the library keeps its own calls out of each other's way: every
 // entry point that touches the device holds the gate shared for its duration (the outermost one of a thread: entry
-// points call each other), a recording holds it alone, for the microseconds it takes.  Writers go first, so a recording
-// cannot starve behind threads that step back to back.  (What the APPLICATION does on other threads during a recording
-// is outside the library's reach: INTEGRATION.md.)
+// points call each other), a capture holds it alone, for the microseconds it takes.  Writers go first, so a capture
+// cannot starve behind threads that step back to back.  (What the application does on other threads meanwhile is outside
+// the library's reach.)
 class RecordGate
 {
     std::mutex              m_;
@@ -79,7 +80,7 @@ struct GateHold
     GateHold &operator=(const GateHold &) = delete;
 };
 
-// Held by the thread that records: gives up the thread's shared hold, takes the gate alone, and puts things back.
+// Held by the thread that captures: gives up the thread's shared hold, takes the gate alone, and puts things back.
 struct RecordAlone
 {
     RecordAlone()

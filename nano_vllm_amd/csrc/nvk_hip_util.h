@@ -8,6 +8,7 @@
 
 #include "nvk_device_scope.h"
 #include "nvk_internal.h"
+#include "nvk_launch.h"
 
 #define NVK_HIP_TRY(expr)                                                                                              \
     do {                                                                                                               \
@@ -26,9 +27,12 @@ inline bool grid_fits(long long groups, int threads) { return groups >= 0 && gro
 
 inline bool for_floats(const void *p) { return ((uintptr_t)p & 3) == 0; } // aligned to one
 
+// Whether launches on `stream` go into a graph and not to the device: captured by the caller, or recorded by this thread.
 inline bool stream_is_capturing(hipStream_t stream)
 {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (Recording::of(stream))
+        return true;
     return stream && hipStreamIsCapturing(stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
 }
 

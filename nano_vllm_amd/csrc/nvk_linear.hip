@@ -30,6 +30,7 @@
 #include "nvk_device_scope.h"
 #include "nvk_addr.hip.h"
 #include "nvk_internal.h"
+#include "nvk_launch.h"
 
 #define HIP_TRY(expr)                                                                                                  \
     do {                                                                                                               \
@@ -1342,7 +1343,7 @@ bool split_workspace(int device, int cus, hipStream_t st, size_t floats, size_t 
     SplitWorkspace &w = g_split_ws[SplitKey{device, st}];
     if (!w.part) {
         hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(st, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone) {
+        if (nvk::Recording::of(st) || hipStreamIsCapturing(st, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone) {
             (void)hipGetLastError();
             return false;
         }
@@ -1667,7 +1668,7 @@ int launch_linear(const float *in, int batch, int in_dim, const float *const *w,
         p.m_tiles = 1;
         const dim3 grid((unsigned)(glu ? (n[0] + 1) / 2 : tiles)), block(64 * nvk::kGemvWaves);
 #define NVK_GEMV_LAUNCH(M_, COLS_, ...) \
-    hipLaunchKernelGGL((nvk::nvk_gemv_kernel<M_, COLS_, NVK_GEMV_DEPTH, __VA_ARGS__>), grid, block, 0, st, p)
+    nvk::launch((nvk::nvk_gemv_kernel<M_, COLS_, NVK_GEMV_DEPTH, __VA_ARGS__>), grid, block, 0, st, p)
 #define NVK_GEMV_ROWS(COLS_, ...)                    \
     do {                                             \
         if (batch == 1)                              \
@@ -1717,9 +1718,9 @@ int launch_linear(const float *in, int batch, int in_dim, const float *const *w,
         if (rc16 != NVK_OK)                                                                                            \
             return rc16;                                                                                               \
         if (rope)                                                                                                      \
-            hipLaunchKernelGGL((nvk::nvk_gemm_skinny16_kernel<TN_, nvk::kSkinnyRope>), grid, block, lds16, st, p);     \
+            nvk::launch((nvk::nvk_gemm_skinny16_kernel<TN_, nvk::kSkinnyRope>), grid, block, lds16, st, p);            \
         else                                                                                                           \
-            hipLaunchKernelGGL((nvk::nvk_gemm_skinny16_kernel<TN_, nvk::kSkinnyPlain>), grid, block, lds16, st, p);    \
+            nvk::launch((nvk::nvk_gemm_skinny16_kernel<TN_, nvk::kSkinnyPlain>), grid, block, lds16, st, p);           \
     } while (0)
             if (tn == 1)
                 NVK_SK16(1);
@@ -1744,15 +1745,15 @@ int launch_linear(const float *in, int batch, int in_dim, const float *const *w,
                 return rc_lds;
             const dim3 grid((unsigned)wgs); // (several row tiles only with the RoPE epilogue)
             if (rope && t == 32)
-                hipLaunchKernelGGL((nvk_gemm_skinny_kernel<32, 1, 64, kSkinnyRope, false>), grid, block, lds, st, p);
+                nvk::launch((nvk_gemm_skinny_kernel<32, 1, 64, kSkinnyRope, false>), grid, block, lds, st, p);
             else if (rope && scale)
-                hipLaunchKernelGGL((nvk_gemm_skinny_kernel<16, 1, 64, kSkinnyRope, true>), grid, block, lds, st, p);
+                nvk::launch((nvk_gemm_skinny_kernel<16, 1, 64, kSkinnyRope, true>), grid, block, lds, st, p);
             else if (rope)
-                hipLaunchKernelGGL((nvk_gemm_skinny_kernel<16, 1, 64, kSkinnyRope, false>), grid, block, lds, st, p);
+                nvk::launch((nvk_gemm_skinny_kernel<16, 1, 64, kSkinnyRope, false>), grid, block, lds, st, p);
             else if (resid)
-                hipLaunchKernelGGL((nvk_gemm_skinny_kernel<16, 1, 64, kSkinnyResid, false>), grid, block, lds, st, p);
+                nvk::launch((nvk_gemm_skinny_kernel<16, 1, 64, kSkinnyResid, false>), grid, block, lds, st, p);
             else
-                hipLaunchKernelGGL((nvk_gemm_skinny_kernel<16, 1, 64, kSkinnyPlain, true>), grid, block, lds, st, p);
+                nvk::launch((nvk_gemm_skinny_kernel<16, 1, 64, kSkinnyPlain, true>), grid, block, lds, st, p);
             HIP_TRY(hipGetLastError());
             return NVK_OK;
         }
@@ -1778,8 +1779,8 @@ int launch_linear(const float *in, int batch, int in_dim, const float *const *w,
                 int rc_lds = opt_in_lds(fns, lds, device);
                 if (rc_lds != NVK_OK)
                     return rc_lds;
-                hipLaunchKernelGGL((nvk::nvk_gemm_skinny_kernel<16, 1, 64, nvk::kSkinnyPlain, false, true>),
-                                   dim3((unsigned)(wgs * sk_split)), block, lds, st, p);
+                nvk::launch((nvk::nvk_gemm_skinny_kernel<16, 1, 64, nvk::kSkinnyPlain, false, true>),
+                            dim3((unsigned)(wgs * sk_split)), block, lds, st, p);
                 HIP_TRY(hipGetLastError());
                 return NVK_OK;
             }
@@ -1795,17 +1796,17 @@ int launch_linear(const float *in, int batch, int in_dim, const float *const *w,
             return rc_lds;
         const dim3 grid((unsigned)wgs);
         if (t == 16 && tm == 2)
-            hipLaunchKernelGGL((nvk::nvk_gemm_skinny_kernel<16, 2, 32>), grid, block, lds, st, p);
+            nvk::launch((nvk::nvk_gemm_skinny_kernel<16, 2, 32>), grid, block, lds, st, p);
         else if (t == 16 && bk == 32)
-            hipLaunchKernelGGL((nvk::nvk_gemm_skinny_kernel<16, 1, 32>), grid, block, lds, st, p);
+            nvk::launch((nvk::nvk_gemm_skinny_kernel<16, 1, 32>), grid, block, lds, st, p);
         else if (t == 16)
-            hipLaunchKernelGGL((nvk::nvk_gemm_skinny_kernel<16, 1, 64>), grid, block, lds, st, p);
+            nvk::launch((nvk::nvk_gemm_skinny_kernel<16, 1, 64>), grid, block, lds, st, p);
         else if (tm == 1)
-            hipLaunchKernelGGL((nvk::nvk_gemm_skinny_kernel<32, 1, 64>), grid, block, lds, st, p);
+            nvk::launch((nvk::nvk_gemm_skinny_kernel<32, 1, 64>), grid, block, lds, st, p);
         else if (tm == 2)
-            hipLaunchKernelGGL((nvk::nvk_gemm_skinny_kernel<32, 2, 32>), grid, block, lds, st, p);
+            nvk::launch((nvk::nvk_gemm_skinny_kernel<32, 2, 32>), grid, block, lds, st, p);
         else
-            hipLaunchKernelGGL((nvk::nvk_gemm_skinny_kernel<32, 3, 32>), grid, block, lds, st, p);
+            nvk::launch((nvk::nvk_gemm_skinny_kernel<32, 3, 32>), grid, block, lds, st, p);
     }
     else {
         p.m_tiles = (batch + bm - 1) / bm;
@@ -1820,7 +1821,7 @@ int launch_linear(const float *in, int batch, int in_dim, const float *const *w,
             int rc_lds = opt_in_lds((const void *)nvk::nvk_gemm_nt_kernel<32, 128, 32, nvk::kNtStream, 1>, lds32, device);
             if (rc_lds != NVK_OK)
                 return rc_lds;
-            hipLaunchKernelGGL((nvk::nvk_gemm_nt_kernel<32, 128, 32, nvk::kNtStream, 1>), dim3((unsigned)grid), dim3(256), lds32, st, p);
+            nvk::launch((nvk::nvk_gemm_nt_kernel<32, 128, 32, nvk::kNtStream, 1>), dim3((unsigned)grid), dim3(256), lds32, st, p);
         }
         else if (stream128) { // (128 x 128 tiles, 32-steps)
             const size_t    lds128 = (size_t)2 * (128 + 128) * (32 + 4) * sizeof(float);
@@ -1828,35 +1829,35 @@ int launch_linear(const float *in, int batch, int in_dim, const float *const *w,
             int rc_lds = opt_in_lds((const void *)nvk::nvk_gemm_nt_kernel<128, 128, 32, nvk::kNtStream>, lds128, device);
             if (rc_lds != NVK_OK)
                 return rc_lds;
-            hipLaunchKernelGGL((nvk::nvk_gemm_nt_kernel<128, 128, 32, nvk::kNtStream>), dim3((unsigned)grid), dim3(256), lds128, st, p);
+            nvk::launch((nvk::nvk_gemm_nt_kernel<128, 128, 32, nvk::kNtStream>), dim3((unsigned)grid), dim3(256), lds128, st, p);
         }
         else if (stream_steps > 0) { // (64 x 64 tiles, 64-steps)
             const long long grid = (long long)p.ksplit * p.m_tiles;
             int rc_lds = opt_in_lds((const void *)nvk::nvk_gemm_nt_kernel<64, 64, 64, nvk::kNtStream>, lds, device);
             if (rc_lds != NVK_OK)
                 return rc_lds;
-            hipLaunchKernelGGL((nvk::nvk_gemm_nt_kernel<64, 64, 64, nvk::kNtStream>), dim3((unsigned)grid), dim3(256), lds, st, p);
+            nvk::launch((nvk::nvk_gemm_nt_kernel<64, 64, 64, nvk::kNtStream>), dim3((unsigned)grid), dim3(256), lds, st, p);
         }
         else if (split > 1) { // (64 x 64 tiles, 64-steps: the slices are whole numbers of them)
             int rc_lds = opt_in_lds((const void *)nvk::nvk_gemm_nt_kernel<64, 64, 64, nvk::kNtSplit>, lds, device);
             if (rc_lds != NVK_OK)
                 return rc_lds;
-            hipLaunchKernelGGL((nvk::nvk_gemm_nt_kernel<64, 64, 64, nvk::kNtSplit>), dim3((unsigned)wgs), dim3(256), lds, st, p);
+            nvk::launch((nvk::nvk_gemm_nt_kernel<64, 64, 64, nvk::kNtSplit>), dim3((unsigned)wgs), dim3(256), lds, st, p);
         }
         else if (bm == 128) {
             int rc_lds = opt_in_lds((const void *)nvk::nvk_gemm_nt_kernel<128, 128, 32>, lds, device);
             if (rc_lds != NVK_OK)
                 return rc_lds;
-            hipLaunchKernelGGL((nvk::nvk_gemm_nt_kernel<128, 128, 32>), dim3((unsigned)wgs), dim3(256), lds, st, p);
+            nvk::launch((nvk::nvk_gemm_nt_kernel<128, 128, 32>), dim3((unsigned)wgs), dim3(256), lds, st, p);
         }
         else if (bk == 64) {
             int rc_lds = opt_in_lds((const void *)nvk::nvk_gemm_nt_kernel<64, 64, 64>, lds, device);
             if (rc_lds != NVK_OK)
                 return rc_lds;
-            hipLaunchKernelGGL((nvk::nvk_gemm_nt_kernel<64, 64, 64>), dim3((unsigned)wgs), dim3(256), lds, st, p);
+            nvk::launch((nvk::nvk_gemm_nt_kernel<64, 64, 64>), dim3((unsigned)wgs), dim3(256), lds, st, p);
         }
         else
-            hipLaunchKernelGGL((nvk::nvk_gemm_nt_kernel<64, 64, 32>), dim3((unsigned)wgs), dim3(256), lds, st, p);
+            nvk::launch((nvk::nvk_gemm_nt_kernel<64, 64, 32>), dim3((unsigned)wgs), dim3(256), lds, st, p);
     }
     HIP_TRY(hipGetLastError());
     return NVK_OK;
@@ -1896,8 +1897,8 @@ int nvk::linked_gemv(const NormLink &link, bool glu, float *out_dev, const float
         if (rc != NVK_OK)
             return rc;
         const int64_t count = (int64_t)rows * out_dim;
-        hipLaunchKernelGGL(nvk::nvk_swiglu_kernel, dim3((unsigned)std::min<int64_t>(1024, (count + 255) / 256)), dim3(256), 0,
-                           (hipStream_t)stream, out_dev, scratch_dev, count);
+        nvk::launch(nvk::nvk_swiglu_kernel, dim3((unsigned)std::min<int64_t>(1024, (count + 255) / 256)), dim3(256), 0,
+                    (hipStream_t)stream, out_dev, scratch_dev, count);
         HIP_TRY(hipGetLastError());
         return NVK_OK;
     }
@@ -1953,8 +1954,8 @@ int nvk_batch_rms_norm_device(float *out_dev, const float *in_dev, const float *
     if (dim % 4 == 0 && (!aligned16(out_dev) || !aligned16(in_dev) || !aligned16(weight_dev)))
         return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_batch_rms_norm_device: pointers must be 16-byte aligned");
     NVK_SCOPE(device);
-    hipLaunchKernelGGL(nvk::nvk_rms_norm_kernel<false>, dim3((unsigned)batch_size), dim3(256), 0, (hipStream_t)stream,
-                       out_dev, const_cast<float *>(in_dev), (const float *)nullptr, weight_dev, dim, eps);
+    nvk::launch(nvk::nvk_rms_norm_kernel<false>, dim3((unsigned)batch_size), dim3(256), 0, (hipStream_t)stream,
+                out_dev, const_cast<float *>(in_dev), (const float *)nullptr, weight_dev, dim, eps);
     HIP_TRY(hipGetLastError());
     return NVK_OK;
 }
@@ -1971,8 +1972,8 @@ int nvk_batch_add_rms_norm_device(float *out_dev, float *x_dev, const float *add
     if (dim % 4 == 0 && (!aligned16(out_dev) || !aligned16(x_dev) || !aligned16(addend_dev) || !aligned16(weight_dev)))
         return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_batch_add_rms_norm_device: pointers must be 16-byte aligned");
     NVK_SCOPE(device);
-    hipLaunchKernelGGL(nvk::nvk_rms_norm_kernel<true>, dim3((unsigned)batch_size), dim3(256), 0, (hipStream_t)stream,
-                       out_dev, x_dev, addend_dev, weight_dev, dim, eps);
+    nvk::launch(nvk::nvk_rms_norm_kernel<true>, dim3((unsigned)batch_size), dim3(256), 0, (hipStream_t)stream,
+                out_dev, x_dev, addend_dev, weight_dev, dim, eps);
     HIP_TRY(hipGetLastError());
     return NVK_OK;
 }
@@ -2028,8 +2029,8 @@ int nvk_batch_swiglu_ffn_device(float *hb_dev, float *hb2_dev, const float *in_d
     if (rc != NVK_OK || gemv)
         return rc;
     const int64_t count = (int64_t)batch_size * hidden_dim;
-    hipLaunchKernelGGL(nvk::nvk_swiglu_kernel, dim3((unsigned)std::min<int64_t>(1024, (count + 255) / 256)), dim3(256), 0,
-                       (hipStream_t)stream, hb_dev, hb2_dev, count);
+    nvk::launch(nvk::nvk_swiglu_kernel, dim3((unsigned)std::min<int64_t>(1024, (count + 255) / 256)), dim3(256), 0,
+                (hipStream_t)stream, hb_dev, hb2_dev, count);
     HIP_TRY(hipGetLastError());
     return NVK_OK;
 }

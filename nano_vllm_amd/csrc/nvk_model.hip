@@ -26,6 +26,7 @@
 
 #include "nvk_device_scope.h"
 #include "nvk_internal.h"
+#include "nvk_launch.h"
 
 #define HIP_TRY(expr)                                                                                                  \
     do {                                                                                                               \
@@ -141,7 +142,7 @@ struct nvk_model
     int   *pinned = nullptr; // tokens | last rows | next tokens
     size_t pinned_ints = 0;
 
-    // The body of a pure decode step (embedding .. sampler, ~12 launches per layer) captured as a hipGraph and replayed
+    // The body of a pure decode step (embedding .. sampler, ~12 launches per layer) recorded as a hipGraph and replayed
     // while nothing it bakes in has changed: with few requests a step is hundreds of short dependent kernels and
     // the launch gaps, not the kernels, set its time.
     bool            use_graphs = true;
@@ -481,10 +482,10 @@ int nvk_model_step_chunks(nvk_model *m, const int *request_ids, const int *chunk
                         && D % 4 == 0 && Hd % 4 == 0 && QD % 4 == 0 && (R <= 2 || (V % 4 == 0 && m->head_dim % 4 == 0 && D % 16 == 0))
                         && R <= nvk::kFusedRowsMax && nvk::qkv_rope_append_ok(R, D, QD, m->n_kv_heads * m->head_dim, m->device);
     auto enqueue_linked = [&]() -> int {
-        hipError_t e1 = hipMemcpyAsync(m->tokens_dev, h_tok, (size_t)R * sizeof(int), hipMemcpyHostToDevice, st);
+        hipError_t e1 = nvk::copy_async(m->tokens_dev, h_tok, (size_t)R * sizeof(int), hipMemcpyHostToDevice, st);
         if (e1 != hipSuccess)
             return nvk::fail(NVK_ERR_HIP, "nvk_model_step_chunks: staging the tokens failed: %s", hipGetErrorString(e1));
-        hipLaunchKernelGGL(nvk_embed_kernel, dim3((unsigned)R), dim3(64), 0, st, m->x, m->tok_emb, m->tokens_dev, D, V);
+        nvk::launch(nvk_embed_kernel, dim3((unsigned)R), dim3(64), 0, st, m->x, m->tok_emb, m->tokens_dev, D, V);
         const int tiles_d = nvk::linked_ss_n(R, D);
         auto      produce = [&](const float *gain) { // x += in . w^T; xn = x * gain; xb = partial sums of x^2
             nvk::NormLink l;
@@ -514,21 +515,21 @@ int nvk_model_step_chunks(nvk_model *m, const int *request_ids, const int *chunk
             r2 = nvk::linked_gemv(consume, false, m->logits, m->xn, m->lm_head, nullptr, R, D, V, m->device, (void *)st);
         if (r2 != NVK_OK)
             return r2;
-        hipLaunchKernelGGL(nvk_argmax_kernel, dim3((unsigned)n), dim3(kArgmaxThreads), 0, st, m->next_dev, m->logits, V);
+        nvk::launch(nvk_argmax_kernel, dim3((unsigned)n), dim3(kArgmaxThreads), 0, st, m->next_dev, m->logits, V);
         hipError_t e2 = hipGetLastError();
         if (e2 == hipSuccess)
-            e2 = hipMemcpyAsync(h_next, m->next_dev, (size_t)n * sizeof(int), hipMemcpyDeviceToHost, st);
+            e2 = nvk::copy_async(h_next, m->next_dev, (size_t)n * sizeof(int), hipMemcpyDeviceToHost, st);
         if (e2 != hipSuccess)
             return nvk::fail(NVK_ERR_HIP, "nvk_model_step_chunks: %s", hipGetErrorString(e2));
         return NVK_OK;
     };
     auto enqueue_plain = [&]() -> int {
-        hipError_t e1 = hipMemcpyAsync(m->tokens_dev, h_tok, (size_t)R * sizeof(int), hipMemcpyHostToDevice, st);
+        hipError_t e1 = nvk::copy_async(m->tokens_dev, h_tok, (size_t)R * sizeof(int), hipMemcpyHostToDevice, st);
         if (e1 == hipSuccess)
-            e1 = hipMemcpyAsync(m->last_rows_dev, h_last, (size_t)n * sizeof(int), hipMemcpyHostToDevice, st);
+            e1 = nvk::copy_async(m->last_rows_dev, h_last, (size_t)n * sizeof(int), hipMemcpyHostToDevice, st);
         if (e1 != hipSuccess)
             return nvk::fail(NVK_ERR_HIP, "nvk_model_step_chunks: staging the tokens failed: %s", hipGetErrorString(e1));
-        hipLaunchKernelGGL(nvk_embed_kernel, dim3((unsigned)R), dim3(64), 0, st, m->x, m->tok_emb, m->tokens_dev, D, V);
+        nvk::launch(nvk_embed_kernel, dim3((unsigned)R), dim3(64), 0, st, m->x, m->tok_emb, m->tokens_dev, D, V);
         const unsigned ew_blocks = 1024;
         // The residual adds (model.hpp:227-228, 238-239) ride in the norm that follows them: after layer l's w_down the
         // sum x += xb and layer l + 1's attention norm are one kernel (its output feeds nvk_batch_layer_hidden already
@@ -558,23 +559,23 @@ int nvk_model_step_chunks(nvk_model *m, const int *request_ids, const int *chunk
             else if (R == n) // every row is a request's last row: the last add rides in the final norm (:238-239, :243)
                 r2 = nvk_batch_add_rms_norm_device(m->xl, m->x, m->xb, m->rms_final, n, D, m->rms_eps, m->device, (void *)st);
             else
-                hipLaunchKernelGGL(nvk_residual_kernel, dim3(ew_blocks), dim3(256), 0, st, m->x, m->xb, (int64_t)R * D / 4);
+                nvk::launch(nvk_residual_kernel, dim3(ew_blocks), dim3(256), 0, st, m->x, m->xb, (int64_t)R * D / 4);
         }
         if (r2 != NVK_OK)
             return r2;
         // final norm + classifier for each request's last row only (model.hpp:243-246), then the greedy sampler
         if (R != n) {
-            hipLaunchKernelGGL(nvk_take_rows_kernel, dim3((unsigned)n), dim3(64), 0, st, m->xl, m->x, m->last_rows_dev, D);
+            nvk::launch(nvk_take_rows_kernel, dim3((unsigned)n), dim3(64), 0, st, m->xl, m->x, m->last_rows_dev, D);
             r2 = nvk_batch_rms_norm_device(m->xl, m->xl, m->rms_final, n, D, m->rms_eps, m->device, (void *)st);
         }
         if (r2 == NVK_OK)
             r2 = nvk_batch_matmul_device(m->logits, m->xl, m->lm_head, n, D, V, m->device, (void *)st);
         if (r2 != NVK_OK)
             return r2;
-        hipLaunchKernelGGL(nvk_argmax_kernel, dim3((unsigned)n), dim3(kArgmaxThreads), 0, st, m->next_dev, m->logits, V);
+        nvk::launch(nvk_argmax_kernel, dim3((unsigned)n), dim3(kArgmaxThreads), 0, st, m->next_dev, m->logits, V);
         hipError_t e2 = hipGetLastError();
         if (e2 == hipSuccess)
-            e2 = hipMemcpyAsync(h_next, m->next_dev, (size_t)n * sizeof(int), hipMemcpyDeviceToHost, st);
+            e2 = nvk::copy_async(h_next, m->next_dev, (size_t)n * sizeof(int), hipMemcpyDeviceToHost, st);
         if (e2 != hipSuccess)
             return nvk::fail(NVK_ERR_HIP, "nvk_model_step_chunks: %s", hipGetErrorString(e2));
         return NVK_OK;
@@ -597,41 +598,27 @@ int nvk_model_step_chunks(nvk_model *m, const int *request_ids, const int *chunk
             const bool seen = std::memcmp(sig, m->graph_seen, sizeof sig) == 0;
             std::memcpy(m->graph_seen, sig, sizeof sig);
             if (stale && seen) {
-                // record the body (nothing runs while capturing); any refusal -- a first-use allocation inside an entry
-                // point, say -- ends the capture and this step runs directly
-                hipGraph_t graph = nullptr;
-                // (nobody else of the library on the device meanwhile: nvk_device_scope.h, the recording gate)
-                nvk::RecordAlone alone;
-                if (hipStreamBeginCapture(st, hipStreamCaptureModeThreadLocal) == hipSuccess) {
-                    const int  rb = enqueue_body();
-                    hipError_t ec = hipStreamEndCapture(st, &graph);
-                    if (rb == NVK_OK && ec == hipSuccess && graph
-                        && hipGraphInstantiate(&m->graph_exec, graph, nullptr, nullptr, 0) == hipSuccess)
-                    {
-                        std::memcpy(m->graph_sig, sig, sizeof sig);
-                        if (std::getenv("NVK_GRAPH_DEBUG"))
-                            std::fprintf(stderr, "nvk_model: recorded a %d-request decode step\n", n);
-                    }
-                    else {
-                        if (std::getenv("NVK_GRAPH_DEBUG"))
-                            std::fprintf(stderr, "nvk_model: capture refused (body %d: %s; end %s)\n", rb,
-                                         rb == NVK_OK ? "ok" : nvk_last_error(), hipGetErrorString(ec));
-                        m->graph_exec = nullptr;
-                        (void)hipGetLastError(); // clear the sticky capture error
-                        if (++m->graph_failures >= 4)
-                            m->use_graphs = false;
-                        // a recording invalidated from outside the library leaves the stream unusable: take a fresh one
-                        if (nvk::pool_renew_stream_if_stuck(m->pool) == NVK_OK) {
-                            void *fresh = nullptr;
-                            if (nvk_pool_stream(m->pool, &fresh) == NVK_OK && fresh != (void *)st) {
-                                st = m->stream = (hipStream_t)fresh;
-                                if (std::getenv("NVK_GRAPH_DEBUG"))
-                                    std::fprintf(stderr, "nvk_model: the recording was invalidated from outside; new stream\n");
-                            }
-                        }
-                    }
-                    if (graph)
-                        (void)hipGraphDestroy(graph);
+                // record the body (nothing runs meanwhile); any refusal -- a first-use allocation inside an entry point, say --
+                // ends the recording and this step runs directly
+                nvk::Recording recording(st);
+                const int      rb = enqueue_body();
+                hipGraphExec_t exec = nullptr;
+                hipError_t     ec = recording.finish(&exec);
+                if (rb == NVK_OK && ec == hipSuccess) {
+                    m->graph_exec = exec;
+                    std::memcpy(m->graph_sig, sig, sizeof sig);
+                    if (std::getenv("NVK_GRAPH_DEBUG"))
+                        std::fprintf(stderr, "nvk_model: recorded a %d-request decode step\n", n);
+                }
+                else {
+                    if (std::getenv("NVK_GRAPH_DEBUG"))
+                        std::fprintf(stderr, "nvk_model: recording refused (body %d: %s; end %s)\n", rb,
+                                     rb == NVK_OK ? "ok" : nvk_last_error(), hipGetErrorString(ec));
+                    if (exec)
+                        (void)hipGraphExecDestroy(exec);
+                    (void)hipGetLastError(); // clear the sticky error
+                    if (++m->graph_failures >= 4)
+                        m->use_graphs = false;
                 }
             }
             if (m->graph_exec) {

@@ -19,6 +19,7 @@
 #include "nvk_hip_util.h"
 #include "nvk_internal.h"
 #include "nvk_kernels.hip.h"
+#include "nvk_launch.h"
 
 #define NVK_VERSION_STRING "nvk_paged_attn 0.1.0 (gfx950)"
 
@@ -212,8 +213,7 @@ int ensure_pin(nvk_pool *pool, size_t bytes)
 // Refused before anything is touched, with the remedy in the message.
 int refuse_growth_under_capture(hipStream_t stream, const char *what)
 {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (stream && hipStreamIsCapturing(stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone)
+    if (nvk::stream_is_capturing(stream))
         return nvk::fail(NVK_ERR_INVALID_ARG,
                          "%s would have to grow while the stream is being captured: size it first, outside the capture "
                          "(nvk_pool_reserve_workspace, or one direct call of the same shape)", what);
@@ -476,16 +476,16 @@ template <int VPL, int QPK> hipError_t launch_decode_full(bool full, bool free_r
     if constexpr (has_free_kernel(VPL, QPK)) {
         if (free_run) { // several kv-head groups, or NVK_DECODE_FREE_RUNNING: see free_running
             if (full)
-                hipLaunchKernelGGL((nvk::nvk_decode_free_kernel<VPL, QPK, true>), grid, block, lds, stream, p);
+                nvk::launch((nvk::nvk_decode_free_kernel<VPL, QPK, true>), grid, block, lds, stream, p);
             else
-                hipLaunchKernelGGL((nvk::nvk_decode_free_kernel<VPL, QPK, false>), grid, block, lds, stream, p);
+                nvk::launch((nvk::nvk_decode_free_kernel<VPL, QPK, false>), grid, block, lds, stream, p);
             return hipGetLastError();
         }
     }
     if (full)
-        hipLaunchKernelGGL((nvk::nvk_decode_kernel<VPL, QPK, true>), grid, block, lds, stream, p);
+        nvk::launch((nvk::nvk_decode_kernel<VPL, QPK, true>), grid, block, lds, stream, p);
     else
-        hipLaunchKernelGGL((nvk::nvk_decode_kernel<VPL, QPK, false>), grid, block, lds, stream, p);
+        nvk::launch((nvk::nvk_decode_kernel<VPL, QPK, false>), grid, block, lds, stream, p);
     return hipGetLastError();
 }
 
@@ -512,35 +512,35 @@ hipError_t launch_decode(const LaunchShape &plan, dim3 grid, dim3 block, hipStre
 {
     if (plan.row_pairs) { // make_shape: vpl 2, full, at most 4 q-heads per wave, kv-head pairs
         switch (plan.qpk) {
-        case 4: hipLaunchKernelGGL((nvk::nvk_decode_rowpairs_kernel<4>), grid, block, plan.lds_bytes, stream, p); break;
-        case 3: hipLaunchKernelGGL((nvk::nvk_decode_rowpairs_kernel<3>), grid, block, plan.lds_bytes, stream, p); break;
-        case 2: hipLaunchKernelGGL((nvk::nvk_decode_rowpairs_kernel<2>), grid, block, plan.lds_bytes, stream, p); break;
-        default: hipLaunchKernelGGL((nvk::nvk_decode_rowpairs_kernel<1>), grid, block, plan.lds_bytes, stream, p); break;
+        case 4: nvk::launch((nvk::nvk_decode_rowpairs_kernel<4>), grid, block, plan.lds_bytes, stream, p); break;
+        case 3: nvk::launch((nvk::nvk_decode_rowpairs_kernel<3>), grid, block, plan.lds_bytes, stream, p); break;
+        case 2: nvk::launch((nvk::nvk_decode_rowpairs_kernel<2>), grid, block, plan.lds_bytes, stream, p); break;
+        default: nvk::launch((nvk::nvk_decode_rowpairs_kernel<1>), grid, block, plan.lds_bytes, stream, p); break;
         }
         return hipGetLastError();
     }
     if (plan.kpw == 2) { // make_shape: vpl 1, not full, at most 4 q-heads per wave
         switch (plan.qpk) {
-        case 4: hipLaunchKernelGGL((nvk::nvk_decode_pairs_kernel<4>), grid, block, plan.lds_bytes, stream, p); break;
-        case 3: hipLaunchKernelGGL((nvk::nvk_decode_pairs_kernel<3>), grid, block, plan.lds_bytes, stream, p); break;
-        case 2: hipLaunchKernelGGL((nvk::nvk_decode_pairs_kernel<2>), grid, block, plan.lds_bytes, stream, p); break;
-        default: hipLaunchKernelGGL((nvk::nvk_decode_pairs_kernel<1>), grid, block, plan.lds_bytes, stream, p); break;
+        case 4: nvk::launch((nvk::nvk_decode_pairs_kernel<4>), grid, block, plan.lds_bytes, stream, p); break;
+        case 3: nvk::launch((nvk::nvk_decode_pairs_kernel<3>), grid, block, plan.lds_bytes, stream, p); break;
+        case 2: nvk::launch((nvk::nvk_decode_pairs_kernel<2>), grid, block, plan.lds_bytes, stream, p); break;
+        default: nvk::launch((nvk::nvk_decode_pairs_kernel<1>), grid, block, plan.lds_bytes, stream, p); break;
         }
         return hipGetLastError();
     }
     if (plan.mfma) {
         if (plan.vpl == 1)
-            hipLaunchKernelGGL((nvk::nvk_decode_mfma_kernel<64>), grid, block, plan.lds_bytes, stream, p);
+            nvk::launch((nvk::nvk_decode_mfma_kernel<64>), grid, block, plan.lds_bytes, stream, p);
         else
-            hipLaunchKernelGGL((nvk::nvk_decode_mfma_kernel<128>), grid, block, plan.lds_bytes, stream, p);
+            nvk::launch((nvk::nvk_decode_mfma_kernel<128>), grid, block, plan.lds_bytes, stream, p);
         return hipGetLastError();
     }
     if (plan.wide) { // make_shape: vpl 2, full, at most 4 q-heads per wave, one kv-head group, no token parts
         switch (plan.qpk) {
-        case 4: hipLaunchKernelGGL((nvk::nvk_decode_wide_kernel<4>), grid, block, plan.lds_bytes, stream, p); break;
-        case 3: hipLaunchKernelGGL((nvk::nvk_decode_wide_kernel<3>), grid, block, plan.lds_bytes, stream, p); break;
-        case 2: hipLaunchKernelGGL((nvk::nvk_decode_wide_kernel<2>), grid, block, plan.lds_bytes, stream, p); break;
-        default: hipLaunchKernelGGL((nvk::nvk_decode_wide_kernel<1>), grid, block, plan.lds_bytes, stream, p); break;
+        case 4: nvk::launch((nvk::nvk_decode_wide_kernel<4>), grid, block, plan.lds_bytes, stream, p); break;
+        case 3: nvk::launch((nvk::nvk_decode_wide_kernel<3>), grid, block, plan.lds_bytes, stream, p); break;
+        case 2: nvk::launch((nvk::nvk_decode_wide_kernel<2>), grid, block, plan.lds_bytes, stream, p); break;
+        default: nvk::launch((nvk::nvk_decode_wide_kernel<1>), grid, block, plan.lds_bytes, stream, p); break;
         }
         return hipGetLastError();
     }
@@ -618,9 +618,9 @@ int plan_prepare(nvk_plan *plan, int num_seqs, int n_heads, const int *ctx_dev, 
 int plan_launch(nvk_plan *plan, const int *ctx_dev, hipStream_t stream)
 {
     if (!plan->direct && plan->num_seqs > 0) {
-        hipLaunchKernelGGL(nvk::nvk_plan_kernel, dim3(1), dim3(nvk::kPlanThreads), 0, stream, ctx_dev, plan->num_seqs,
-                           plan->shape.chunk_tokens, plan->shape.max_chunks, plan->items, plan->counters,
-                           plan->counters + 1, plan->shape.chunk_skew);
+        nvk::launch(nvk::nvk_plan_kernel, dim3(1), dim3(nvk::kPlanThreads), 0, stream, ctx_dev, plan->num_seqs,
+                    plan->shape.chunk_tokens, plan->shape.max_chunks, plan->items, plan->counters,
+                    plan->counters + 1, plan->shape.chunk_skew);
         HIP_TRY(hipGetLastError());
     }
     plan->built = true;
@@ -773,16 +773,16 @@ int enqueue_planned(nvk_pool *pool, int layer, const nvk_plan *plan, const float
         if (!sh.force_serial_merge && sh.max_chunks >= 4 && sh.max_chunks <= nvk::kMergeWideMaxChunks && n_heads <= 65535
             && (long long)plan->num_seqs * n_heads <= NVK_MERGE_WIDE_ROWS) {
             const dim3 mgrid((unsigned)plan->num_seqs, (unsigned)n_heads);
-            hipLaunchKernelGGL(nvk::nvk_merge_wide_kernel, mgrid, dim3(256), 0, stream, ws.ws_o, ws.ws_ml,
-                               seq_chunks, plan->ctx_lens_dev, plan->uniform_ctx, sh.chunk_tokens, out_dev, n_heads,
-                               pool->head_dim, sh.max_chunks);
+            nvk::launch(nvk::nvk_merge_wide_kernel, mgrid, dim3(256), 0, stream, ws.ws_o, ws.ws_ml,
+                        seq_chunks, plan->ctx_lens_dev, plan->uniform_ctx, sh.chunk_tokens, out_dev, n_heads,
+                        pool->head_dim, sh.max_chunks);
         }
         else {
             const int  vecs = n_heads * (pool->head_dim / 4);
             const dim3 mgrid((unsigned)plan->num_seqs, (unsigned)((vecs + 255) / 256));
-            hipLaunchKernelGGL(nvk::nvk_merge_kernel, mgrid, dim3(256), 0, stream, ws.ws_o, ws.ws_ml, seq_chunks,
-                               plan->ctx_lens_dev, plan->uniform_ctx, sh.chunk_tokens, out_dev, n_heads, pool->head_dim,
-                               sh.max_chunks);
+            nvk::launch(nvk::nvk_merge_kernel, mgrid, dim3(256), 0, stream, ws.ws_o, ws.ws_ml, seq_chunks,
+                        plan->ctx_lens_dev, plan->uniform_ctx, sh.chunk_tokens, out_dev, n_heads, pool->head_dim,
+                        sh.max_chunks);
         }
         HIP_TRY(hipGetLastError());
     }
@@ -1440,9 +1440,9 @@ int nvk_pool_append_batch(nvk_pool *pool, int layer, int num_seqs, const float *
     else if (ptr_kind != NVK_PTR_DEVICE) {
         return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_pool_append_batch: ptr_kind %d", ptr_kind);
     }
-    hipLaunchKernelGGL(nvk::nvk_append_kernel, dim3((unsigned)num_seqs), dim3(256), 0, pool->stream, pool->k_layer(layer),
-                       pool->v_layer(layer), dk, dv, dt, max_blocks, dp, pool->num_blocks, pool->block_size,
-                       pool->bs_magic, row);
+    nvk::launch(nvk::nvk_append_kernel, dim3((unsigned)num_seqs), dim3(256), 0, pool->stream, pool->k_layer(layer),
+                pool->v_layer(layer), dk, dv, dt, max_blocks, dp, pool->num_blocks, pool->block_size,
+                pool->bs_magic, row);
     HIP_TRY(hipGetLastError());
     if (ptr_kind == NVK_PTR_HOST)
         HIP_TRY(hipStreamSynchronize(pool->stream));
@@ -1514,10 +1514,10 @@ int nvk_pool_rope_append_batch(nvk_pool *pool, int layer, int num_seqs, int n_he
     else if (ptr_kind != NVK_PTR_DEVICE) {
         return nvk::fail(NVK_ERR_INVALID_ARG, "nvk_pool_rope_append_batch: ptr_kind %d", ptr_kind);
     }
-    hipLaunchKernelGGL(nvk::nvk_rope_append_kernel, dim3((unsigned)num_seqs), dim3(256), (size_t)half * sizeof(float2), st,
-                       pool->k_layer(layer), pool->v_layer(layer), dq, dk, dv, dt, (const int *)nullptr, max_blocks, dp,
-                       rotate ? pool->rope_inv_freq : (const float *)nullptr,
-                       pool->num_blocks, pool->block_size, pool->bs_magic, n_heads, pool->n_kv_heads, hd);
+    nvk::launch(nvk::nvk_rope_append_kernel, dim3((unsigned)num_seqs), dim3(256), (size_t)half * sizeof(float2), st,
+                pool->k_layer(layer), pool->v_layer(layer), dq, dk, dv, dt, (const int *)nullptr, max_blocks, dp,
+                rotate ? pool->rope_inv_freq : (const float *)nullptr,
+                pool->num_blocks, pool->block_size, pool->bs_magic, n_heads, pool->n_kv_heads, hd);
     HIP_TRY(hipGetLastError());
     if (ptr_kind == NVK_PTR_HOST) {
         if (rotate)
@@ -1528,31 +1528,6 @@ int nvk_pool_rope_append_batch(nvk_pool *pool, int layer, int num_seqs, int n_he
 }
 
 } // extern "C"
-
-int nvk::pool_renew_stream_if_stuck(nvk_pool *pool)
-{
-    if (!pool)
-        return nvk::fail(NVK_ERR_INVALID_ARG, "pool_renew_stream_if_stuck: null pool");
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(pool->stream, &status) == hipSuccess && status == hipStreamCaptureStatusNone)
-        return NVK_OK;
-    (void)hipGetLastError();
-    NVK_SCOPE(pool->device);
-    hipStream_t fresh = nullptr;
-    HIP_TRY(hipStreamCreateWithFlags(&fresh, hipStreamNonBlocking));
-    // (what was enqueued before the recording began has to be over before anything follows it on the new stream; the old
-    //  stream itself can no longer be waited for)
-    hipError_t e = hipDeviceSynchronize();
-    if (e != hipSuccess) {
-        (void)hipStreamDestroy(fresh);
-        return nvk::fail(NVK_ERR_HIP, "pool_renew_stream_if_stuck: hipDeviceSynchronize failed: %s", hipGetErrorString(e));
-    }
-    (void)hipStreamDestroy(pool->stream);
-    (void)hipGetLastError();
-    pool->stream = fresh;
-    return NVK_OK;
-}
-
 
 int nvk::pool_rope_append_target(nvk_pool *pool, int layer, float rope_theta, const int *block_tables_dev, int max_blocks,
                                  const int *positions_dev, RopeAppendTarget *out)
@@ -1641,9 +1616,9 @@ int nvk_pool_gather(nvk_pool *pool, int layer, const int *block_table, int num_t
     float *dv = (float *)(pool->stage + out_a);
     int   *dt = (int *)(pool->stage + 2 * out_a);
     HIP_TRY(hipMemcpyAsync(dt, block_table, tab_b, hipMemcpyHostToDevice, pool->stream));
-    hipLaunchKernelGGL(nvk::nvk_gather_kernel, dim3((unsigned)num_tokens), dim3(64), 0, pool->stream, pool->k_layer(layer),
-                       pool->v_layer(layer), dt, num_tokens, kv_head, pool->num_blocks, pool->block_size, pool->bs_magic,
-                       pool->n_kv_heads, pool->head_dim, dk, dv);
+    nvk::launch(nvk::nvk_gather_kernel, dim3((unsigned)num_tokens), dim3(64), 0, pool->stream, pool->k_layer(layer),
+                pool->v_layer(layer), dt, num_tokens, kv_head, pool->num_blocks, pool->block_size, pool->bs_magic,
+                pool->n_kv_heads, pool->head_dim, dk, dv);
     HIP_TRY(hipGetLastError());
     HIP_TRY(hipMemcpyAsync(k_out, dk, out_b, hipMemcpyDeviceToHost, pool->stream));
     HIP_TRY(hipMemcpyAsync(v_out, dv, out_b, hipMemcpyDeviceToHost, pool->stream));
@@ -1658,11 +1633,11 @@ int nvk_pool_fill_uniform(nvk_pool *pool, int layer, uint64_t seed_k, uint64_t s
         return rc;
     NVK_SCOPE(pool->device);
     const dim3  grid((unsigned)(pool->num_cus * 8)), block(256);
-    hipLaunchKernelGGL(nvk::nvk_fill_kernel, grid, block, 0, pool->stream, pool->k_layer(layer), seed_k,
-                       (uint64_t)pool->layer_floats);
+    nvk::launch(nvk::nvk_fill_kernel, grid, block, 0, pool->stream, pool->k_layer(layer), seed_k,
+                (uint64_t)pool->layer_floats);
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(nvk::nvk_fill_kernel, grid, block, 0, pool->stream, pool->v_layer(layer), seed_v,
-                       (uint64_t)pool->layer_floats);
+    nvk::launch(nvk::nvk_fill_kernel, grid, block, 0, pool->stream, pool->v_layer(layer), seed_v,
+                (uint64_t)pool->layer_floats);
     HIP_TRY(hipGetLastError());
     HIP_TRY(hipStreamSynchronize(pool->stream));
     return NVK_OK;
@@ -2261,10 +2236,10 @@ int nvk_pool_rope_append_chunks(nvk_pool *pool, int layer, int num_seqs, int n_h
         HIP_TRY(hipMemcpyAsync((void *)dt, block_tables, tab_b, hipMemcpyHostToDevice, st));
     }
     // one workgroup per new token: batch_rope (batch_ops.hpp:25-56) and the append loop (model_chunked.hpp:82-94)
-    hipLaunchKernelGGL(nvk::nvk_rope_append_kernel, dim3((unsigned)rows.total_q), dim3(256), (size_t)half * sizeof(float2),
-                       st, pool->k_layer(layer), pool->v_layer(layer), dq, dk, dv, dt, rows.row_seq, max_blocks,
-                       rows.row_pos, rotate ? pool->rope_inv_freq : (const float *)nullptr, pool->num_blocks,
-                       pool->block_size, pool->bs_magic, n_heads, pool->n_kv_heads, hd);
+    nvk::launch(nvk::nvk_rope_append_kernel, dim3((unsigned)rows.total_q), dim3(256), (size_t)half * sizeof(float2),
+                st, pool->k_layer(layer), pool->v_layer(layer), dq, dk, dv, dt, rows.row_seq, max_blocks,
+                rows.row_pos, rotate ? pool->rope_inv_freq : (const float *)nullptr, pool->num_blocks,
+                pool->block_size, pool->bs_magic, n_heads, pool->n_kv_heads, hd);
     HIP_TRY(hipGetLastError());
     if (ptr_kind == NVK_PTR_HOST) {
         if (rotate)
@@ -2338,15 +2313,15 @@ int nvk_prefill_device(nvk_pool *pool, int layer, int num_seqs, int n_heads, con
                              work.n_items, grid_y);
         const dim3   grid((unsigned)(work.n_items * grid_y));
         if (hdp == 64)
-            hipLaunchKernelGGL((nvk::nvk_prefill_kernel<64>), grid, dim3(256), lds, st, pp);
+            nvk::launch((nvk::nvk_prefill_kernel<64>), grid, dim3(256), lds, st, pp);
         else
-            hipLaunchKernelGGL((nvk::nvk_prefill_kernel<128>), grid, dim3(256), lds, st, pp);
+            nvk::launch((nvk::nvk_prefill_kernel<128>), grid, dim3(256), lds, st, pp);
         HIP_TRY(hipGetLastError());
         if (work.max_parts > 1) { // combine the key-range partials per query row (rows with one part are done)
             const int  vecs = n_heads * (pool->head_dim / 4);
             const dim3 mgrid((unsigned)work.total_q, (unsigned)((vecs + 255) / 256));
-            hipLaunchKernelGGL(nvk::nvk_merge_kernel, mgrid, dim3(256), 0, st, pool->ws_o, pool->ws_ml, work.row_parts_dev,
-                               (const int *)nullptr, 0, 1, out_dev, n_heads, pool->head_dim, work.max_parts);
+            nvk::launch(nvk::nvk_merge_kernel, mgrid, dim3(256), 0, st, pool->ws_o, pool->ws_ml, work.row_parts_dev,
+                        (const int *)nullptr, 0, 1, out_dev, n_heads, pool->head_dim, work.max_parts);
             HIP_TRY(hipGetLastError());
         }
         return NVK_OK;
